@@ -34,7 +34,7 @@
 extern "C" {
 #endif
 
-#define PTX_ABI_VERSION 7
+#define PTX_ABI_VERSION 8
 #define PTX_API __attribute__((visibility("default")))
 
 /*
@@ -49,8 +49,9 @@ extern "C" {
  * update; the LayerNorm entry points refuse it.
  */
 enum ptx_dtype { PTX_F32 = 0, PTX_BF16 = 1, PTX_MIXED = 2, PTX_F16 = 3 };
-/* PTX_F16 (IEEE half) is taken by the LayerNorm entry points only, which dispatch on float /
- * Half / BFloat16 like the reference's kernel (layer_norm_cuda_kernel.cu:304-330). */
+/* PTX_F16 (IEEE half) is taken by the LayerNorm entry points, which dispatch on float /
+ * Half / BFloat16 like the reference's kernel (layer_norm_cuda_kernel.cu:304-330), and by the
+ * dropout and relative position bias entry points. */
 
 enum ptx_status {
   PTX_OK = 0,
@@ -567,6 +568,89 @@ PTX_API int ptx_single_stage_run(const ptx_single_stage* stage, void* stream);
  * reported against (bench.py, `hbm_ceiling`); src and dst must not overlap.
  */
 PTX_API int ptx_hbm_stream(const void* src, void* dst, int64_t bytes, int nontemporal, void* stream);
+
+/*
+ * Dropout in front of a residual sum (the reference's dropout_add_rowwise, protenix/model/modules/
+ * fused_ops.py:40-113, whose mask is shared along one axis of the pair tensor):
+ *   out = residual + m x        m = 1 / (1 - p) where the element is kept, else 0
+ *   x          [rows][cols], x_dtype
+ *   residual   [rows][cols], stream_dtype, or NULL: none
+ *   out        [rows][cols], stream_dtype; may alias residual, or x where the types agree
+ * Rows are [outer][shared][inner]; the rows of one (outer, inner) have the same mask row r =
+ * outer * inner + inner index (shared = 1: every row its own).  The mask is not stored: it comes
+ * from Philox4x32-10 with the seed as key.  Columns in blocks of 8: block k of mask row r takes its
+ * 16-bit halves, low half first, from the counter (k, r, 0, 0) and 16 bits below them from (k, r, 0, 1); an
+ * element is kept where the 32-bit number is at least round(p 2^32).  It depends on the seed, the
+ * mask row and the column only.  p = 0: no dropout; p = 1: nothing is kept.
+ *   seed       the seed; or seed_ptr: one 64-bit whole number in device memory, read by the launch
+ * The gradient of x is the same call on the gradient of out, without a residual; the residual's is
+ * the gradient of out itself.  Types: x and stream of one of PTX_F32, PTX_BF16, PTX_F16, or one
+ * of them PTX_F32.  rows < 2^31, rows a multiple of shared * inner.
+ */
+PTX_API int ptx_dropout_add(const void* x, const void* residual, void* out, int64_t rows, int cols, int64_t shared,
+                            int64_t inner, double p, uint64_t seed, const int64_t* seed_ptr, int x_dtype,
+                            int stream_dtype, void* stream);
+
+/*
+ * The same sum and the LayerNorm of it that the next update reads, in one pass:
+ *   h = residual + m x,   y = (h - mean) rstd gamma + beta
+ *   y            [rows][cols], x_dtype;  h [rows][cols], stream_dtype (x_dtype where there is no residual)
+ *   gamma, beta  [cols], param_dtype, either may be NULL
+ *   mean, rstd   fp32 [rows], each may be NULL: of the sum before it is rounded to h
+ * x_dtype = stream_dtype, or 16-bit x beside an fp32 stream; at most 32768 columns.  y may alias x, h the residual;
+ * every other pair must not overlap.
+ */
+PTX_API int ptx_dropout_add_layernorm_fwd(const void* x, const void* residual, const void* gamma, const void* beta,
+                                          void* y, void* h, float* mean, float* rstd, int64_t rows, int cols,
+                                          int64_t shared, int64_t inner, double p, float eps, uint64_t seed,
+                                          const int64_t* seed_ptr, int x_dtype, int stream_dtype, int param_dtype,
+                                          void* stream);
+/*
+ * Its gradients, from dy (x_dtype) and dh (stream_dtype; either may be NULL: zero).  dx (x_dtype), dresidual (stream_dtype),
+ * dgamma and dbeta (param_dtype) are written where given; dgamma / dbeta need the workspace (uninitialised fp32).
+ * h: the forward's where stream_dtype is PTX_F32.  NULL: h is formed again from x and the residual (NULL: none), as it must be
+ * for 16-bit streams, whose rounded h would cost dgamma its accuracy.  No atomics: the sums' order is fixed.
+ */
+PTX_API int64_t ptx_dropout_add_layernorm_bwd_workspace_elems(int64_t rows, int cols);
+PTX_API int ptx_dropout_add_layernorm_bwd(const void* dy, const void* dh, const void* x, const void* residual,
+                                          const void* h, const float* mean, const float* rstd, const void* gamma,
+                                          void* dx, void* dresidual, void* dgamma, void* dbeta, float* workspace,
+                                          int64_t rows, int cols, int64_t shared, int64_t inner, double p,
+                                          uint64_t seed, const int64_t* seed_ptr, int x_dtype, int stream_dtype,
+                                          int param_dtype, void* stream);
+
+/*
+ * Learned bias by buckets of relative position:
+ *   out[b][h][i][j] = table[bucket(k_pos[b][j] - q_pos[b][i])][h]
+ * The bucket of a difference d with n = min(|d|, max_distance): with s the last of `side` buckets whose start is
+ * at most n, neg_base + neg_step s for d <= 0 and pos_base + pos_step s for d > 0; pairs whose groups differ have bucket
+ * `count` (a further row of the table, there exactly when groups are given).
+ */
+#define PTX_RELATIVE_BUCKETS_MAX 255    /* largest count */
+#define PTX_RELATIVE_DISTANCE_MAX 8192  /* largest max_distance */
+typedef struct ptx_relative_buckets {
+  int32_t max_distance, count, side;
+  int32_t neg_base, neg_step, pos_base, pos_step;
+  uint16_t starts[256];                 /* [side], ascending, starts[0] = 0 */
+} ptx_relative_buckets;
+/*
+ *   buckets      in host memory, read before the call returns
+ *   table        [count (+ 1)][heads], table_dtype
+ *   out          [batch][heads][q_len][k_len], out_dtype: the table's values rounded once
+ *   q_pos, k_pos [batch][q_len], [batch][k_len]; or NULL: q_first + i, k_first + j in every batch
+ *   q_group, k_group  likewise; both or neither
+ */
+PTX_API int ptx_relative_bias_fwd(const ptx_relative_buckets* buckets, const void* table, void* out, int batch,
+                                  int heads, int q_len, int k_len, const int64_t* q_pos, const int64_t* k_pos,
+                                  int64_t q_first, int64_t k_first, const int64_t* q_group, const int64_t* k_group,
+                                  int table_dtype, int out_dtype, void* stream);
+/* dtable [count (+ 1)][heads], table_dtype: sums of dout (out_dtype) over all elements of a bucket, in fp32 and a fixed order.
+ * workspace: ptx_relative_bias_bwd_workspace_elems(heads, rows of the table) fp32 elements, uninitialised. */
+PTX_API int64_t ptx_relative_bias_bwd_workspace_elems(int heads, int table_rows);
+PTX_API int ptx_relative_bias_bwd(const ptx_relative_buckets* buckets, const void* dout, void* dtable, float* workspace,
+                                  int batch, int heads, int q_len, int k_len, const int64_t* q_pos,
+                                  const int64_t* k_pos, int64_t q_first, int64_t k_first, const int64_t* q_group,
+                                  const int64_t* k_group, int table_dtype, int out_dtype, void* stream);
 
 #ifdef __cplusplus
 }

@@ -3,10 +3,12 @@ TriangleMultiplication*, TriangleAttention, LayerNorm, Transition,
 AttentionPairBias, PairformerBlock and PairformerStack, backed by hand-written
 gfx950 kernels in libprotenix_amd.so (C ABI: include/protenix_amd.h)."""
 
+from .dropout import dropout_add, dropout_add_layer_norm
 from .graph import Graphed
 from .layer_norm import FusedLayerNorm, LayerNorm
 from .pairformer import PairformerBlock, PairformerStack
 from .primitives import Linear, LinearNoBias, Transition
+from .relative_bias import RelativeBuckets, RelativePositionBias, relative_position_bias
 from .transformer import AttentionPairBias
 from .tri_attention import TriAttentionFunction, tri_attention, tri_attention_forward
 from .triangular import (
@@ -31,4 +33,5 @@ __all__ = [
     "TriangleMultiplicationIncoming", "TriangleMultiplicationOutgoing",
     "TriangleMultiplicativeUpdate", "kernel_triangular_mult", "triangle_multiplicative_update",
     "TriAttentionFunction", "tri_attention", "tri_attention_forward",
+    "dropout_add", "dropout_add_layer_norm", "RelativeBuckets", "RelativePositionBias", "relative_position_bias",
 ]

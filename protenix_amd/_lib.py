@@ -14,12 +14,21 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libprotenix_amd.so")
 
 PTX_F32, PTX_BF16, PTX_MIXED, PTX_F16 = 0, 1, 2, 3
-ABI_VERSION = 7
+ABI_VERSION = 8
 
 _p = ctypes.c_void_p
 _i = ctypes.c_int
 _l = ctypes.c_int64
 _f = ctypes.c_float
+_d = ctypes.c_double
+_u = ctypes.c_uint64
+
+
+class RelativeBucketsStruct(ctypes.Structure):
+    """ptx_relative_buckets"""
+    _fields_ = [(n, ctypes.c_int32) for n in ("max_distance", "count", "side", "neg_base", "neg_step", "pos_base", "pos_step")
+                ] + [("starts", ctypes.c_uint16 * 256)]
+
 
 # name -> (restype, argtypes); mirrors include/protenix_amd.h one to one
 SIGNATURES = {
@@ -87,6 +96,13 @@ SIGNATURES = {
     "ptx_swiglu_fwd": (_i, [_p, _p, _p, _p, _i, _i, _i, _i, _p]),
     "ptx_single_attention_fwd": (_i, [_p, _p, _p, _p, _p, _i, _p, _i, _i, _i, _l, _l, _l, _f, _i, _p]),
     "ptx_pair_bias_fwd": (_i, [_p] * 5 + [_i, _i, _i, _i, _f, _i, _p]),
+    "ptx_dropout_add": (_i, [_p, _p, _p, _l, _i, _l, _l, _d, _u, _p, _i, _i, _p]),
+    "ptx_dropout_add_layernorm_fwd": (_i, [_p] * 8 + [_l, _i, _l, _l, _d, _f, _u, _p, _i, _i, _i, _p]),
+    "ptx_dropout_add_layernorm_bwd_workspace_elems": (_l, [_l, _i]),
+    "ptx_dropout_add_layernorm_bwd": (_i, [_p] * 13 + [_l, _i, _l, _l, _d, _u, _p, _i, _i, _i, _p]),
+    "ptx_relative_bias_fwd": (_i, [_p, _p, _p, _i, _i, _i, _i, _p, _p, _l, _l, _p, _p, _i, _i, _p]),
+    "ptx_relative_bias_bwd_workspace_elems": (_l, [_i, _i]),
+    "ptx_relative_bias_bwd": (_i, [_p, _p, _p, _p, _i, _i, _i, _i, _p, _p, _l, _l, _p, _p, _i, _i, _p]),
     "ptx_hbm_stream": (_i, [_p, _p, _l, _i, _p]),
 }
 

@@ -1,6 +1,7 @@
 // extern "C" boundary of libprotenix_amd.so: argument validation, dtype
 // dispatch, launch-error capture.  See include/protenix_amd.h for the contract.
 #include <algorithm>
+#include <math.h>
 #include <stdarg.h>
 #include <stdio.h>
 
@@ -8,6 +9,7 @@
 
 #include "../../include/protenix_amd.h"
 #include "common.h"
+#include "dropout.h"
 #include "kernels.h"
 
 namespace {
@@ -1116,6 +1118,172 @@ PTX_API int ptx_hbm_stream(const void* src, void* dst, int64_t bytes, int nontem
               "hbm_stream: pointers must be 16-byte aligned");
   ptx::hbm_stream(src, dst, bytes, nontemporal, (hipStream_t)stream);
   return after_launch("hbm_stream");
+}
+
+// ---- residual dropout ---------------------------------------------------------------------------
+static int dropout_of(ptx::Dropout& d, const char* what, int64_t rows, int cols, int64_t shared, int64_t inner, double p, uint64_t seed,
+                      const int64_t* seed_ptr) {
+  PTX_REQUIRE(rows >= 0 && cols > 0, PTX_ERR_BAD_ARG, "%s: rows=%lld cols=%d", what, (long long)rows, cols);
+  PTX_REQUIRE(rows < ((int64_t)1 << 31), PTX_ERR_UNSUPPORTED, "%s: rows=%lld too large", what, (long long)rows);
+  PTX_REQUIRE(p >= 0.0 && p <= 1.0, PTX_ERR_BAD_ARG, "%s: p=%g outside 0..1", what, p);
+  PTX_REQUIRE(shared > 0 && inner > 0 && shared < ((int64_t)1 << 31) && inner < ((int64_t)1 << 31) && rows % (shared * inner) == 0,
+              PTX_ERR_BAD_ARG, "%s: %lld rows are not [outer][%lld][%lld]", what, (long long)rows, (long long)shared, (long long)inner);
+  const uint64_t threshold = (uint64_t)llrint(p * 4294967296.0);
+  d.key[0] = (uint32_t)seed;
+  d.key[1] = (uint32_t)(seed >> 32);
+  d.seed = seed_ptr;
+  d.hi = (uint32_t)(threshold >> 16);
+  d.lo = (uint32_t)(threshold & 0xFFFF);
+  d.scale = p < 1.0 ? (float)(1.0 / (1.0 - p)) : 0.0f;
+  d.shared = (uint32_t)shared;
+  d.inner = (uint32_t)inner;
+  return PTX_OK;
+}
+
+// Calls CALL with TX, TR for 16-bit or fp32 x beside a stream of its own type or of fp32.
+#define PTX_DISPATCH_STREAM(x_dtype, stream_dtype, CALL)          \
+  do {                                                            \
+    if ((x_dtype) == PTX_F32) {                                   \
+      typedef float TX;                                           \
+      typedef float TR;                                           \
+      CALL;                                                       \
+    } else if ((x_dtype) == PTX_BF16 && (stream_dtype) == PTX_F32) { \
+      typedef ptx::bf16_t TX;                                     \
+      typedef float TR;                                           \
+      CALL;                                                       \
+    } else if ((x_dtype) == PTX_BF16) {                           \
+      typedef ptx::bf16_t TX;                                     \
+      typedef ptx::bf16_t TR;                                     \
+      CALL;                                                       \
+    } else if ((stream_dtype) == PTX_F32) {                       \
+      typedef ptx::f16_t TX;                                      \
+      typedef float TR;                                           \
+      CALL;                                                       \
+    } else {                                                      \
+      typedef ptx::f16_t TX;                                      \
+      typedef ptx::f16_t TR;                                      \
+      CALL;                                                       \
+    }                                                             \
+  } while (0)
+
+PTX_API int ptx_dropout_add(const void* x, const void* residual, void* out, int64_t rows, int cols, int64_t shared, int64_t inner,
+                            double p, uint64_t seed, const int64_t* seed_ptr, int x_dtype, int stream_dtype, void* stream) {
+  PTX_REQUIRE(dtype_ok_ln(x_dtype) && dtype_ok_ln(stream_dtype), PTX_ERR_BAD_ARG, "dropout_add: unknown dtype %d or %d", x_dtype, stream_dtype);
+  PTX_REQUIRE(x_dtype == stream_dtype || x_dtype == PTX_F32 || stream_dtype == PTX_F32, PTX_ERR_UNSUPPORTED,
+              "dropout_add: two different 16-bit types");
+  PTX_REQUIRE(!residual || x_dtype == stream_dtype || stream_dtype == PTX_F32, PTX_ERR_UNSUPPORTED,
+              "dropout_add: fp32 x onto a 16-bit residual");
+  ptx::Dropout d;
+  const int rc = dropout_of(d, "dropout_add", rows, cols, shared, inner, p, seed, seed_ptr);
+  if (rc != PTX_OK || rows == 0) return rc;
+  PTX_REQUIRE(x && out, PTX_ERR_BAD_ARG, "dropout_add: null x or out");
+  const hipStream_t st = (hipStream_t)stream;
+  if (x_dtype == PTX_F32 && stream_dtype == PTX_BF16)
+    ptx::dropout_add<float, ptx::bf16_t>((const float*)x, nullptr, (ptx::bf16_t*)out, rows, cols, d, st);
+  else if (x_dtype == PTX_F32 && stream_dtype == PTX_F16)
+    ptx::dropout_add<float, ptx::f16_t>((const float*)x, nullptr, (ptx::f16_t*)out, rows, cols, d, st);
+  else
+    PTX_DISPATCH_STREAM(x_dtype, stream_dtype,
+                        (ptx::dropout_add<TX, TR>)((const TX*)x, (const TR*)residual, (TR*)out, rows, cols, d, st));
+  return after_launch("dropout_add");
+}
+
+static int dropnorm_args(ptx::Dropout& d, const char* what, int64_t rows, int cols, int64_t shared, int64_t inner, double p,
+                         uint64_t seed, const int64_t* seed_ptr, int x_dtype, int stream_dtype, int param_dtype) {
+  PTX_REQUIRE(dtype_ok_ln(x_dtype) && dtype_ok_ln(stream_dtype) && dtype_ok_ln(param_dtype), PTX_ERR_BAD_ARG,
+              "%s: unknown dtype among %d, %d, %d", what, x_dtype, stream_dtype, param_dtype);
+  PTX_REQUIRE(x_dtype == stream_dtype || stream_dtype == PTX_F32, PTX_ERR_UNSUPPORTED,
+              "%s: the stream has x's type or is fp32", what);
+  PTX_REQUIRE(cols <= ptx::dropnorm_max_cols(), PTX_ERR_UNSUPPORTED, "%s: rows of %d columns (%d at most)", what, cols,
+              ptx::dropnorm_max_cols());
+  return dropout_of(d, what, rows, cols, shared, inner, p, seed, seed_ptr);
+}
+
+PTX_API int ptx_dropout_add_layernorm_fwd(const void* x, const void* residual, const void* gamma, const void* beta, void* y, void* h,
+                                          float* mean, float* rstd, int64_t rows, int cols, int64_t shared, int64_t inner, double p,
+                                          float eps, uint64_t seed, const int64_t* seed_ptr, int x_dtype, int stream_dtype,
+                                          int param_dtype, void* stream) {
+  ptx::Dropout d;
+  const int rc = dropnorm_args(d, "dropout_add_layernorm", rows, cols, shared, inner, p, seed, seed_ptr, x_dtype, stream_dtype, param_dtype);
+  if (rc != PTX_OK || rows == 0) return rc;
+  PTX_REQUIRE(x && y && h, PTX_ERR_BAD_ARG, "dropout_add_layernorm: null x, y or h");
+  PTX_DISPATCH_STREAM(x_dtype, stream_dtype,
+                      (ptx::dropnorm_fwd<TX, TR>)((const TX*)x, (const TR*)residual, gamma, beta, param_dtype, (TX*)y, (TR*)h, mean, rstd,
+                                                  rows, cols, eps, d, (hipStream_t)stream));
+  return after_launch("dropout_add_layernorm");
+}
+
+PTX_API int64_t ptx_dropout_add_layernorm_bwd_workspace_elems(int64_t rows, int cols) {
+  return ptx::dropnorm_bwd_workspace_elems(rows, cols);
+}
+
+PTX_API int ptx_dropout_add_layernorm_bwd(const void* dy, const void* dh, const void* x, const void* residual, const void* h,
+                                          const float* mean, const float* rstd, const void* gamma, void* dx, void* dresidual,
+                                          void* dgamma, void* dbeta, float* workspace, int64_t rows, int cols, int64_t shared,
+                                          int64_t inner, double p, uint64_t seed, const int64_t* seed_ptr, int x_dtype,
+                                          int stream_dtype, int param_dtype, void* stream) {
+  ptx::Dropout d;
+  const int rc = dropnorm_args(d, "dropout_add_layernorm_bwd", rows, cols, shared, inner, p, seed, seed_ptr, x_dtype, stream_dtype, param_dtype);
+  if (rc != PTX_OK) return rc;
+  PTX_REQUIRE(rows == 0 || !(dgamma || dbeta) || workspace, PTX_ERR_BAD_ARG, "dropout_add_layernorm_bwd: dgamma / dbeta need the workspace");
+  if (rows == 0 && !dgamma && !dbeta) return PTX_OK;
+  PTX_REQUIRE(rows == 0 || ((h || x) && mean && rstd), PTX_ERR_BAD_ARG, "dropout_add_layernorm_bwd: null pointer");
+  PTX_DISPATCH_STREAM(x_dtype, stream_dtype,
+                      (ptx::dropnorm_bwd<TX, TR>)((const TX*)dy, (const TR*)dh, (const TX*)x, (const TR*)residual, (const TR*)h, mean, rstd,
+                                                  gamma, param_dtype, (TX*)dx, (TR*)dresidual, dgamma, dbeta, workspace, rows, cols, d,
+                                                  (hipStream_t)stream));
+  return after_launch("dropout_add_layernorm_bwd");
+}
+
+// ---- learned bias by buckets of relative position ---------------------------------------------------
+static int relative_bias_args(const char* what, const ptx_relative_buckets* bk, int batch, int heads, int q_len, int k_len,
+                              const int64_t* q_group, const int64_t* k_group, int table_dtype, int out_dtype) {
+  PTX_REQUIRE(dtype_ok_ln(table_dtype) && dtype_ok_ln(out_dtype), PTX_ERR_BAD_ARG, "%s: unknown dtype %d or %d", what, table_dtype, out_dtype);
+  PTX_REQUIRE(batch >= 0 && heads > 0 && q_len >= 0 && k_len >= 0, PTX_ERR_BAD_ARG, "%s: batch=%d heads=%d q_len=%d k_len=%d", what,
+              batch, heads, q_len, k_len);
+  PTX_REQUIRE(bk, PTX_ERR_BAD_ARG, "%s: null buckets", what);
+  PTX_REQUIRE(bk->count >= 1 && bk->count <= PTX_RELATIVE_BUCKETS_MAX && bk->max_distance >= 0 &&
+                  bk->max_distance <= PTX_RELATIVE_DISTANCE_MAX,
+              PTX_ERR_UNSUPPORTED, "%s: %d buckets up to distance %d (%d and %d at most)", what, bk->count, bk->max_distance,
+              PTX_RELATIVE_BUCKETS_MAX, PTX_RELATIVE_DISTANCE_MAX);
+  PTX_REQUIRE(bk->side >= 1 && bk->side <= 256 && bk->starts[0] == 0, PTX_ERR_BAD_ARG, "%s: %d buckets of a side", what, bk->side);
+  for (int s = 1; s < bk->side; ++s)
+    PTX_REQUIRE(bk->starts[s] >= bk->starts[s - 1], PTX_ERR_BAD_ARG, "%s: bucket %d starts before the one in front of it", what, s);
+  // every bucket the kernels can form is a row of the table
+  const int64_t ends[4] = {bk->neg_base, bk->neg_base + (int64_t)bk->neg_step * (bk->side - 1), bk->pos_base,
+                           bk->pos_base + (int64_t)bk->pos_step * (bk->side - 1)};
+  for (int64_t e : ends) PTX_REQUIRE(e >= 0 && e < bk->count, PTX_ERR_BAD_ARG, "%s: bucket %lld outside 0..%d", what, (long long)e, bk->count - 1);
+  PTX_REQUIRE(!q_group == !k_group, PTX_ERR_BAD_ARG, "%s: groups of the queries without the keys' or the reverse", what);
+  PTX_REQUIRE((double)batch * heads * q_len * k_len < 1e11 && heads <= 32768, PTX_ERR_UNSUPPORTED, "%s: too large", what);
+  return PTX_OK;
+}
+
+PTX_API int ptx_relative_bias_fwd(const ptx_relative_buckets* buckets, const void* table, void* out, int batch, int heads, int q_len,
+                                  int k_len, const int64_t* q_pos, const int64_t* k_pos, int64_t q_first, int64_t k_first,
+                                  const int64_t* q_group, const int64_t* k_group, int table_dtype, int out_dtype, void* stream) {
+  const int rc = relative_bias_args("relative_bias", buckets, batch, heads, q_len, k_len, q_group, k_group, table_dtype, out_dtype);
+  if (rc != PTX_OK) return rc;
+  if (batch == 0 || q_len == 0 || k_len == 0) return PTX_OK;
+  PTX_REQUIRE(table && out, PTX_ERR_BAD_ARG, "relative_bias: null table or out");
+  PTX_DISPATCH_LN(out_dtype, ptx::relative_bias_fwd<T>(*buckets, table, table_dtype, (T*)out, batch, heads, q_len, k_len, q_pos, k_pos,
+                                                       q_first, k_first, q_group, k_group, (hipStream_t)stream));
+  return after_launch("relative_bias");
+}
+
+PTX_API int64_t ptx_relative_bias_bwd_workspace_elems(int heads, int table_rows) {
+  return ptx::relative_bias_bwd_workspace_elems(heads, table_rows);
+}
+
+PTX_API int ptx_relative_bias_bwd(const ptx_relative_buckets* buckets, const void* dout, void* dtable, float* workspace, int batch,
+                                  int heads, int q_len, int k_len, const int64_t* q_pos, const int64_t* k_pos, int64_t q_first,
+                                  int64_t k_first, const int64_t* q_group, const int64_t* k_group, int table_dtype, int out_dtype,
+                                  void* stream) {
+  const int rc = relative_bias_args("relative_bias_bwd", buckets, batch, heads, q_len, k_len, q_group, k_group, table_dtype, out_dtype);
+  if (rc != PTX_OK) return rc;
+  PTX_REQUIRE(dtable && workspace && (dout || batch == 0 || q_len == 0 || k_len == 0), PTX_ERR_BAD_ARG, "relative_bias_bwd: null pointer");
+  PTX_DISPATCH_LN(out_dtype, ptx::relative_bias_bwd<T>(*buckets, (const T*)dout, dtable, table_dtype, workspace, batch, heads, q_len, k_len,
+                                                       q_pos, k_pos, q_first, k_first, q_group, k_group, (hipStream_t)stream));
+  return after_launch("relative_bias_bwd");
 }
 
 }  // extern "C"

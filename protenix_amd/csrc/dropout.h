@@ -1,0 +1,110 @@
+// The dropout mask of the residual updates, and 8-column vectors at any alignment: shared by dropout.hip and dropnorm.hip.
+//
+// The mask is never stored: forward and backward kernels draw it from Philox4x32-10, the counter-based generator of
+// Salmon, Moraes, Dror and Shaw (Parallel random numbers: as easy as 1, 2, 3, 2011).  A mask row's columns lie in
+// blocks of 8; block k of mask row r has the counter (k, r, 0, draw) and the seed as its key.  Draw 0 gives the block's
+// 8 numbers of 16 bits (word i / 2, low half first), draw 1 the 16 bits below them: an element is kept where the 32-bit
+// number is at least round(p 2^32).  The second draw is made only where a first number equals the threshold's upper half
+// (8 in 65536 blocks; never where the lower half is 0, as for p = 1/4), so that p has a resolution of 2^-32 for the
+// price of 16 bits.  What a number depends on is its mask row and column alone: neither the types, the
+// alignment nor the launch.
+#pragma once
+#include "common.h"
+
+namespace ptx {
+
+struct Dropout {
+  uint32_t key[2];
+  const int64_t* seed;   // read from device memory where given: the key then
+  uint32_t hi, lo;       // the threshold round(p 2^32): hi 2^16 + lo; 0 = no dropout, 2^16 and 0 = nothing stays
+  float scale;           // 1 / (1 - p), 0 for p = 1
+  // Rows are [outer][shared][inner]; the rows of one (outer, inner) have the same mask row, outer * inner + inner.
+  uint32_t shared, inner;
+};
+
+__device__ __forceinline__ Dropout with_key(Dropout d) {
+  if (d.seed && (d.hi | d.lo)) {
+    const uint64_t s = (uint64_t)*d.seed;
+    d.key[0] = (uint32_t)s;
+    d.key[1] = (uint32_t)(s >> 32);
+  }
+  return d;
+}
+
+__device__ __forceinline__ void philox(uint32_t (&c)[4], uint32_t k0, uint32_t k1) {
+#pragma unroll
+  for (int r = 0; r < 10; ++r) {
+    const uint64_t a = (uint64_t)c[0] * 0xD2511F53u, b = (uint64_t)c[2] * 0xCD9E8D57u;
+    c[0] = (uint32_t)(b >> 32) ^ c[1] ^ k0;
+    c[1] = (uint32_t)b;
+    c[2] = (uint32_t)(a >> 32) ^ c[3] ^ k1;
+    c[3] = (uint32_t)a;
+    k0 += 0x9E3779B9u;
+    k1 += 0xBB67AE85u;
+  }
+}
+
+// factor[e]: what element e of block k of the mask row is multiplied by, `scale` or 0.
+__device__ __forceinline__ void dropout_factors(const Dropout& d, uint32_t row, uint32_t k, float (&factor)[8]) {
+  uint32_t w[4] = {k, row, 0u, 0u};
+  philox(w, d.key[0], d.key[1]);
+  // (a number equal to hi is kept where lo is 0; where it is not, the second draw decides)
+  const uint32_t cut = d.hi + (d.lo != 0);
+  bool tie = false;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const uint32_t u = e & 1 ? w[e >> 1] >> 16 : w[e >> 1] & 0xFFFFu;
+    factor[e] = u >= cut ? d.scale : 0.0f;
+    tie = tie || u == d.hi;
+  }
+  if (d.lo != 0 && tie) {
+    uint32_t v[4] = {k, row, 0u, 1u};
+    philox(v, d.key[0], d.key[1]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t u = e & 1 ? w[e >> 1] >> 16 : w[e >> 1] & 0xFFFFu;
+      const uint32_t below = e & 1 ? v[e >> 1] >> 16 : v[e >> 1] & 0xFFFFu;
+      if (u == d.hi && below >= d.lo) factor[e] = d.scale;
+    }
+  }
+}
+
+// x * factor, with exactly 0 for a dropped element whatever it holds
+__device__ __forceinline__ float dropped(float x, float factor) { return factor != 0.0f ? x * factor : 0.0f; }
+// res + x * factor in one rounding
+__device__ __forceinline__ float dropped_add(float x, float factor, float res) {
+  return factor != 0.0f ? __builtin_fmaf(x, factor, res) : res;
+}
+
+// Eight columns at an element's alignment (rows of odd lengths): gfx950 takes vector accesses at any address, so an
+// odd row costs the lines it straddles and nothing else.  n: how many of the columns exist; the others read as 0.
+template <typename T> struct Unaligned8 { typedef T type __attribute__((ext_vector_type(8), aligned(sizeof(T)))); };
+
+template <typename T> __device__ __forceinline__ f32x8 load_cols(const T* p, int n) {
+  typedef typename Unaligned8<T>::type V;
+  f32x8 out;
+  if (n >= 8) {
+    const V v = *reinterpret_cast<const V*>(p);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) out[e] = (float)v[e];
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) out[e] = e < n ? (float)p[e] : 0.0f;
+  }
+  return out;
+}
+template <typename T> __device__ __forceinline__ void store_cols(T* p, f32x8 v, int n) {
+  typedef typename Unaligned8<T>::type V;
+  if (n >= 8) {
+    V o;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = (T)v[e];
+    *reinterpret_cast<V*>(p) = o;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < n) p[e] = (T)v[e];
+  }
+}
+
+}  // namespace ptx

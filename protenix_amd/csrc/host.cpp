@@ -13,6 +13,7 @@
 
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 
+#include <array>
 #include <cstring>
 #include <mutex>
 #include <set>
@@ -1137,6 +1138,226 @@ Tensor tri_attention(const Tensor& q, const Tensor& k, const Tensor& v, const op
   return TriAttentionFn::apply(q, k, v, b1, b2);
 }
 
+// ---- residual dropout, its sum with LayerNorm, the relative position bias ---------------------------------
+// Arguments as dropout.py and relative_bias.py have checked them.
+struct RowsOf {
+  int64_t rows, cols, shared, inner;
+};
+
+// A backward pass recorded into a graph adds to a leaf's gradient on the stream the leaf's accumulator was made on.
+// One that an eager graph made and still holds is on another stream than the recording's: the pass would pull that stream into the
+// recording and leave it there, which ends the process, so the forward call is refused.
+void refuse_foreign_accumulators(hipStream_t st, std::initializer_list<const Tensor*> leaves) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(st, &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
+  for (const Tensor* t : leaves) {
+    if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+    if (!node) continue;
+    const auto made_on = node->stream();
+    if (made_on && c10::hip::HIPStreamMasqueradingAsCUDA(*made_on).stream() != st)
+      throw std::runtime_error("protenix_amd: a call recorded into a graph has an input whose gradient an eager graph that is still alive "
+                               "accumulates on another stream; drop the results of the eager calls first");
+  }
+}
+void refuse_double_backward() {
+  if (at::GradMode::is_enabled()) throw std::runtime_error("protenix_amd: this operator's gradient is not differentiable (create_graph=True)");
+}
+Tensor given(const optional<Tensor>& t) { return t ? *t : Tensor(); }
+Tensor dense(const optional<Tensor>& t) { return t && t->defined() ? t->contiguous() : Tensor(); }
+bool wants(const Tensor& t) { return t.defined() && t.requires_grad(); }
+
+Tensor dropout_add_call(const Tensor& x, const Tensor& res, at::ScalarType out_type, const RowsOf& r, double p, uint64_t number, const Tensor& seed) {
+  const Tensor xc = x.contiguous();
+  Tensor out = at::empty(x.sizes(), x.options().dtype(out_type).memory_format(at::MemoryFormat::Contiguous));
+  check(ptx_dropout_add(ptr(xc), ptr(res), ptr(out), r.rows, (int)r.cols, r.shared, r.inner, p, number, (const int64_t*)ptr(seed),
+                        code_of(x.scalar_type()), code_of(out_type), current_stream(x)), "dropout_add");
+  return out;
+}
+
+struct DropoutAddFn : torch::autograd::Function<DropoutAddFn> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const optional<Tensor>& residual, const optional<Tensor>& seed,
+                        const RowsOf& r, double p, uint64_t number) {
+    const Tensor res = dense(residual), sd = given(seed);
+    ctx->save_for_backward({sd});
+    ctx->saved_data["rows"] = std::vector<int64_t>{r.rows, r.cols, r.shared, r.inner, (int64_t)number, (int64_t)x.scalar_type()};
+    ctx->saved_data["p"] = p;
+    ctx->saved_data["res"] = res.defined();
+    return dropout_add_call(x, res, res.defined() ? res.scalar_type() : x.scalar_type(), r, p, number, sd);
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    refuse_double_backward();
+    const Tensor seed = ctx->get_saved_variables()[0], &grad = grads[0];
+    const auto v = ctx->saved_data["rows"].toIntVector();
+    at::DeviceGuard dev(grad.device());
+    Tensor dx;
+    if (ctx->needs_input_grad(0))
+      dx = dropout_add_call(grad, Tensor(), (at::ScalarType)v[5], {v[0], v[1], v[2], v[3]}, ctx->saved_data["p"].toDouble(), (uint64_t)v[4], seed);
+    // (needs_input_grad counts the tensors that were given)
+    const bool res = ctx->saved_data["res"].toBool() && ctx->needs_input_grad(1);
+    return {dx, res ? grad : Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+Tensor dropout_add(const Tensor& x, const optional<Tensor>& residual, int64_t rows, int64_t cols, int64_t shared, int64_t inner, double p,
+                   uint64_t number, const optional<Tensor>& seed) {
+  py::gil_scoped_release nogil;
+  at::DeviceGuard dev(x.device());
+  const RowsOf r{rows, cols, shared, inner};
+  const Tensor res = given(residual);
+  if (at::GradMode::is_enabled() && (wants(x) || wants(res))) {
+    refuse_foreign_accumulators(current_stream(x), {&x, &res});
+    return DropoutAddFn::apply(x, residual, seed, r, p, number);
+  }
+  return dropout_add_call(x, dense(residual), res.defined() ? res.scalar_type() : x.scalar_type(), r, p, number, given(seed));
+}
+
+// y, h and, for a backward pass, the rows' statistics [2][rows]
+std::tuple<Tensor, Tensor, Tensor> dropnorm_call(const Tensor& x, const Tensor& res, const Tensor& w, const Tensor& b, const RowsOf& r,
+                                                 double p, double eps, uint64_t number, const Tensor& seed, bool want_stats) {
+  Tensor y = at::empty_like(x), h = at::empty_like(res.defined() ? res : x), stats;
+  if (want_stats) stats = at::empty({2, r.rows}, x.options().dtype(at::kFloat));
+  float* st = (float*)ptr(stats);
+  const auto param = w.defined() ? w.scalar_type() : b.defined() ? b.scalar_type() : at::kFloat;
+  check(ptx_dropout_add_layernorm_fwd(ptr(x), ptr(res), ptr(w), ptr(b), ptr(y), ptr(h), st, st ? st + r.rows : nullptr, r.rows, (int)r.cols,
+                                      r.shared, r.inner, p, (float)eps, number, (const int64_t*)ptr(seed), code_of(x.scalar_type()),
+                                      code_of(h.scalar_type()), code_of(param), current_stream(x)), "dropout_add_layernorm");
+  return {y, h, stats};
+}
+
+struct DropoutAddLayerNormFn : torch::autograd::Function<DropoutAddLayerNormFn> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& x_, const optional<Tensor>& residual,
+                                                const optional<Tensor>& weight, const optional<Tensor>& bias, const optional<Tensor>& seed_,
+                                                const RowsOf& r, double p, double eps, uint64_t number) {
+    ctx->set_materialize_grads(false);
+    const Tensor x = x_.contiguous(), res = dense(residual), w = dense(weight), b = dense(bias), seed = given(seed_);
+    auto [y, h, stats] = dropnorm_call(x, res, w, b, r, p, eps, number, seed, true);
+    // the sum itself where the stream is fp32; else what it is formed from (see ptx_dropout_add_layernorm_bwd)
+    const bool keep_h = h.scalar_type() == at::kFloat;
+    ctx->save_for_backward({keep_h ? Tensor() : x, keep_h ? Tensor() : res, keep_h ? h : Tensor(), stats, w, seed});
+    const auto param = w.defined() ? w.scalar_type() : b.defined() ? b.scalar_type() : at::kFloat;
+    ctx->saved_data["rows"] = std::vector<int64_t>{r.rows, r.cols, r.shared, r.inner, (int64_t)number, (int64_t)x.scalar_type(), (int64_t)param,
+                                                   res.defined() + 2 * w.defined() + 4 * b.defined()};
+    ctx->saved_data["p"] = p;
+    return {y, h};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    refuse_double_backward();
+    torch::autograd::variable_list out(9);
+    if (!grads[0].defined() && !grads[1].defined()) return out;
+    const auto t = ctx->get_saved_variables();
+    const Tensor &x = t[0], &res = t[1], &h = t[2], &stats = t[3], &w = t[4], &seed = t[5];
+    const auto v = ctx->saved_data["rows"].toIntVector();
+    const double p = ctx->saved_data["p"].toDouble();
+    const int64_t rows = v[0], cols = v[1];
+    const auto x_type = (at::ScalarType)v[5], param = (at::ScalarType)v[6];
+    const Tensor& like = h.defined() ? h : x;
+    const auto stream_type = like.scalar_type();
+    at::DeviceGuard dev(like.device());
+    const Tensor dy = dense(grads[0]), dh = dense(grads[1]);
+    int next = 0;   // (needs_input_grad counts the tensors that were given)
+    auto needs = [&](bool was_given) { return was_given && ctx->needs_input_grad(next++); };
+    const bool need_x = needs(true), need_res = needs(v[7] & 1), need_w = needs(v[7] & 2), need_b = needs(v[7] & 4);
+    const bool one = p == 0.0 && x_type == stream_type && need_x && need_res;   // (the two gradients are the same values)
+    Tensor dx, dres, dw, db, ws;
+    if (need_res) dres = at::empty_like(like);
+    if (need_x && !one) dx = at::empty(like.sizes(), like.options().dtype(x_type));
+    if (need_w) dw = at::empty({cols}, like.options().dtype(param));
+    if (need_b) db = at::empty({cols}, like.options().dtype(param));
+    if (need_w || need_b)
+      ws = at::empty({ptx_dropout_add_layernorm_bwd_workspace_elems(std::max<int64_t>(rows, 1), (int)cols)}, like.options().dtype(at::kFloat));
+    const float* st = (const float*)ptr(stats);
+    check(ptx_dropout_add_layernorm_bwd(ptr(dy), ptr(dh), ptr(x), ptr(res), ptr(h), st, st + rows, ptr(w), ptr(dx), ptr(dres), ptr(dw), ptr(db),
+                                        (float*)ptr(ws), rows, (int)cols, v[2], v[3], p, (uint64_t)v[4], (const int64_t*)ptr(seed), code_of(x_type),
+                                        code_of(stream_type), code_of(param), current_stream(like)), "dropout_add_layernorm_bwd");
+    out[0] = one ? dres : dx;
+    out[1] = dres;
+    out[2] = dw;
+    out[3] = db;
+    return out;
+  }
+};
+
+std::tuple<Tensor, Tensor> dropout_add_layer_norm(const Tensor& x, const optional<Tensor>& residual, const optional<Tensor>& weight,
+                                                  const optional<Tensor>& bias, int64_t rows, int64_t cols, int64_t shared, int64_t inner, double p,
+                                                  double eps, uint64_t number, const optional<Tensor>& seed) {
+  py::gil_scoped_release nogil;
+  at::DeviceGuard dev(x.device());
+  const RowsOf r{rows, cols, shared, inner};
+  const Tensor res = given(residual), w = given(weight), b = given(bias);
+  if (at::GradMode::is_enabled() && (wants(x) || wants(res) || wants(w) || wants(b))) {
+    refuse_foreign_accumulators(current_stream(x), {&x, &res, &w, &b});
+    const auto out = DropoutAddLayerNormFn::apply(x, residual, weight, bias, seed, r, p, eps, number);
+    return {out[0], out[1]};
+  }
+  const auto [y, h, stats] = dropnorm_call(x.contiguous(), dense(residual), dense(weight), dense(bias), r, p, eps, number, given(seed), false);
+  return {y, h};
+}
+
+struct BiasCall {
+  ptx_relative_buckets buckets;
+  int size[4];   // batch, heads, queries, keys
+  int64_t q_first, k_first;
+};
+
+Tensor relative_bias_call(const Tensor& table, const Tensor& q, const Tensor& k, const Tensor& gq, const Tensor& gk, const BiasCall& c,
+                          at::ScalarType type) {
+  const Tensor t = table.contiguous();
+  Tensor out = at::empty({c.size[0], c.size[1], c.size[2], c.size[3]}, t.options().dtype(type));
+  check(ptx_relative_bias_fwd(&c.buckets, ptr(t), ptr(out), c.size[0], c.size[1], c.size[2], c.size[3], (const int64_t*)ptr(q),
+                              (const int64_t*)ptr(k), c.q_first, c.k_first, (const int64_t*)ptr(gq), (const int64_t*)ptr(gk),
+                              code_of(t.scalar_type()), code_of(type), current_stream(t)), "relative_bias");
+  return out;
+}
+
+struct RelativeBiasFn : torch::autograd::Function<RelativeBiasFn> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& table, const optional<Tensor>& q, const optional<Tensor>& k,
+                        const optional<Tensor>& gq, const optional<Tensor>& gk, const BiasCall& c, at::ScalarType type) {
+    ctx->save_for_backward({given(q), given(k), given(gq), given(gk)});
+    // (the buckets are a plain struct: carried as the bytes they are)
+    ctx->saved_data["call"] = std::string((const char*)&c, sizeof(c));
+    ctx->saved_data["table"] = std::vector<int64_t>{table.size(0), table.size(1), (int64_t)table.scalar_type()};
+    return relative_bias_call(table, given(q), given(k), given(gq), given(gk), c, type);
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    refuse_double_backward();
+    const auto t = ctx->get_saved_variables();
+    const auto v = ctx->saved_data["table"].toIntVector();
+    const std::string bytes = ctx->saved_data["call"].toStringRef();
+    BiasCall c;
+    std::memcpy(&c, bytes.data(), sizeof(c));
+    at::DeviceGuard dev(grads[0].device());
+    const Tensor dout = grads[0].contiguous();
+    Tensor dtable = at::empty({v[0], v[1]}, dout.options().dtype((at::ScalarType)v[2]));
+    Tensor ws = at::empty({ptx_relative_bias_bwd_workspace_elems((int)v[1], (int)v[0])}, dout.options().dtype(at::kFloat));
+    check(ptx_relative_bias_bwd(&c.buckets, ptr(dout), ptr(dtable), (float*)ptr(ws), c.size[0], c.size[1], c.size[2], c.size[3],
+                                (const int64_t*)ptr(t[0]), (const int64_t*)ptr(t[1]), c.q_first, c.k_first, (const int64_t*)ptr(t[2]),
+                                (const int64_t*)ptr(t[3]), code_of(dtable.scalar_type()), code_of(dout.scalar_type()), current_stream(dout)),
+          "relative_bias_bwd");
+    return {dtable, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+// buckets: the address of a ptx_relative_buckets
+Tensor relative_bias(const Tensor& table, uintptr_t buckets, const std::array<int64_t, 4>& size, const optional<Tensor>& q, const optional<Tensor>& k,
+                     const optional<Tensor>& gq, const optional<Tensor>& gk, int64_t q_first, int64_t k_first, at::ScalarType type) {
+  BiasCall c;
+  c.buckets = *(const ptx_relative_buckets*)buckets;
+  for (int i = 0; i < 4; ++i) {
+    if (size[i] > 0x7fffffff) throw std::runtime_error("relative_bias: unsupported shape (2): a side of 2^31 or more");
+    c.size[i] = (int)size[i];
+  }
+  c.q_first = q_first;
+  c.k_first = k_first;
+  py::gil_scoped_release nogil;
+  at::DeviceGuard dev(table.device());
+  if (at::GradMode::is_enabled() && table.requires_grad()) {
+    refuse_foreign_accumulators(current_stream(table), {&table});
+    return RelativeBiasFn::apply(table, q, k, gq, gk, c, type);
+  }
+  return relative_bias_call(table, given(q), given(k), given(gq), given(gk), c, type);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_host, m) {
@@ -1167,4 +1388,7 @@ PYBIND11_MODULE(_host, m) {
   py::class_<Mark, std::shared_ptr<Mark>>(m, "Mark").def("elapsed_time", &Mark::elapsed_time);
   m.def("layer_norm", &layer_norm);
   m.def("tri_attention", &tri_attention);
+  m.def("dropout_add", &dropout_add);
+  m.def("dropout_add_layer_norm", &dropout_add_layer_norm);
+  m.def("relative_bias", &relative_bias);
 }

@@ -5,6 +5,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+struct ptx_relative_buckets;
+
 namespace ptx {
 
 // T: arithmetic / weight / workspace type.  TZ (where present): storage type of the pair
@@ -230,6 +232,34 @@ template <typename T>
 int triattn_bwd(const void* q, const void* k, const void* v, const void* b1, const void* b2,
                 const void* o, const float* lse, const void* dout, void* dq, void* dk, void* dv,
                 void* db2, float* delta, float* parts, int n_rows, int s, int heads, hipStream_t stream);
+
+// out = residual + dropout(x) (res null: dropout(x) alone), TI the type of x, TO that of the residual and out; see dropout.hip.
+struct Dropout;
+template <typename TI, typename TO>
+int dropout_add(const TI* x, const TO* res, TO* out, int64_t rows, int cols, const Dropout& drop, hipStream_t stream);
+// The same sum h and its LayerNorm y, and the gradients of both (see dropnorm.hip); param_type: ptx_dtype of gamma, beta and their
+// gradients.  Rows of up to dropnorm_max_cols() columns.
+int dropnorm_max_cols();
+template <typename TX, typename TR>
+int dropnorm_fwd(const TX* x, const TR* res, const void* gamma, const void* beta, int param_type, TX* y, TR* h, float* mean,
+                 float* rstd, int64_t rows, int cols, float eps, const Dropout& drop, hipStream_t stream);
+int64_t dropnorm_bwd_workspace_elems(int64_t rows, int cols);
+template <typename TX, typename TR>
+int dropnorm_bwd(const TX* dy, const TR* dh, const TX* x, const TR* res, const TR* h, const float* mean, const float* rstd,
+                 const void* gamma, int param_type, TX* dx, TR* dres, void* dgamma, void* dbeta, float* workspace, int64_t rows,
+                 int cols, const Dropout& drop, hipStream_t stream);
+// Column sums of fp32 partial rows, [2][parts][cols] -> a, b of param_type (either may be null): layernorm_bwd's second launch.
+void column_sums(const float* part, int parts, int cols, int param_type, void* a, void* b, hipStream_t stream);
+// Learned bias by buckets of relative position, and its table's gradient (see relbias.hip).
+template <typename T>
+int relative_bias_fwd(const ptx_relative_buckets& bk, const void* table, int table_type, T* out, int batch, int heads, int q_len,
+                      int k_len, const int64_t* q_pos, const int64_t* k_pos, int64_t q_first, int64_t k_first, const int64_t* q_group,
+                      const int64_t* k_group, hipStream_t stream);
+int64_t relative_bias_bwd_workspace_elems(int heads, int n_buckets);
+template <typename T>
+int relative_bias_bwd(const ptx_relative_buckets& bk, const T* dout, void* dtable, int table_type, float* workspace, int batch,
+                      int heads, int q_len, int k_len, const int64_t* q_pos, const int64_t* k_pos, int64_t q_first, int64_t k_first,
+                      const int64_t* q_group, const int64_t* k_group, hipStream_t stream);
 
 // Streams `bytes` (a multiple of 16) from src to dst; src null: write-only, dst null: read-only.
 int hbm_stream(const void* src, void* dst, int64_t bytes, int nontemporal, hipStream_t stream);

@@ -489,6 +489,16 @@ __global__ __launch_bounds__(1024) void layernorm_bwd_reduce_kernel(
   }
 }
 
+void column_sums(const float* part, int parts, int cols, int param_type, void* a, void* b, hipStream_t stream) {
+  const dim3 grid((cols + kReduceCols - 1) / kReduceCols, b ? 2 : 1);
+  if (param_type == 0)        // (ptx_dtype)
+    layernorm_bwd_reduce_kernel<float><<<grid, dim3(1024), 0, stream>>>(part, parts, cols, (float*)a, (float*)b);
+  else if (param_type == 1)
+    layernorm_bwd_reduce_kernel<bf16_t><<<grid, dim3(1024), 0, stream>>>(part, parts, cols, (bf16_t*)a, (bf16_t*)b);
+  else
+    layernorm_bwd_reduce_kernel<f16_t><<<grid, dim3(1024), 0, stream>>>(part, parts, cols, (f16_t*)a, (f16_t*)b);
+}
+
 template <typename T, int VEC>
 static int dispatch_ln_bwd_vec(const T* dout, const T* x, const float* mean, const float* rstd,
                                const T* gamma, T* dx, float* part, int64_t rows, int cols,

@@ -720,3 +720,87 @@ def hbm_stream(src: Optional[torch.Tensor], dst: Optional[torch.Tensor], nontemp
     with torch.cuda.device(t.device):
         _call("hbm_stream", _lib.load().ptx_hbm_stream, _ptr(src), _ptr(dst), t.numel() * t.element_size(),
               int(nontemporal), _stream())
+
+
+# ---- residual dropout, its sum with LayerNorm, relative position bias -----------------------------------
+# (arguments as the modules dropout.py and relative_bias.py have checked them; `rows` = (rows, cols, shared, inner) as the
+# C ABI counts them, `seed` = (whole number, None) or (0, one-element int64 tensor))
+def dropout_add(x: torch.Tensor, residual: Optional[torch.Tensor], out_dtype: torch.dtype, rows: tuple, p: float, seed: tuple) -> torch.Tensor:
+    """[residual +] dropout(x); on a gradient, without a residual, the gradient of x."""
+    lib = _lib.load()
+    x = x.contiguous()
+    res = None if residual is None else residual.contiguous()
+    out = torch.empty(x.shape, dtype=out_dtype, device=x.device)
+    n, cols, shared, inner = rows
+    with torch.cuda.device(x.device):
+        _call("dropout_add", lib.ptx_dropout_add, _ptr(x), _ptr(res), _ptr(out), n, cols, shared, inner, p, seed[0], _ptr(seed[1]),
+              _dt_ln(x), _dt_ln(out), _stream())
+    return out
+
+
+def dropout_add_layer_norm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: Optional[torch.Tensor],
+                           bias: Optional[torch.Tensor], rows: tuple, p: float, eps: float, seed: tuple, return_stats: bool):
+    """(y, h, statistics [2, rows] or None) of contiguous x and residual."""
+    lib = _lib.load()
+    n, cols, shared, inner = rows
+    param = weight if weight is not None else bias
+    y = torch.empty_like(x)
+    h = torch.empty_like(x if residual is None else residual)
+    stats = torch.empty((2, n), dtype=torch.float32, device=x.device) if return_stats else None
+    with torch.cuda.device(x.device):
+        _call("dropout_add_layernorm", lib.ptx_dropout_add_layernorm_fwd, _ptr(x), _ptr(residual), _ptr(weight), _ptr(bias), _ptr(y),
+              _ptr(h), _ptr(stats), None if stats is None else stats.data_ptr() + 4 * n, n, cols, shared, inner, p, eps, seed[0],
+              _ptr(seed[1]), _dt_ln(x), _dt_ln(h), _lib.PTX_F32 if param is None else _dt_ln(param), _stream())
+    return y, h, stats
+
+
+def dropout_add_layer_norm_backward(dy, dh, x, residual, h, stats, weight, param_dtype, rows: tuple, p: float, seed: tuple,
+                                    need: tuple):
+    """Gradients (x, residual, weight, bias), those of `need`; x and residual given (16-bit streams) or h (fp32 ones)."""
+    lib = _lib.load()
+    n, cols, shared, inner = rows
+    like = x if x is not None else h
+    res_dtype = like.dtype if h is None else h.dtype
+    x_dtype = x.dtype if x is not None else (dy.dtype if dy is not None else need[4])
+    empty = lambda dtype: torch.empty(like.shape, dtype=dtype, device=like.device)
+    one = p == 0.0 and x_dtype == res_dtype and need[0] and need[1]      # (the two gradients are the same values)
+    dres = empty(res_dtype) if need[1] else None
+    dx = empty(x_dtype) if need[0] and not one else None
+    dw = torch.empty(cols, dtype=param_dtype, device=like.device) if need[2] else None
+    db = torch.empty(cols, dtype=param_dtype, device=like.device) if need[3] else None
+    ws = None
+    if dw is not None or db is not None:
+        ws = _workspace((lib.ptx_dropout_add_layernorm_bwd_workspace_elems(max(n, 1), cols),), torch.float32, like.device)
+    codes = {torch.float32: _lib.PTX_F32, torch.bfloat16: _lib.PTX_BF16, torch.float16: _lib.PTX_F16}
+    with torch.cuda.device(like.device):
+        _call("dropout_add_layernorm_bwd", lib.ptx_dropout_add_layernorm_bwd, _ptr(dy), _ptr(dh), _ptr(x), _ptr(residual), _ptr(h),
+              _ptr(stats), stats.data_ptr() + 4 * n, _ptr(weight), _ptr(dx), _ptr(dres), _ptr(dw), _ptr(db), _ptr(ws), n, cols, shared,
+              inner, p, seed[0], _ptr(seed[1]), codes[x_dtype], codes[res_dtype], codes[param_dtype], _stream())
+    return (dres if one else dx), dres, dw, db
+
+
+def relative_bias(buckets, table: torch.Tensor, size: tuple, q: tuple, k: tuple, groups: tuple, dtype: torch.dtype) -> torch.Tensor:
+    """[B, H, Q, K] for size = (B, H, Q, K); q, k = (positions [B, n] or None, first); groups = ([B, Q], [B, K]) or (None, None)."""
+    import ctypes
+
+    lib = _lib.load()
+    out = torch.empty(size, dtype=dtype, device=table.device)
+    with torch.cuda.device(table.device):
+        _call("relative_bias", lib.ptx_relative_bias_fwd, ctypes.addressof(buckets), _ptr(table), _ptr(out), *size, _ptr(q[0]),
+              _ptr(k[0]), q[1], k[1], _ptr(groups[0]), _ptr(groups[1]), _dt_ln(table), _dt_ln(out), _stream())
+    return out
+
+
+def relative_bias_backward(buckets, dout: torch.Tensor, table_shape, table_dtype: torch.dtype, size: tuple, q: tuple, k: tuple,
+                           groups: tuple) -> torch.Tensor:
+    """The table's gradient from that of the bias."""
+    import ctypes
+
+    lib = _lib.load()
+    dout = dout.contiguous()
+    dtable = torch.empty(table_shape, dtype=table_dtype, device=dout.device)
+    ws = _workspace((lib.ptx_relative_bias_bwd_workspace_elems(size[1], table_shape[0]),), torch.float32, dout.device)
+    with torch.cuda.device(dout.device):
+        _call("relative_bias_bwd", lib.ptx_relative_bias_bwd, ctypes.addressof(buckets), _ptr(dout), _ptr(dtable), _ptr(ws), *size,
+              _ptr(q[0]), _ptr(k[0]), q[1], k[1], _ptr(groups[0]), _ptr(groups[1]), _dt_ln(dtable), _dt_ln(dout), _stream())
+    return dtable
