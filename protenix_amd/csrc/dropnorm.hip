@@ -27,16 +27,12 @@ struct NormParam {
 };
 constexpr int kF32 = 0, kBF16 = 1;
 
-__device__ __forceinline__ f32x8 load_param(NormParam w, int col, int n, float absent) {
-  f32x8 v;
-  if (!w.p) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = absent;
-    return v;
-  }
-  if (w.type == kF32) return load_cols((const float*)w.p + col, n);
-  if (w.type == kBF16) return load_cols((const bf16_t*)w.p + col, n);
-  return load_cols((const f16_t*)w.p + col, n);
+template <bool SHORT> __device__ __forceinline__ f32x8 load_param(NormParam w, int col, int cols, int n, float absent) {
+  if (n == 0) return f32x8{};
+  if (!w.p) return f32x8{absent, absent, absent, absent, absent, absent, absent, absent};
+  if (w.type == kF32) return used_cols<SHORT, float>(load_cols<SHORT>((const float*)w.p, col, cols), n);
+  if (w.type == kBF16) return used_cols<SHORT, bf16_t>(load_cols<SHORT>((const bf16_t*)w.p, col, cols), n);
+  return used_cols<SHORT, f16_t>(load_cols<SHORT>((const f16_t*)w.p, col, cols), n);
 }
 
 template <int G> __device__ __forceinline__ float lanes_sum(float v) {
@@ -79,8 +75,8 @@ __device__ __forceinline__ uint32_t mask_row_of(const Dropout& d, uint32_t row) 
   return o * d.inner + row % d.inner;
 }
 
-// TX: type of x and y; TR: of the residual and h.
-template <typename TX, typename TR, int G, int WPR, int NC>
+// TX: type of x and y; TR: of the residual and h.  SHORT: fewer than 8 columns.
+template <typename TX, typename TR, int G, int WPR, int NC, bool SHORT>
 __global__ __launch_bounds__((Lay<G, WPR>::kThreads)) void dropnorm_fwd_kernel(
     const TX* __restrict__ x, const TR* __restrict__ res, NormParam gamma, NormParam beta, TX* __restrict__ y, TR* __restrict__ h,
     float* __restrict__ mean_out, float* __restrict__ rstd_out, int64_t rows, int cols, float eps, Dropout drop) {
@@ -88,45 +84,57 @@ __global__ __launch_bounds__((Lay<G, WPR>::kThreads)) void dropnorm_fwd_kernel(
   __shared__ float slots[2][16][2];
   const int lane = threadIdx.x % L::kSpan, sub_row = threadIdx.x / L::kSpan;
   const float inv_n = 1.0f / (float)cols;
+  const bool masked = (drop.hi | drop.lo) != 0;
   drop = with_key(drop);
+  struct Raw {
+    Raw8<TX> x[NC];
+    Raw8<TR> res[NC];
+  };
+  // (rows and columns beyond the end: the last ones once more, not used)
+  auto load = [&](Raw& raw, int64_t row) {
+    const int64_t at = min(row, rows - 1) * cols;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      raw.x[c] = load_cols<SHORT>(x + at, (c * L::kSpan + lane) * 8, cols);
+      raw.res[c] = Raw8<TR>{};
+      if (res) raw.res[c] = load_cols<SHORT>(res + at, (c * L::kSpan + lane) * 8, cols);
+    }
+  };
+  const int64_t step = (int64_t)gridDim.x * L::kRows;
+  int64_t row0 = (int64_t)blockIdx.x * L::kRows;
+  Raw cur;
+  load(cur, row0 + sub_row);
   f32x8 gm[NC], bt[NC];
   int n[NC];
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
     const int col = (c * L::kSpan + lane) * 8;
     n[c] = max(min(cols - col, 8), 0);
-    gm[c] = n[c] ? load_param(gamma, col, n[c], 1.0f) : f32x8{};
-    bt[c] = n[c] ? load_param(beta, col, n[c], 0.0f) : f32x8{};
+    gm[c] = load_param<SHORT>(gamma, col, cols, n[c], 1.0f);
+    bt[c] = load_param<SHORT>(beta, col, cols, n[c], 0.0f);
   }
   int turn = 0;
   // (every wave of a workgroup makes the same number of turns: the sums hold barriers)
-  for (int64_t row0 = (int64_t)blockIdx.x * L::kRows; row0 < rows; row0 += (int64_t)gridDim.x * L::kRows) {
+  for (; row0 < rows; row0 += step) {
     const int64_t row = row0 + sub_row;
     const bool ok = row < rows;
+    Raw next;
+    if (row0 + step < rows) load(next, row + step);
     f32x8 v[NC];
     float s[1] = {0.0f};
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      v[c] = f32x8{};
-      if (!ok || !n[c]) continue;
       const int k = c * L::kSpan + lane;
-      const int64_t at = row * cols + k * 8;
-      v[c] = load_cols(x + at, n[c]);
-      f32x8 r = f32x8{};
-      if (res) r = load_cols(res + at, n[c]);
-      if (drop.hi | drop.lo) {
-        float factor[8];
-        dropout_factors(drop, mask_row_of(drop, (uint32_t)row), k, factor);
+      float factor[8];
+      if (masked) dropout_factors(drop, mask_row_of(drop, (uint32_t)min(row, rows - 1)), k, factor);
+      const f32x8 r = used_cols<SHORT, TR>(cur.res[c], n[c]);
+      v[c] = used_cols<SHORT, TX>(cur.x[c], n[c]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[c][e] = dropped_add(v[c][e], factor[e], r[e]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[c][e] += r[e];
+      for (int e = 0; e < 8; ++e) {
+        v[c][e] = masked ? dropped_add(v[c][e], factor[e], r[e]) : v[c][e] + r[e];
+        s[0] += e < n[c] ? v[c][e] : 0.0f;
       }
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (e < n[c]) s[0] += v[c][e];
-      store_cols(h + at, v[c], n[c]);
+      if (ok && n[c]) store_cols(h + row * cols + k * 8, v[c], n[c]);
     }
     row_sums<G, WPR>(s, slots, turn);
     const float mean = s[0] * inv_n;
@@ -136,28 +144,30 @@ __global__ __launch_bounds__((Lay<G, WPR>::kThreads)) void dropnorm_fwd_kernel(
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         v[c][e] -= mean;
-        if (e < n[c]) q[0] = __builtin_fmaf(v[c][e], v[c][e], q[0]);
+        q[0] = __builtin_fmaf(v[c][e], e < n[c] ? v[c][e] : 0.0f, q[0]);
       }
     row_sums<G, WPR>(q, slots, turn);
     const float rstd = rsqrtf(q[0] * inv_n + eps);
-    if (!ok) continue;
-    if (lane == 0) {
-      if (mean_out) mean_out[row] = mean;
-      if (rstd_out) rstd_out[row] = rstd;
-    }
+    if (ok) {
+      if (lane == 0) {
+        if (mean_out) mean_out[row] = mean;
+        if (rstd_out) rstd_out[row] = rstd;
+      }
 #pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      if (!n[c]) continue;
+      for (int c = 0; c < NC; ++c) {
+        if (!n[c]) continue;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[c][e] = __builtin_fmaf(v[c][e] * rstd, gm[c][e], bt[c][e]);
-      store_cols(y + row * cols + (c * L::kSpan + lane) * 8, v[c], n[c]);
+        for (int e = 0; e < 8; ++e) v[c][e] = __builtin_fmaf(v[c][e] * rstd, gm[c][e], bt[c][e]);
+        store_cols(y + row * cols + (c * L::kSpan + lane) * 8, v[c], n[c]);
+      }
     }
+    cur = next;
   }
 }
 
 // dy, dh, dx, dres may be null (a gradient that is not there is zero; one that is not wanted is not written); h is null
 // where the sum is to be formed again from x and the residual (null: none).
-template <typename TX, typename TR, int G, int WPR, int NC>
+template <typename TX, typename TR, int G, int WPR, int NC, bool SHORT>
 __global__ __launch_bounds__((Lay<G, WPR>::kThreads)) void dropnorm_bwd_kernel(
     const TX* __restrict__ dy, const TR* __restrict__ dh, const TX* __restrict__ x, const TR* __restrict__ res,
     const TR* __restrict__ h, const float* __restrict__ mean, const float* __restrict__ rstd, NormParam gamma, TX* __restrict__ dx,
@@ -168,52 +178,67 @@ __global__ __launch_bounds__((Lay<G, WPR>::kThreads)) void dropnorm_bwd_kernel(
   const float inv_n = 1.0f / (float)cols;
   drop = with_key(drop);
   const bool masked = (drop.hi | drop.lo) != 0, again = h == nullptr;
+  const TR* stream = again ? res : h;
+  struct Raw {
+    Raw8<TX> dy[NC], x[NC];
+    Raw8<TR> dh[NC], stream[NC];
+    float mean, rstd;
+  };
+  auto load = [&](Raw& raw, int64_t row) {
+    row = min(row, rows - 1);
+    const int64_t at = row * cols;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int col = (c * L::kSpan + lane) * 8;
+      raw.dy[c] = raw.x[c] = Raw8<TX>{};
+      raw.dh[c] = raw.stream[c] = Raw8<TR>{};
+      if (dy) raw.dy[c] = load_cols<SHORT>(dy + at, col, cols);
+      if (dh) raw.dh[c] = load_cols<SHORT>(dh + at, col, cols);
+      if (again) raw.x[c] = load_cols<SHORT>(x + at, col, cols);
+      if (stream) raw.stream[c] = load_cols<SHORT>(stream + at, col, cols);
+    }
+    raw.mean = mean[row];
+    raw.rstd = rstd[row];
+  };
+  const int64_t step = (int64_t)gridDim.x * L::kRows;
+  int64_t row0 = (int64_t)blockIdx.x * L::kRows;
+  Raw cur;
+  load(cur, row0 + sub_row);
   f32x8 gm[NC], dg[NC], db[NC];
   int n[NC];
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
     const int col = (c * L::kSpan + lane) * 8;
     n[c] = max(min(cols - col, 8), 0);
-    gm[c] = n[c] ? load_param(gamma, col, n[c], 1.0f) : f32x8{};
+    gm[c] = load_param<SHORT>(gamma, col, cols, n[c], 1.0f);
     dg[c] = db[c] = f32x8{};
   }
   int turn = 0;
-  for (int64_t row0 = (int64_t)blockIdx.x * L::kRows; row0 < rows; row0 += (int64_t)gridDim.x * L::kRows) {
+  for (; row0 < rows; row0 += step) {
     const int64_t row = row0 + sub_row;
     const bool ok = row < rows;
-    const float mu = ok ? mean[row] : 0.0f, rs = ok ? rstd[row] : 0.0f;
-    f32x8 xh[NC], d[NC], up[NC];
+    Raw next;
+    if (row0 + step < rows) load(next, row + step);
+    f32x8 xh[NC], d[NC];
     float factor[NC][8];
     float s[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      xh[c] = d[c] = up[c] = f32x8{};
-      if (!ok || !n[c]) continue;
       const int k = c * L::kSpan + lane;
-      const int64_t at = row * cols + k * 8;
-      if (dy) d[c] = load_cols(dy + at, n[c]);
-      if (dh) up[c] = load_cols(dh + at, n[c]);
-      f32x8 r = f32x8{};
+      if (masked) dropout_factors(drop, mask_row_of(drop, (uint32_t)min(row, rows - 1)), k, factor[c]);
+      // (columns and rows beyond the end: dy = 0 and a deviation of 0 keep them out of every sum)
+      const int have = ok ? n[c] : 0;
+      xh[c] = used_cols<SHORT, TR>(cur.stream[c], n[c]);
+      d[c] = used_cols<SHORT, TX>(cur.dy[c], n[c]);
       if (again) {
-        xh[c] = load_cols(x + at, n[c]);
-        if (res) r = load_cols(res + at, n[c]);
-      } else {
-        xh[c] = load_cols(h + at, n[c]);
-      }
-      if (masked) dropout_factors(drop, mask_row_of(drop, (uint32_t)row), k, factor[c]);
-      if (again) {
-        if (masked) {
+        const f32x8 u = used_cols<SHORT, TX>(cur.x[c], n[c]);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) xh[c][e] = dropped_add(xh[c][e], factor[c][e], r[e]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) xh[c][e] += r[e];
-        }
+        for (int e = 0; e < 8; ++e) xh[c][e] = masked ? dropped_add(u[e], factor[c][e], xh[c][e]) : u[e] + xh[c][e];
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        // (columns beyond the row's end: dy = 0 keeps them out of every sum)
-        xh[c][e] = (xh[c][e] - mu) * rs;
+        xh[c][e] = e < have ? (xh[c][e] - cur.mean) * cur.rstd : 0.0f;
+        d[c][e] = e < have ? d[c][e] : 0.0f;
         const float g = gm[c][e] * d[c][e];
         s[0] += g;
         s[1] = __builtin_fmaf(g, xh[c][e], s[1]);
@@ -227,9 +252,9 @@ __global__ __launch_bounds__((Lay<G, WPR>::kThreads)) void dropnorm_bwd_kernel(
     for (int c = 0; c < NC; ++c) {
       if (!ok || !n[c]) continue;
       const int64_t at = row * cols + (c * L::kSpan + lane) * 8;
+      const f32x8 up = used_cols<SHORT, TR>(cur.dh[c], n[c]);
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        d[c][e] = __builtin_fmaf(gm[c][e] * d[c][e] - a - xh[c][e] * b, rs, up[c][e]);
+      for (int e = 0; e < 8; ++e) d[c][e] = __builtin_fmaf(gm[c][e] * d[c][e] - a - xh[c][e] * b, cur.rstd, up[e]);
       if (dres) store_cols(dres + at, d[c], n[c]);
       if (dx) {
         if (masked) {
@@ -239,6 +264,7 @@ __global__ __launch_bounds__((Lay<G, WPR>::kThreads)) void dropnorm_bwd_kernel(
         store_cols(dx + at, d[c], n[c]);
       }
     }
+    cur = next;
   }
   if (!part) return;
   const int64_t parts = gridDim.x;
@@ -276,9 +302,10 @@ __global__ __launch_bounds__((Lay<G, WPR>::kThreads)) void dropnorm_bwd_kernel(
   }
 }
 
-// The first layout that holds a row's blocks of 8 columns: (lanes, waves, blocks per lane).
+// The first layout that holds a row's blocks of 8 columns: (lanes, waves, blocks per lane, fewer than 8 columns).
 #define PTX_DN_LAYOUTS(X) \
-  X(8, 1, 1) X(16, 1, 1) X(32, 1, 1) X(64, 1, 1) X(64, 2, 1) X(64, 4, 1) X(64, 8, 1) X(64, 16, 1) X(64, 16, 2) X(64, 16, 4)
+  X(8, 1, 1, true) X(8, 1, 1, false) X(16, 1, 1, false) X(32, 1, 1, false) X(64, 1, 1, false) X(64, 2, 1, false) X(64, 4, 1, false) \
+  X(64, 8, 1, false) X(64, 16, 1, false) X(64, 16, 2, false) X(64, 16, 4, false)
 constexpr int kDropnormCols = 32768;
 
 int dropnorm_max_cols() { return kDropnormCols; }
@@ -295,9 +322,9 @@ int dropnorm_fwd(const TX* x, const TR* res, const void* gamma, const void* beta
                  float* rstd, int64_t rows, int cols, float eps, const Dropout& drop, hipStream_t stream) {
   if (rows == 0) return 0;
   const int n_vec = (cols + 7) / 8;
-#define PTX_DN_CASE(G, WPR, NC)                                                                                              \
-  if (n_vec <= Lay<G, WPR>::kSpan * (NC)) {                                                                                  \
-    dropnorm_fwd_kernel<TX, TR, G, WPR, NC><<<dim3(walkers<G, WPR>(rows, 32)), dim3(Lay<G, WPR>::kThreads), 0, stream>>>(    \
+#define PTX_DN_CASE(G, WPR, NC, SHORT)                                                                                              \
+  if (SHORT ? cols < 8 : n_vec <= Lay<G, WPR>::kSpan * (NC)) {                                                                                  \
+    dropnorm_fwd_kernel<TX, TR, G, WPR, NC, SHORT><<<dim3(walkers<G, WPR>(rows, 32)), dim3(Lay<G, WPR>::kThreads), 0, stream>>>(    \
         x, res, NormParam{gamma, param_type}, NormParam{beta, param_type}, y, h, mean, rstd, rows, cols, eps, drop);                 \
     return 0;                                                                                                                \
   }
@@ -323,10 +350,10 @@ int dropnorm_bwd(const TX* dy, const TR* dh, const TX* x, const TR* res, const T
   const int n_vec = (cols + 7) / 8;
   int parts = 0;
   auto launch = [&]() {
-#define PTX_DN_CASE(G, WPR, NC)                                                                                               \
-  if (n_vec <= Lay<G, WPR>::kSpan * (NC)) {                                                                                   \
+#define PTX_DN_CASE(G, WPR, NC, SHORT)                                                                                               \
+  if (SHORT ? cols < 8 : n_vec <= Lay<G, WPR>::kSpan * (NC)) {                                                                                   \
     parts = walkers<G, WPR>(rows, kDropnormBwdWaves);                                                                         \
-    dropnorm_bwd_kernel<TX, TR, G, WPR, NC><<<dim3(parts), dim3(Lay<G, WPR>::kThreads), 0, stream>>>(                         \
+    dropnorm_bwd_kernel<TX, TR, G, WPR, NC, SHORT><<<dim3(parts), dim3(Lay<G, WPR>::kThreads), 0, stream>>>(                         \
         dy, dh, x, res, h, mean, rstd, NormParam{gamma, param_type}, dx, dres, part, rows, cols, drop);                           \
     return 0;                                                                                                                 \
   }

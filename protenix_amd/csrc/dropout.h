@@ -76,30 +76,51 @@ __device__ __forceinline__ float dropped_add(float x, float factor, float res) {
   return factor != 0.0f ? __builtin_fmaf(x, factor, res) : res;
 }
 
-// Eight columns at an element's alignment (rows of odd lengths): gfx950 takes vector accesses at any address, so an
-// odd row costs the lines it straddles and nothing else.  n: how many of the columns exist; the others read as 0.
+// Eight elements at an element's alignment (rows of odd lengths): gfx950 takes vector accesses at any address, so an
+// odd row costs the lines it straddles and nothing else.
 template <typename T> struct Unaligned8 { typedef T type __attribute__((ext_vector_type(8), aligned(sizeof(T)))); };
+template <typename T> using Raw8 = typename Unaligned8<T>::type;
 
-template <typename T> __device__ __forceinline__ f32x8 load_cols(const T* p, int n) {
-  typedef typename Unaligned8<T>::type V;
-  f32x8 out;
-  if (n >= 8) {
-    const V v = *reinterpret_cast<const V*>(p);
+template <typename T> __device__ __forceinline__ f32x8 widened(const Raw8<T>& v) {
+  f32x8 o;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) out[e] = (float)v[e];
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) out[e] = e < n ? (float)p[e] : 0.0f;
-  }
-  return out;
+  for (int e = 0; e < 8; ++e) o[e] = (float)v[e];
+  return o;
 }
-template <typename T> __device__ __forceinline__ void store_cols(T* p, f32x8 v, int n) {
-  typedef typename Unaligned8<T>::type V;
-  if (n >= 8) {
-    V o;
+template <typename T> __device__ __forceinline__ Raw8<T> rounded(const f32x8& v) {
+  Raw8<T> o;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] = (T)v[e];
-    *reinterpret_cast<V*>(p) = o;
+  for (int e = 0; e < 8; ++e) o[e] = (T)v[e];
+  return o;
+}
+
+// Columns col .. col + n - 1 of a row (n <= 8).  The load of a row's last, shorter block is moved back to where it ends with the
+// row, so that a load is one instruction without a branch (behind a branch the next load would wait for this one), and what it
+// brings is moved to its place when it is used.  Rows of fewer than 8 columns (SHORT) are read one by one.
+template <bool SHORT, typename T> __device__ __forceinline__ Raw8<T> load_cols(const T* row, int col, int cols) {
+  if constexpr (SHORT) {
+    Raw8<T> v;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = e < cols ? row[e] : (T)0.0f;
+    return v;
+  } else {
+    return *reinterpret_cast<const Raw8<T>*>(row + min(col, cols - 8));
+  }
+}
+template <bool SHORT, typename T> __device__ __forceinline__ f32x8 used_cols(const Raw8<T>& raw, int n) {
+  f32x8 v = widened<T>(raw);
+  if (!SHORT && n < 8) {
+    const int s = 8 - n;
+#pragma unroll
+    for (int step = 4; step >= 1; step >>= 1)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = s & step ? (e + step < 8 ? v[e + step] : 0.0f) : v[e];
+  }
+  return v;
+}
+template <typename T> __device__ __forceinline__ void store_cols(T* p, const f32x8& v, int n) {
+  if (n >= 8) {
+    *reinterpret_cast<Raw8<T>*>(p) = rounded<T>(v);
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e)

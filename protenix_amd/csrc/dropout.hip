@@ -9,48 +9,76 @@
 
 namespace ptx {
 
-// TI: type of x; TO: of the residual and the sum.
-template <typename TI, typename TO, bool RES>
+// TI: type of x; TO: of the residual and the sum.  AHEAD: rows requested before the first is worked on (1: a mask row is
+// one row).  SHORT: fewer than 8 columns.
+template <typename TI, typename TO, bool RES, int AHEAD, bool SHORT>
 __global__ __launch_bounds__(256) void dropout_add_kernel(const TI* __restrict__ x, const TO* __restrict__ res, TO* __restrict__ out,
-                                                          int cols, uint32_t n_vec, int64_t n_blocks, int rows_at_once, Dropout drop) {
+                                                          int cols, uint32_t n_vec, int64_t n_blocks, uint32_t rows_at_once, Dropout drop) {
   const bool masked = (drop.hi | drop.lo) != 0;
   drop = with_key(drop);
   for (int64_t block = (int64_t)blockIdx.x * 256 + threadIdx.x; block < n_blocks; block += (int64_t)gridDim.x * 256) {
     const uint32_t mask_row = (uint32_t)(block / n_vec), k = (uint32_t)(block - (int64_t)mask_row * n_vec);
-    const uint32_t outer = mask_row / drop.inner, in = mask_row - outer * drop.inner;
-    const uint32_t s0 = blockIdx.y * rows_at_once, s1 = min(s0 + rows_at_once, drop.shared);
+    const uint32_t outer = AHEAD == 1 ? mask_row : mask_row / drop.inner, in = AHEAD == 1 ? 0 : mask_row - outer * drop.inner;
+    const uint32_t s0 = AHEAD == 1 ? 0 : blockIdx.y * rows_at_once, s1 = AHEAD == 1 ? 1 : min(s0 + rows_at_once, drop.shared);
     const int n = min(cols - (int)(k * 8), 8);
-    float factor[8] = {1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f};
-    if (masked) dropout_factors(drop, mask_row, k, factor);
-    const int64_t step = (int64_t)drop.inner * cols;
-    int64_t at = (((int64_t)outer * drop.shared + s0) * drop.inner + in) * cols + k * 8;
-    for (uint32_t s = s0; s < s1; ++s, at += step) {
-      f32x8 v = load_cols(x + at, n);
-      if (RES) {
-        const f32x8 r = load_cols(res + at, n);
+    float factor[8];
+    const int64_t step = AHEAD == 1 ? 0 : (int64_t)drop.inner * cols;
+    int64_t at = AHEAD == 1 ? (int64_t)mask_row * cols : (((int64_t)outer * drop.shared + s0) * drop.inner + in) * cols;
+    for (uint32_t s = s0; s < s1; s += AHEAD) {
+      Raw8<TI> raw[AHEAD];
+      Raw8<TO> raw_res[AHEAD];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = dropped_add(v[e], factor[e], r[e]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = dropped(v[e], factor[e]);
+      for (uint32_t r = 0; r < AHEAD; ++r) {
+        const int64_t row = at + (s + r < s1 ? r : s1 - 1 - s) * step;      // (beyond the last: that one once more)
+        raw[r] = load_cols<SHORT>(x + row, k * 8, cols);
+        if (RES) raw_res[r] = load_cols<SHORT>(res + row, k * 8, cols);
       }
-      store_cols(out + at, v, n);
+      if (s == s0) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) factor[e] = 1.0f;
+        if (masked) dropout_factors(drop, mask_row, k, factor);
+      }
+#pragma unroll
+      for (uint32_t r = 0; r < AHEAD; ++r) {
+        if (s + r >= s1) break;
+        f32x8 v = used_cols<SHORT, TI>(raw[r], n);
+        if (RES) {
+          const f32x8 y = used_cols<SHORT, TO>(raw_res[r], n);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = dropped_add(v[e], factor[e], y[e]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = dropped(v[e], factor[e]);
+        }
+        store_cols(out + at + k * 8, v, n);
+        at += step;
+      }
     }
   }
+}
+
+template <typename TI, typename TO, bool RES>
+static void launch(const TI* x, const TO* res, TO* out, int64_t rows, int cols, const Dropout& drop, hipStream_t stream) {
+  const uint32_t n_vec = (uint32_t)((cols + 7) / 8);
+  const int64_t n_blocks = rows / drop.shared * n_vec;
+  const uint32_t at_once = std::min<uint32_t>(drop.shared, std::max<uint32_t>(8, (drop.shared + 65534) / 65535));
+  // (2^32 threads at most along a grid's axis)
+  const dim3 grid((unsigned)std::min<int64_t>((n_blocks + 255) / 256, 1 << 23), (drop.shared + at_once - 1) / at_once);
+  if (cols < 8 && drop.shared == 1)
+    dropout_add_kernel<TI, TO, RES, 1, true><<<grid, dim3(256), 0, stream>>>(x, res, out, cols, n_vec, n_blocks, at_once, drop);
+  else if (cols < 8)
+    dropout_add_kernel<TI, TO, RES, 4, true><<<grid, dim3(256), 0, stream>>>(x, res, out, cols, n_vec, n_blocks, at_once, drop);
+  else if (drop.shared == 1)
+    dropout_add_kernel<TI, TO, RES, 1, false><<<grid, dim3(256), 0, stream>>>(x, res, out, cols, n_vec, n_blocks, at_once, drop);
+  else
+    dropout_add_kernel<TI, TO, RES, 4, false><<<grid, dim3(256), 0, stream>>>(x, res, out, cols, n_vec, n_blocks, at_once, drop);
 }
 
 template <typename TI, typename TO>
 int dropout_add(const TI* x, const TO* res, TO* out, int64_t rows, int cols, const Dropout& drop, hipStream_t stream) {
   if (rows == 0) return 0;
-  const uint32_t n_vec = (uint32_t)((cols + 7) / 8);
-  const int64_t n_blocks = rows / drop.shared * n_vec, groups = (n_blocks + 255) / 256;
-  const int at_once = std::min<int>(drop.shared, std::max(8, (int)((drop.shared + 65534) / 65535)));
-  // (2^32 threads at most along a grid's axis)
-  const dim3 grid((unsigned)std::min<int64_t>(groups, 1 << 23), (drop.shared + at_once - 1) / at_once);
-  if (res)
-    dropout_add_kernel<TI, TO, true><<<grid, dim3(256), 0, stream>>>(x, res, out, cols, n_vec, n_blocks, at_once, drop);
-  else
-    dropout_add_kernel<TI, TO, false><<<grid, dim3(256), 0, stream>>>(x, nullptr, out, cols, n_vec, n_blocks, at_once, drop);
+  if (res) launch<TI, TO, true>(x, res, out, rows, cols, drop, stream);
+  else launch<TI, TO, false>(x, nullptr, out, rows, cols, drop, stream);
   return 0;
 }
 
