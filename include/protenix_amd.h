@@ -597,7 +597,7 @@ PTX_API int ptx_dropout_add(const void* x, const void* residual, void* out, int6
  *   y            [rows][cols], x_dtype;  h [rows][cols], stream_dtype (x_dtype where there is no residual)
  *   gamma, beta  [cols], param_dtype, either may be NULL
  *   mean, rstd   fp32 [rows], each may be NULL: of the sum before it is rounded to h
- * x_dtype = stream_dtype, or 16-bit x beside an fp32 stream; at most 32768 columns.  y may alias x, h the residual;
+ * x_dtype = stream_dtype, or 16-bit x beside an fp32 stream; at most 16384 columns.  y may alias x, h the residual;
  * every other pair must not overlap.
  */
 PTX_API int ptx_dropout_add_layernorm_fwd(const void* x, const void* residual, const void* gamma, const void* beta,
@@ -608,8 +608,8 @@ PTX_API int ptx_dropout_add_layernorm_fwd(const void* x, const void* residual, c
 /*
  * Its gradients, from dy (x_dtype) and dh (stream_dtype; either may be NULL: zero).  dx (x_dtype), dresidual (stream_dtype),
  * dgamma and dbeta (param_dtype) are written where given; dgamma / dbeta need the workspace (uninitialised fp32).
- * h: the forward's where stream_dtype is PTX_F32.  NULL: h is formed again from x and the residual (NULL: none), as it must be
- * for 16-bit streams, whose rounded h would cost dgamma its accuracy.  No atomics: the sums' order is fixed.
+ * An fp32 stream takes the forward's h (x and residual are not read); a 16-bit one x and the residual (NULL: none), from which h is
+ * formed again: its rounded value would cost dgamma its accuracy.  No atomics: the sums' order is fixed.
  */
 PTX_API int64_t ptx_dropout_add_layernorm_bwd_workspace_elems(int64_t rows, int cols);
 PTX_API int ptx_dropout_add_layernorm_bwd(const void* dy, const void* dh, const void* x, const void* residual,

@@ -1227,7 +1227,8 @@ PTX_API int ptx_dropout_add_layernorm_bwd(const void* dy, const void* dh, const 
   if (rc != PTX_OK) return rc;
   PTX_REQUIRE(rows == 0 || !(dgamma || dbeta) || workspace, PTX_ERR_BAD_ARG, "dropout_add_layernorm_bwd: dgamma / dbeta need the workspace");
   if (rows == 0 && !dgamma && !dbeta) return PTX_OK;
-  PTX_REQUIRE(rows == 0 || ((h || x) && mean && rstd), PTX_ERR_BAD_ARG, "dropout_add_layernorm_bwd: null pointer");
+  PTX_REQUIRE(rows == 0 || ((stream_dtype == PTX_F32 ? h : x) && mean && rstd), PTX_ERR_BAD_ARG,
+              "dropout_add_layernorm_bwd: null pointer (an fp32 stream needs h, a 16-bit one x)");
   PTX_DISPATCH_STREAM(x_dtype, stream_dtype,
                       (ptx::dropnorm_bwd<TX, TR>)((const TX*)dy, (const TR*)dh, (const TX*)x, (const TR*)residual, (const TR*)h, mean, rstd,
                                                   gamma, param_dtype, (TX*)dx, (TR*)dresidual, dgamma, dbeta, workspace, rows, cols, d,

@@ -5,9 +5,9 @@
 //              dres = rstd (g - avg(g) - xh avg(g xh)) + dh,  dx = m dres,
 //              dgamma = sum_rows dy xh,  dbeta = sum_rows dy
 //
-// A row lies over its lanes in registers, one block of 8 columns per lane (= one draw of the mask, see dropout.h), two or
-// four blocks for rows of more than 8192 columns: G lanes of a wave for up to 512 columns, WPR waves of a workgroup beyond, whose sums
-// meet in LDS.  Statistics are fp32 and taken in two passes over the registers, from the sum before it is rounded to h.
+// A row lies over its lanes in registers, one block of 8 columns per lane (= one draw of the mask, see dropout.h), two for
+// rows of more than 8192 columns: G lanes of a wave for up to 512 columns, as many waves of a workgroup as hold it
+// beyond, whose sums meet in LDS.  Statistics are fp32 and taken in two passes over the registers, from the sum before it is rounded to h.
 // The backward pass takes h from memory where it is fp32, and forms it again from x and the residual where the stream
 // has 16 bits: xh of a rounded h would leave dgamma with an error of 2^-9 instead of 2^-24, for the sake of one
 // 16-bit read.  dgamma and dbeta: column sums in registers over the rows a workgroup walks, one row of fp32 partial sums
@@ -41,32 +41,42 @@ template <int G> __device__ __forceinline__ float lanes_sum(float v) {
   return v;
 }
 
-// Sums over the lanes of a row: within G lanes, or over the WPR waves of a workgroup through one of the slots (a slot is
+// Sums over the lanes of a row: within G lanes, or (WAVES > 1) over the waves of a workgroup through one of the slots (a slot is
 // used again two exchanges later, when every wave has passed the barrier of the exchange between).
-template <int G, int WPR, int N> __device__ __forceinline__ void row_sums(float (&v)[N], float (*slots)[16][2], int& turn) {
+template <int WAVES> struct Slots {
+  f32x4 sum[2][2][WAVES > 1 ? WAVES / 4 : 1];   // [exchange][value][wave]
+};
+// (waves that a workgroup does not have count as 0)
+template <int WAVES> __device__ __forceinline__ void clear(Slots<WAVES>& s) {
+  if (WAVES > 1 && threadIdx.x < 4 * WAVES && (int)(threadIdx.x % WAVES) >= (int)(blockDim.x >> 6)) ((float*)s.sum)[threadIdx.x] = 0.0f;
+}
+template <int G, int WAVES, int N> __device__ __forceinline__ void row_sums(float (&v)[N], Slots<WAVES>& slots, int& turn) {
 #pragma unroll
   for (int i = 0; i < N; ++i) v[i] = lanes_sum<G>(v[i]);
-  if constexpr (WPR > 1) {
-    float(*s)[2] = slots[turn];
+  if constexpr (WAVES > 1) {
+    f32x4(*s)[WAVES / 4] = slots.sum[turn];
     turn ^= 1;
     if ((threadIdx.x & 63) == 0)
 #pragma unroll
-      for (int i = 0; i < N; ++i) s[threadIdx.x >> 6][i] = v[i];
+      for (int i = 0; i < N; ++i) ((float*)s[i])[threadIdx.x >> 6] = v[i];
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       float t = 0.0f;
 #pragma unroll
-      for (int w = 0; w < WPR; ++w) t += s[w][i];
+      for (int w = 0; w < WAVES / 4; ++w) t += (s[i][w][0] + s[i][w][1]) + (s[i][w][2] + s[i][w][3]);
       v[i] = t;
     }
   }
 }
 
-template <int G, int WPR> struct Lay {
-  static constexpr int kThreads = WPR == 1 ? 256 : 64 * WPR;
-  static constexpr int kRows = WPR == 1 ? 256 / G : 1;       // rows a workgroup holds at once
-  static constexpr int kSpan = WPR == 1 ? G : 64 * WPR;      // lanes of a row
+// WAVES = 1: four waves to a workgroup, 64 / G rows to a wave.  Else a row to a workgroup of up to WAVES waves.
+template <int G, int WAVES> struct Lay {
+  static constexpr int kThreads = WAVES == 1 ? 256 : 64 * WAVES;
+  static constexpr int kRows = WAVES == 1 ? 256 / G : 1;       // rows a workgroup holds at once
+  static __device__ __forceinline__ int span() { return WAVES == 1 ? G : (int)blockDim.x; }      // lanes of a row
+  static __device__ __forceinline__ int lane() { return WAVES == 1 ? threadIdx.x % G : threadIdx.x; }
+  static __device__ __forceinline__ int sub_row() { return WAVES == 1 ? threadIdx.x / G : 0; }
 };
 
 __device__ __forceinline__ uint32_t mask_row_of(const Dropout& d, uint32_t row) {
@@ -75,68 +85,59 @@ __device__ __forceinline__ uint32_t mask_row_of(const Dropout& d, uint32_t row) 
   return o * d.inner + row % d.inner;
 }
 
-// TX: type of x and y; TR: of the residual and h.  SHORT: fewer than 8 columns.
-template <typename TX, typename TR, int G, int WPR, int NC, bool SHORT>
-__global__ __launch_bounds__((Lay<G, WPR>::kThreads)) void dropnorm_fwd_kernel(
+// TX: type of x and y; TR: of the residual and h.  SHORT: fewer than 8 columns.  RES: with a residual.
+template <typename TX, typename TR, int G, int WAVES, int NC, bool SHORT, bool RES>
+__global__ __launch_bounds__((Lay<G, WAVES>::kThreads)) void dropnorm_fwd_kernel(
     const TX* __restrict__ x, const TR* __restrict__ res, NormParam gamma, NormParam beta, TX* __restrict__ y, TR* __restrict__ h,
     float* __restrict__ mean_out, float* __restrict__ rstd_out, int64_t rows, int cols, float eps, Dropout drop) {
-  typedef Lay<G, WPR> L;
-  __shared__ float slots[2][16][2];
-  const int lane = threadIdx.x % L::kSpan, sub_row = threadIdx.x / L::kSpan;
+  typedef Lay<G, WAVES> L;
+  __shared__ Slots<WAVES> slots;
+  clear(slots);
+  const int span = L::span(), lane = L::lane(), sub_row = L::sub_row();
   const float inv_n = 1.0f / (float)cols;
-  const bool masked = (drop.hi | drop.lo) != 0;
   drop = with_key(drop);
-  struct Raw {
-    Raw8<TX> x[NC];
-    Raw8<TR> res[NC];
-  };
-  // (rows and columns beyond the end: the last ones once more, not used)
-  auto load = [&](Raw& raw, int64_t row) {
-    const int64_t at = min(row, rows - 1) * cols;
-#pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      raw.x[c] = load_cols<SHORT>(x + at, (c * L::kSpan + lane) * 8, cols);
-      raw.res[c] = Raw8<TR>{};
-      if (res) raw.res[c] = load_cols<SHORT>(res + at, (c * L::kSpan + lane) * 8, cols);
-    }
-  };
-  const int64_t step = (int64_t)gridDim.x * L::kRows;
-  int64_t row0 = (int64_t)blockIdx.x * L::kRows;
-  Raw cur;
-  load(cur, row0 + sub_row);
   f32x8 gm[NC], bt[NC];
   int n[NC];
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
-    const int col = (c * L::kSpan + lane) * 8;
+    const int col = (c * span + lane) * 8;
     n[c] = max(min(cols - col, 8), 0);
     gm[c] = load_param<SHORT>(gamma, col, cols, n[c], 1.0f);
     bt[c] = load_param<SHORT>(beta, col, cols, n[c], 0.0f);
   }
   int turn = 0;
   // (every wave of a workgroup makes the same number of turns: the sums hold barriers)
-  for (; row0 < rows; row0 += step) {
-    const int64_t row = row0 + sub_row;
-    const bool ok = row < rows;
-    Raw next;
-    if (row0 + step < rows) load(next, row + step);
+  for (int64_t row0 = (int64_t)blockIdx.x * L::kRows; row0 < rows; row0 += (int64_t)gridDim.x * L::kRows) {
+    // (rows and columns beyond the end: the last ones once more, not used)
+    const int64_t row = min(row0 + sub_row, rows - 1);
+    const bool ok = row0 + sub_row < rows;
+    // The mask first: waves that draw while others load keep the memory busier than loads that run ahead of it, or a row ahead, do
+    // (4110 rows of 1035 fp32: 15.6 us, 17.5 and 18.6).
+    uint32_t keeps[NC];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) keeps[c] = dropout_keeps(drop, mask_row_of(drop, (uint32_t)row), c * span + lane);
+    Raw8<TX> raw_x[NC];
+    Raw8<TR> raw_res[NC];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      raw_x[c] = load_cols<SHORT>(x + row * cols, (c * span + lane) * 8, cols);
+      if (RES) raw_res[c] = load_cols<SHORT>(res + row * cols, (c * span + lane) * 8, cols);
+    }
     f32x8 v[NC];
     float s[1] = {0.0f};
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      const int k = c * L::kSpan + lane;
-      float factor[8];
-      if (masked) dropout_factors(drop, mask_row_of(drop, (uint32_t)min(row, rows - 1)), k, factor);
-      const f32x8 r = used_cols<SHORT, TR>(cur.res[c], n[c]);
-      v[c] = used_cols<SHORT, TX>(cur.x[c], n[c]);
+      f32x8 r = f32x8{};
+      if (RES) r = used_cols<SHORT, TR>(raw_res[c], n[c]);
+      v[c] = used_cols<SHORT, TX>(raw_x[c], n[c]);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        v[c][e] = masked ? dropped_add(v[c][e], factor[e], r[e]) : v[c][e] + r[e];
+        v[c][e] = __builtin_fmaf(kept(v[c][e], keeps[c], e), drop.scale, r[e]);
         s[0] += e < n[c] ? v[c][e] : 0.0f;
       }
-      if (ok && n[c]) store_cols(h + row * cols + k * 8, v[c], n[c]);
+      if (ok && n[c]) store_cols(h + row * cols + (c * span + lane) * 8, v[c], n[c]);
     }
-    row_sums<G, WPR>(s, slots, turn);
+    row_sums<G, WAVES>(s, slots, turn);
     const float mean = s[0] * inv_n;
     float q[1] = {0.0f};
 #pragma unroll
@@ -146,99 +147,87 @@ __global__ __launch_bounds__((Lay<G, WPR>::kThreads)) void dropnorm_fwd_kernel(
         v[c][e] -= mean;
         q[0] = __builtin_fmaf(v[c][e], e < n[c] ? v[c][e] : 0.0f, q[0]);
       }
-    row_sums<G, WPR>(q, slots, turn);
+    row_sums<G, WAVES>(q, slots, turn);
     const float rstd = rsqrtf(q[0] * inv_n + eps);
-    if (ok) {
-      if (lane == 0) {
-        if (mean_out) mean_out[row] = mean;
-        if (rstd_out) rstd_out[row] = rstd;
-      }
-#pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        if (!n[c]) continue;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[c][e] = __builtin_fmaf(v[c][e] * rstd, gm[c][e], bt[c][e]);
-        store_cols(y + row * cols + (c * L::kSpan + lane) * 8, v[c], n[c]);
-      }
+    if (!ok) continue;
+    if (lane == 0) {
+      if (mean_out) mean_out[row] = mean;
+      if (rstd_out) rstd_out[row] = rstd;
     }
-    cur = next;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      if (!n[c]) continue;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[c][e] = __builtin_fmaf(v[c][e] * rstd, gm[c][e], bt[c][e]);
+      store_cols(y + row * cols + (c * span + lane) * 8, v[c], n[c]);
+    }
   }
 }
 
-// dy, dh, dx, dres may be null (a gradient that is not there is zero; one that is not wanted is not written); h is null
-// where the sum is to be formed again from x and the residual (null: none).
-template <typename TX, typename TR, int G, int WPR, int NC, bool SHORT>
-__global__ __launch_bounds__((Lay<G, WPR>::kThreads)) void dropnorm_bwd_kernel(
+// dy, dh, dx, dres may be null (a gradient that is not there is zero; one that is not wanted is not written).  With a stream of
+// 16 bits h is formed again from x and the residual (null: none), else it is read and x and res are not.
+template <typename TX, typename TR, int G, int WAVES, int NC, bool SHORT>
+__global__ __launch_bounds__((Lay<G, WAVES>::kThreads)) void dropnorm_bwd_kernel(
     const TX* __restrict__ dy, const TR* __restrict__ dh, const TX* __restrict__ x, const TR* __restrict__ res,
     const TR* __restrict__ h, const float* __restrict__ mean, const float* __restrict__ rstd, NormParam gamma, TX* __restrict__ dx,
     TR* __restrict__ dres, float* __restrict__ part, int64_t rows, int cols, Dropout drop) {
-  typedef Lay<G, WPR> L;
-  __shared__ float slots[2][16][2];
-  const int lane = threadIdx.x % L::kSpan, sub_row = threadIdx.x / L::kSpan;
+  typedef Lay<G, WAVES> L;
+  constexpr bool AGAIN = sizeof(TR) == 2;
+  __shared__ Slots<WAVES> slots;
+  clear(slots);
+  const int span = L::span(), lane = L::lane(), sub_row = L::sub_row();
   const float inv_n = 1.0f / (float)cols;
   drop = with_key(drop);
-  const bool masked = (drop.hi | drop.lo) != 0, again = h == nullptr;
-  const TR* stream = again ? res : h;
-  struct Raw {
-    Raw8<TX> dy[NC], x[NC];
-    Raw8<TR> dh[NC], stream[NC];
-    float mean, rstd;
-  };
-  auto load = [&](Raw& raw, int64_t row) {
-    row = min(row, rows - 1);
-    const int64_t at = row * cols;
-#pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      const int col = (c * L::kSpan + lane) * 8;
-      raw.dy[c] = raw.x[c] = Raw8<TX>{};
-      raw.dh[c] = raw.stream[c] = Raw8<TR>{};
-      if (dy) raw.dy[c] = load_cols<SHORT>(dy + at, col, cols);
-      if (dh) raw.dh[c] = load_cols<SHORT>(dh + at, col, cols);
-      if (again) raw.x[c] = load_cols<SHORT>(x + at, col, cols);
-      if (stream) raw.stream[c] = load_cols<SHORT>(stream + at, col, cols);
-    }
-    raw.mean = mean[row];
-    raw.rstd = rstd[row];
-  };
-  const int64_t step = (int64_t)gridDim.x * L::kRows;
-  int64_t row0 = (int64_t)blockIdx.x * L::kRows;
-  Raw cur;
-  load(cur, row0 + sub_row);
+  // (what is not there is read from where something is, and not used: loads without a branch wait for one another least)
+  const TR* some = AGAIN ? (const TR*)x : h;
+  const bool have_dy = dy, have_dh = dh, have_res = res;
+  if (!have_dy) dy = (const TX*)some;
+  if (!have_dh) dh = some;
+  const TR* stream = AGAIN ? (have_res ? res : some) : h;
   f32x8 gm[NC], dg[NC], db[NC];
   int n[NC];
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
-    const int col = (c * L::kSpan + lane) * 8;
+    const int col = (c * span + lane) * 8;
     n[c] = max(min(cols - col, 8), 0);
     gm[c] = load_param<SHORT>(gamma, col, cols, n[c], 1.0f);
     dg[c] = db[c] = f32x8{};
   }
   int turn = 0;
-  for (; row0 < rows; row0 += step) {
-    const int64_t row = row0 + sub_row;
-    const bool ok = row < rows;
-    Raw next;
-    if (row0 + step < rows) load(next, row + step);
+  for (int64_t row0 = (int64_t)blockIdx.x * L::kRows; row0 < rows; row0 += (int64_t)gridDim.x * L::kRows) {
+    const int64_t row = min(row0 + sub_row, rows - 1);
+    const bool ok = row0 + sub_row < rows;
+    Raw8<TX> raw_dy[NC], raw_x[NC];
+    Raw8<TR> raw_dh[NC], raw_stream[NC];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int col = (c * span + lane) * 8;
+      raw_stream[c] = load_cols<SHORT>(stream + row * cols, col, cols);
+      if (AGAIN) raw_x[c] = load_cols<SHORT>(x + row * cols, col, cols);
+      raw_dy[c] = load_cols<SHORT>(dy + row * cols, col, cols);
+      raw_dh[c] = load_cols<SHORT>(dh + row * cols, col, cols);
+    }
+    const float mu = mean[row], rs = rstd[row];
     f32x8 xh[NC], d[NC];
-    float factor[NC][8];
+    uint32_t keeps[NC];
     float s[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      const int k = c * L::kSpan + lane;
-      if (masked) dropout_factors(drop, mask_row_of(drop, (uint32_t)min(row, rows - 1)), k, factor[c]);
+      keeps[c] = dropout_keeps(drop, mask_row_of(drop, (uint32_t)row), c * span + lane);
       // (columns and rows beyond the end: dy = 0 and a deviation of 0 keep them out of every sum)
-      const int have = ok ? n[c] : 0;
-      xh[c] = used_cols<SHORT, TR>(cur.stream[c], n[c]);
-      d[c] = used_cols<SHORT, TX>(cur.dy[c], n[c]);
-      if (again) {
-        const f32x8 u = used_cols<SHORT, TX>(cur.x[c], n[c]);
+      const int have = ok ? n[c] : 0, have_d = have_dy ? have : 0;
+      xh[c] = used_cols<SHORT, TR>(raw_stream[c], n[c]);
+      d[c] = used_cols<SHORT, TX>(raw_dy[c], n[c]);
+      if (AGAIN) {
+        const f32x8 u = used_cols<SHORT, TX>(raw_x[c], n[c]);
+        if (!have_res) xh[c] = f32x8{};
 #pragma unroll
-        for (int e = 0; e < 8; ++e) xh[c][e] = masked ? dropped_add(u[e], factor[c][e], xh[c][e]) : u[e] + xh[c][e];
+        for (int e = 0; e < 8; ++e) xh[c][e] = __builtin_fmaf(kept(u[e], keeps[c], e), drop.scale, xh[c][e]);
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        xh[c][e] = e < have ? (xh[c][e] - cur.mean) * cur.rstd : 0.0f;
-        d[c][e] = e < have ? d[c][e] : 0.0f;
+        xh[c][e] = e < have ? (xh[c][e] - mu) * rs : 0.0f;
+        d[c][e] = e < have_d ? d[c][e] : 0.0f;
         const float g = gm[c][e] * d[c][e];
         s[0] += g;
         s[1] = __builtin_fmaf(g, xh[c][e], s[1]);
@@ -246,33 +235,30 @@ __global__ __launch_bounds__((Lay<G, WPR>::kThreads)) void dropnorm_bwd_kernel(
         db[c][e] += d[c][e];
       }
     }
-    row_sums<G, WPR>(s, slots, turn);
+    row_sums<G, WAVES>(s, slots, turn);
     const float a = s[0] * inv_n, b = s[1] * inv_n;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       if (!ok || !n[c]) continue;
-      const int64_t at = row * cols + (c * L::kSpan + lane) * 8;
-      const f32x8 up = used_cols<SHORT, TR>(cur.dh[c], n[c]);
+      const int64_t at = row * cols + (c * span + lane) * 8;
+      const f32x8 up = used_cols<SHORT, TR>(raw_dh[c], n[c]);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) d[c][e] = __builtin_fmaf(gm[c][e] * d[c][e] - a - xh[c][e] * b, cur.rstd, up[e]);
+      for (int e = 0; e < 8; ++e) d[c][e] = __builtin_fmaf(gm[c][e] * d[c][e] - a - xh[c][e] * b, rs, have_dh ? up[e] : 0.0f);
       if (dres) store_cols(dres + at, d[c], n[c]);
       if (dx) {
-        if (masked) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) d[c][e] = dropped(d[c][e], factor[c][e]);
-        }
+        for (int e = 0; e < 8; ++e) d[c][e] = kept(d[c][e], keeps[c], e) * drop.scale;
         store_cols(dx + at, d[c], n[c]);
       }
     }
-    cur = next;
   }
   if (!part) return;
   const int64_t parts = gridDim.x;
   float* out[2] = {part + (int64_t)blockIdx.x * cols, part + (parts + blockIdx.x) * cols};
-  if constexpr (WPR > 1) {
+  if constexpr (WAVES > 1) {
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      const int col = (c * L::kSpan + lane) * 8;
+      const int col = (c * span + lane) * 8;
       if (!n[c]) continue;
       store_cols(out[0] + col, dg[c], n[c]);
       store_cols(out[1] + col, db[c], n[c]);
@@ -302,43 +288,53 @@ __global__ __launch_bounds__((Lay<G, WPR>::kThreads)) void dropnorm_bwd_kernel(
   }
 }
 
-// The first layout that holds a row's blocks of 8 columns: (lanes, waves, blocks per lane, fewer than 8 columns).
+// The first layout that holds a row's blocks of 8 columns: (lanes, waves at most, blocks per lane, fewer than 8 columns).
 #define PTX_DN_LAYOUTS(X) \
-  X(8, 1, 1, true) X(8, 1, 1, false) X(16, 1, 1, false) X(32, 1, 1, false) X(64, 1, 1, false) X(64, 2, 1, false) X(64, 4, 1, false) \
-  X(64, 8, 1, false) X(64, 16, 1, false) X(64, 16, 2, false) X(64, 16, 4, false)
-constexpr int kDropnormCols = 32768;
+  X(8, 1, 1, true) X(8, 1, 1, false) X(16, 1, 1, false) X(32, 1, 1, false) X(64, 1, 1, false) X(64, 8, 1, false) X(64, 16, 1, false) \
+  X(64, 16, 2, false)
+constexpr int kDropnormCols = 16384;
 
 int dropnorm_max_cols() { return kDropnormCols; }
 
-// Workgroups that walk the rows: rows of up to 512 columns a wave or less each, 8 workgroups of four waves per compute unit; longer ones
-// as many waves.
-template <int G, int WPR> static int walkers(int64_t rows, int waves_per_cu) {
-  const int64_t most = std::max(1, 256 * waves_per_cu / (Lay<G, WPR>::kThreads / 64));
-  return (int)std::min<int64_t>((rows + Lay<G, WPR>::kRows - 1) / Lay<G, WPR>::kRows, most);
+// A launch's shape: workgroups of one row in the fewest waves that hold it, or of four waves of rows, which walk the rows: as many as
+// `waves_per_cu` on each of the 256 compute units, or as have `turns` turns to make (but one per compute unit).
+struct Walk {
+  int groups, threads;
+};
+template <int G, int WAVES, int NC> static Walk walk(int64_t rows, int n_vec, int waves_per_cu, int turns) {
+  Walk w;
+  w.threads = WAVES == 1 ? 256 : (n_vec + 64 * NC - 1) / (64 * NC) * 64;
+  const int64_t batches = (rows + Lay<G, WAVES>::kRows - 1) / Lay<G, WAVES>::kRows;
+  w.groups = (int)std::min<int64_t>({batches, std::max<int64_t>(256, batches / turns), std::max(1, 256 * waves_per_cu / (w.threads / 64))});
+  return w;
 }
+#define PTX_DN_FITS(G, WAVES, NC, SHORT) (SHORT ? cols < 8 : n_vec <= G * WAVES * NC)
 
 template <typename TX, typename TR>
 int dropnorm_fwd(const TX* x, const TR* res, const void* gamma, const void* beta, int param_type, TX* y, TR* h, float* mean,
                  float* rstd, int64_t rows, int cols, float eps, const Dropout& drop, hipStream_t stream) {
   if (rows == 0) return 0;
   const int n_vec = (cols + 7) / 8;
-#define PTX_DN_CASE(G, WPR, NC, SHORT)                                                                                              \
-  if (SHORT ? cols < 8 : n_vec <= Lay<G, WPR>::kSpan * (NC)) {                                                                                  \
-    dropnorm_fwd_kernel<TX, TR, G, WPR, NC, SHORT><<<dim3(walkers<G, WPR>(rows, 32)), dim3(Lay<G, WPR>::kThreads), 0, stream>>>(    \
-        x, res, NormParam{gamma, param_type}, NormParam{beta, param_type}, y, h, mean, rstd, rows, cols, eps, drop);                 \
-    return 0;                                                                                                                \
+#define PTX_DN_CASE(G, WAVES, NC, SHORT)                                                                              \
+  if (PTX_DN_FITS(G, WAVES, NC, SHORT)) {                                                                             \
+    const Walk w = walk<G, WAVES, NC>(rows, n_vec, 32, 1);                                                            \
+    auto* kernel = res ? dropnorm_fwd_kernel<TX, TR, G, WAVES, NC, SHORT, true> : dropnorm_fwd_kernel<TX, TR, G, WAVES, NC, SHORT, false>; \
+    kernel<<<dim3(w.groups), dim3(w.threads), 0, stream>>>(x, res, NormParam{gamma, param_type}, NormParam{beta, param_type}, y, h,    \
+                                                           mean, rstd, rows, cols, eps, drop);                        \
+    return 0;                                                                                                         \
   }
   PTX_DN_LAYOUTS(PTX_DN_CASE)
 #undef PTX_DN_CASE
   return 1;
 }
 
-constexpr int kDropnormBwdWaves = 16;   // waves per compute unit = 4096 at most in all
+// Backward: waves per compute unit, and turns of a workgroup at the least, which leaves a row of partial sums each.  Us of
+// 16384 rows of 2048 bf16 with its sums: 16 waves 89, 12 85, 8 82; of 2055 rows of 1024 fp32: 22, 19, 17, with four turns 16.
+constexpr int kDropnormBwdWaves = 8, kDropnormBwdTurns = 4;
 
 int64_t dropnorm_bwd_workspace_elems(int64_t rows, int cols) {
   if (rows <= 0 || cols <= 0) return 0;
-  // (one row of partial sums per workgroup, for dgamma and dbeta: four waves to a workgroup at the least, or one row
-  // of more than 512 columns in two)
+  // (a row of partial sums per workgroup, for dgamma and dbeta: of two waves and one row, or of four, at the least)
   return 2 * std::min<int64_t>(rows, 256 * kDropnormBwdWaves / 2) * cols;
 }
 
@@ -350,12 +346,13 @@ int dropnorm_bwd(const TX* dy, const TR* dh, const TX* x, const TR* res, const T
   const int n_vec = (cols + 7) / 8;
   int parts = 0;
   auto launch = [&]() {
-#define PTX_DN_CASE(G, WPR, NC, SHORT)                                                                                               \
-  if (SHORT ? cols < 8 : n_vec <= Lay<G, WPR>::kSpan * (NC)) {                                                                                   \
-    parts = walkers<G, WPR>(rows, kDropnormBwdWaves);                                                                         \
-    dropnorm_bwd_kernel<TX, TR, G, WPR, NC, SHORT><<<dim3(parts), dim3(Lay<G, WPR>::kThreads), 0, stream>>>(                         \
-        dy, dh, x, res, h, mean, rstd, NormParam{gamma, param_type}, dx, dres, part, rows, cols, drop);                           \
-    return 0;                                                                                                                 \
+#define PTX_DN_CASE(G, WAVES, NC, SHORT)                                                               \
+  if (PTX_DN_FITS(G, WAVES, NC, SHORT)) {                                                              \
+    const Walk w = walk<G, WAVES, NC>(rows, n_vec, kDropnormBwdWaves, kDropnormBwdTurns);              \
+    parts = w.groups;                                                                                  \
+    dropnorm_bwd_kernel<TX, TR, G, WAVES, NC, SHORT><<<dim3(parts), dim3(w.threads), 0, stream>>>(     \
+        dy, dh, x, res, h, mean, rstd, NormParam{gamma, param_type}, dx, dres, part, rows, cols, drop); \
+    return 0;                                                                                          \
   }
     PTX_DN_LAYOUTS(PTX_DN_CASE)
 #undef PTX_DN_CASE

@@ -17,7 +17,7 @@ struct Dropout {
   uint32_t key[2];
   const int64_t* seed;   // read from device memory where given: the key then
   uint32_t hi, lo;       // the threshold round(p 2^32): hi 2^16 + lo; 0 = no dropout, 2^16 and 0 = nothing stays
-  float scale;           // 1 / (1 - p), 0 for p = 1
+  float scale;           // 1 / (1 - p), 1 for p = 0, 0 for p = 1
   // Rows are [outer][shared][inner]; the rows of one (outer, inner) have the same mask row, outer * inner + inner.
   uint32_t shared, inner;
 };
@@ -31,49 +31,56 @@ __device__ __forceinline__ Dropout with_key(Dropout d) {
   return d;
 }
 
+__device__ __forceinline__ uint32_t xor3(uint32_t a, uint32_t b, uint32_t c) { return __builtin_amdgcn_bitop3_b32(a, b, c, 0x96); }
+
 __device__ __forceinline__ void philox(uint32_t (&c)[4], uint32_t k0, uint32_t k1) {
 #pragma unroll
   for (int r = 0; r < 10; ++r) {
     const uint64_t a = (uint64_t)c[0] * 0xD2511F53u, b = (uint64_t)c[2] * 0xCD9E8D57u;
-    c[0] = (uint32_t)(b >> 32) ^ c[1] ^ k0;
+    c[0] = xor3((uint32_t)(b >> 32), c[1], k0);
     c[1] = (uint32_t)b;
-    c[2] = (uint32_t)(a >> 32) ^ c[3] ^ k1;
+    c[2] = xor3((uint32_t)(a >> 32), c[3], k1);
     c[3] = (uint32_t)a;
     k0 += 0x9E3779B9u;
     k1 += 0xBB67AE85u;
   }
 }
 
-// factor[e]: what element e of block k of the mask row is multiplied by, `scale` or 0.
-__device__ __forceinline__ void dropout_factors(const Dropout& d, uint32_t row, uint32_t k, float (&factor)[8]) {
+// Which elements of block k of the mask row stay: bit e / 2 + 16 (e % 2) for element e (as the words hold them; the other bits
+// are of no use).
+__device__ __forceinline__ uint32_t dropout_keeps(const Dropout& d, uint32_t row, uint32_t k) {
+  if (!(d.hi | d.lo)) return ~0u;
+  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
   uint32_t w[4] = {k, row, 0u, 0u};
   philox(w, d.key[0], d.key[1]);
   // (a number equal to hi is kept where lo is 0; where it is not, the second draw decides)
-  const uint32_t cut = d.hi + (d.lo != 0);
-  bool tie = false;
+  const unsigned short least = (unsigned short)(d.hi + (d.lo != 0) - 1);      // what is above it is kept
+  const u16x2 above = {least, least}, one = {1, 1}, same = {(unsigned short)d.hi, (unsigned short)d.hi};
+  uint32_t keeps = 0;
+  u16x2 off = {0xFFFF, 0xFFFF};
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const uint32_t u = e & 1 ? w[e >> 1] >> 16 : w[e >> 1] & 0xFFFFu;
-    factor[e] = u >= cut ? d.scale : 0.0f;
-    tie = tie || u == d.hi;
+  for (int i = 3; i >= 0; --i) {
+    const u16x2 u = __builtin_bit_cast(u16x2, w[i]);
+    keeps = keeps << 1 | __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_elementwise_sub_sat(u, above), one));
+    off = __builtin_elementwise_min(off, u ^ same);
   }
-  if (d.lo != 0 && tie) {
+  if (d.lo != 0 && (off[0] == 0 || off[1] == 0)) {
     uint32_t v[4] = {k, row, 0u, 1u};
     philox(v, d.key[0], d.key[1]);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const uint32_t u = e & 1 ? w[e >> 1] >> 16 : w[e >> 1] & 0xFFFFu;
       const uint32_t below = e & 1 ? v[e >> 1] >> 16 : v[e >> 1] & 0xFFFFu;
-      if (u == d.hi && below >= d.lo) factor[e] = d.scale;
+      if (u == d.hi && below >= d.lo) keeps |= 1u << (e / 2 + 16 * (e % 2));
     }
   }
+  asm volatile("" : "+v"(keeps));      // (formed here: where it is used, the compiler would wait for loads in between first)
+  return keeps;
 }
 
-// x * factor, with exactly 0 for a dropped element whatever it holds
-__device__ __forceinline__ float dropped(float x, float factor) { return factor != 0.0f ? x * factor : 0.0f; }
-// res + x * factor in one rounding
-__device__ __forceinline__ float dropped_add(float x, float factor, float res) {
-  return factor != 0.0f ? __builtin_fmaf(x, factor, res) : res;
+// x where element e stays, else exactly 0 whatever x holds; `scale` is left to the caller's multiplication
+__device__ __forceinline__ float kept(float x, uint32_t keeps, int e) {
+  return __uint_as_float(__float_as_uint(x) & (uint32_t)((int32_t)(keeps << (31 - (e / 2 + 16 * (e % 2)))) >> 31));
 }
 
 // Eight elements at an element's alignment (rows of odd lengths): gfx950 takes vector accesses at any address, so an
@@ -97,19 +104,21 @@ template <typename T> __device__ __forceinline__ Raw8<T> rounded(const f32x8& v)
 // Columns col .. col + n - 1 of a row (n <= 8).  The load of a row's last, shorter block is moved back to where it ends with the
 // row, so that a load is one instruction without a branch (behind a branch the next load would wait for this one), and what it
 // brings is moved to its place when it is used.  Rows of fewer than 8 columns (SHORT) are read one by one.
-template <bool SHORT, typename T> __device__ __forceinline__ Raw8<T> load_cols(const T* row, int col, int cols) {
+template <bool SHORT, bool NT = false, typename T> __device__ __forceinline__ Raw8<T> load_cols(const T* row, int col, int cols) {
   if constexpr (SHORT) {
     Raw8<T> v;
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = e < cols ? row[e] : (T)0.0f;
     return v;
   } else {
-    return *reinterpret_cast<const Raw8<T>*>(row + min(col, cols - 8));
+    const Raw8<T>* p = reinterpret_cast<const Raw8<T>*>(row + min(col, cols - 8));
+    return NT ? __builtin_nontemporal_load(p) : *p;
   }
 }
 template <bool SHORT, typename T> __device__ __forceinline__ f32x8 used_cols(const Raw8<T>& raw, int n) {
   f32x8 v = widened<T>(raw);
   if (!SHORT && n < 8) {
+    asm volatile("");      // (kept behind its branch: made into selects for every lane, this is a fifth of a kernel's arithmetic)
     const int s = 8 - n;
 #pragma unroll
     for (int step = 4; step >= 1; step >>= 1)
@@ -118,9 +127,11 @@ template <bool SHORT, typename T> __device__ __forceinline__ f32x8 used_cols(con
   }
   return v;
 }
-template <typename T> __device__ __forceinline__ void store_cols(T* p, const f32x8& v, int n) {
+template <bool NT = false, typename T> __device__ __forceinline__ void store_cols(T* p, const f32x8& v, int n) {
   if (n >= 8) {
-    *reinterpret_cast<Raw8<T>*>(p) = rounded<T>(v);
+    Raw8<T>* to = reinterpret_cast<Raw8<T>*>(p);
+    const Raw8<T> o = rounded<T>(v);
+    if (NT) __builtin_nontemporal_store(o, to); else *to = o;
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e)

@@ -288,7 +288,7 @@ __global__ __launch_bounds__(256) void relative_bias_bwd_kernel(Buckets bk, int 
     };
     if (!k.narrow) {
       for_queries(k, t, sub, [&](int, int i) {
-        const f32x8 v = values(load_cols<SHORT>(d + (int64_t)i * t.k_len, k.j, t.k_len));
+        const f32x8 v = values(load_cols<SHORT, true>(d + (int64_t)i * t.k_len, k.j, t.k_len));
         at_far_query(bk, mid, t, qa, ka, k, i, [&](const int(&u)[8]) { each(v, u); });
       });
       continue;
@@ -296,7 +296,7 @@ __global__ __launch_bounds__(256) void relative_bias_bwd_kernel(Buckets bk, int 
     // (a step: a block of queries, AHEAD or fewer of them in a lane; those that are not there: the last one once more, not used)
     auto load = [&](Raw8<T>(&raw)[AHEAD], int i, int n) {
 #pragma unroll
-      for (int r = 0; r < AHEAD; ++r) raw[r] = load_cols<SHORT>(d + (int64_t)(i + min(r, n - 1)) * t.k_len, k.j, t.k_len);
+      for (int r = 0; r < AHEAD; ++r) raw[r] = load_cols<SHORT, true>(d + (int64_t)(i + min(r, n - 1)) * t.k_len, k.j, t.k_len);
     };
     Raw8<T> raw[AHEAD], next[AHEAD];
     int l = sub * t.per_lane, i = l;

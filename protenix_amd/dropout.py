@@ -143,7 +143,7 @@ def dropout_add_layer_norm(x: torch.Tensor, residual: Optional[torch.Tensor] = N
                            seed: Seed = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """(LayerNorm(h), h) with h = residual + dropout(x), in one pass; differentiable in x, residual, weight and bias.
 
-    x, residual, p, shared_dim, training and seed as in `dropout_add`; the norm is over the last dimension (at most 32768), of
+    x, residual, p, shared_dim, training and seed as in `dropout_add`; the norm is over the last dimension (at most 16384), of
     the fp32 sum before it is rounded to h, and has x's type; h has the residual's.  weight, bias: [x.shape[-1]], of one of the
     three types, the same for both, either may be None; their gradients have their type and come out of a fixed order of
     additions.  p = 0 (the default): the residual sum and norm of a network in use."""

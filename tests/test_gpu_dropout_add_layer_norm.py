@@ -80,7 +80,7 @@ def test_row_lengths(types, cols):
     _compare(*args, 0.15, 21, None, 1e-5, y, h, grads)
 
 
-@pytest.mark.parametrize("cols", [8193, 16384, 20001, 32768])
+@pytest.mark.parametrize("cols", [8193, 12288, 16383, 16384])
 @pytest.mark.parametrize("types", [(F32, F32), (BF16, BF16), (F16, F32)])
 def test_very_long_rows(types, cols):
     args = _inputs((3, cols), *types, seed=cols)
@@ -226,7 +226,7 @@ def test_refusals():
     w = torch.ones(8, device="cuda")
     for args, kw, match in [((x, x, w[:4]), {}, "weight and bias"), ((x, x, w, w.to(BF16)), {}, "weight and bias"),
                             ((x, x, w.cpu()), {}, "weight and bias"), ((x, x, w.double()), {}, "float32"), ((x.to(BF16), x.to(F16)), {}, "type"),
-                            ((x[:, :0],), {}, "empty"), ((torch.zeros(2, 32769, device="cuda"),), {}, "unsupported shape"),
+                            ((x[:, :0],), {}, "empty"), ((torch.zeros(2, 16385, device="cuda"),), {}, "unsupported shape"),
                             ((x, x), {"p": 2.0}, "probability"), ((x, x), {"shared_dim": -1, "p": 0.1}, "last"), ((x, x[:1]), {}, "differ")]:
         with pytest.raises(RuntimeError, match=match):
             P.dropout_add_layer_norm(*args, **kw)

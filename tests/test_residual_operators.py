@@ -98,10 +98,10 @@ def test_c_entry_points_refuse_before_a_launch():
     fwd = lambda rows=4, cols=8, p=0.0, xt=0, st=0, wt=0: lib.ptx_dropout_add_layernorm_fwd(
         *([None] * 8), rows, cols, 1, 1, p, 1e-5, 1, None, xt, st, wt, None)
     assert fwd(rows=0) == 0 and fwd() == 1
-    assert fwd(cols=32769) == 2 and fwd(xt=0, st=1) == 2 and fwd(xt=1, st=3) == 2 and fwd(wt=2) == 1 and fwd(p=2.0) == 1
+    assert fwd(cols=16385) == 2 and fwd(xt=0, st=1) == 2 and fwd(xt=1, st=3) == 2 and fwd(wt=2) == 1 and fwd(p=2.0) == 1
     bwd = lambda rows=4, cols=8, dw=None, xt=0, st=0: lib.ptx_dropout_add_layernorm_bwd(
         *([None] * 10), dw, None, None, rows, cols, 1, 1, 0.0, 1, None, xt, st, 0, None)
-    assert bwd(rows=0) == 0 and bwd() == 1 and bwd(dw=8) == 1 and bwd(cols=40000) == 2 and bwd(xt=3, st=1) == 2
+    assert bwd(rows=0) == 0 and bwd() == 1 and bwd(dw=8) == 1 and bwd(cols=20000) == 2 and bwd(xt=3, st=1) == 2
     assert lib.ptx_dropout_add_layernorm_bwd_workspace_elems(0, 8) == 0
     assert lib.ptx_dropout_add_layernorm_bwd_workspace_elems(5, 8) >= 2 * 8
 
