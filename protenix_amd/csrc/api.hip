@@ -1124,7 +1124,8 @@ PTX_API int ptx_hbm_stream(const void* src, void* dst, int64_t bytes, int nontem
 static int dropout_of(ptx::Dropout& d, const char* what, int64_t rows, int cols, int64_t shared, int64_t inner, double p, uint64_t seed,
                       const int64_t* seed_ptr) {
   PTX_REQUIRE(rows >= 0 && cols > 0, PTX_ERR_BAD_ARG, "%s: rows=%lld cols=%d", what, (long long)rows, cols);
-  PTX_REQUIRE(rows < ((int64_t)1 << 31), PTX_ERR_UNSUPPORTED, "%s: rows=%lld too large", what, (long long)rows);
+  PTX_REQUIRE(rows < ((int64_t)1 << 31) && cols <= 0x7fffffff - 8, PTX_ERR_UNSUPPORTED, "%s: %lld rows of %d columns are too many", what,
+              (long long)rows, cols);
   PTX_REQUIRE(p >= 0.0 && p <= 1.0, PTX_ERR_BAD_ARG, "%s: p=%g outside 0..1", what, p);
   PTX_REQUIRE(shared > 0 && inner > 0 && shared < ((int64_t)1 << 31) && inner < ((int64_t)1 << 31) && rows % (shared * inner) == 0,
               PTX_ERR_BAD_ARG, "%s: %lld rows are not [outer][%lld][%lld]", what, (long long)rows, (long long)shared, (long long)inner);

@@ -35,12 +35,6 @@ template <bool SHORT> __device__ __forceinline__ f32x8 load_param(NormParam w, i
   return used_cols<SHORT, f16_t>(load_cols<SHORT>((const f16_t*)w.p, col, cols), n);
 }
 
-template <int G> __device__ __forceinline__ float lanes_sum(float v) {
-#pragma unroll
-  for (int m = G / 2; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
-  return v;
-}
-
 // Sums over the lanes of a row: within G lanes, or (WAVES > 1) over the waves of a workgroup through one of the slots (a slot is
 // used again two exchanges later, when every wave has passed the barrier of the exchange between).
 template <int WAVES> struct Slots {

@@ -83,6 +83,33 @@ __device__ __forceinline__ float kept(float x, uint32_t keeps, int e) {
   return __uint_as_float(__float_as_uint(x) & (uint32_t)((int32_t)(keeps << (31 - (e / 2 + 16 * (e % 2)))) >> 31));
 }
 
+// The sum over G neighbouring lanes, in all of them, on the vector pipe: moves within rows of 16 lanes, then exchanges of rows and
+// halves (a shuffle through LDS takes some hundred cycles a step, and a norm's row has up to eighteen of them).
+template <int CTRL> __device__ __forceinline__ float lane_move(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true));
+}
+template <int G> __device__ __forceinline__ float lanes_sum(float v) {
+  static_assert(G == 8 || G == 16 || G == 32 || G == 64, "8, 16, 32 or 64 lanes");
+  v += lane_move<0xB1>(v);      // lane ^ 1 (within four: 1 0 3 2)
+  v += lane_move<0x4E>(v);      // lane ^ 2 (2 3 0 1)
+  v += lane_move<0x141>(v);     // 7 - lane within 8: the other four
+  if constexpr (G >= 16) v += lane_move<0x140>(v);      // 15 - lane within 16: the other eight
+  // (the results by way of variables: a cast of a vector's element takes the first one)
+  if constexpr (G >= 32) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, v);
+    const auto w = __builtin_amdgcn_permlane16_swap(u, u, false, false);      // rows 0 0 2 2 and 1 1 3 3
+    const uint32_t a = w[0], b = w[1];
+    v = __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
+  }
+  if constexpr (G >= 64) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, v);
+    const auto w = __builtin_amdgcn_permlane32_swap(u, u, false, false);      // the halves
+    const uint32_t a = w[0], b = w[1];
+    v = __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
+  }
+  return v;
+}
+
 // Eight elements at an element's alignment (rows of odd lengths): gfx950 takes vector accesses at any address, so an
 // odd row costs the lines it straddles and nothing else.
 template <typename T> struct Unaligned8 { typedef T type __attribute__((ext_vector_type(8), aligned(sizeof(T)))); };

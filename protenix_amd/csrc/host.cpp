@@ -1149,7 +1149,11 @@ struct RowsOf {
 // recording and leave it there, which ends the process, so the forward call is refused.
 void refuse_foreign_accumulators(hipStream_t st, std::initializer_list<const Tensor*> leaves) {
   hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-  if (hipStreamIsCapturing(st, &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
+  if (hipStreamIsCapturing(st, &status) != hipSuccess) {
+    (void)hipGetLastError();      // (the default stream while another one records: not for a later launch to report)
+    return;
+  }
+  if (status == hipStreamCaptureStatusNone) return;
   for (const Tensor* t : leaves) {
     if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
     const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
@@ -1298,12 +1302,14 @@ struct BiasCall {
   ptx_relative_buckets buckets;
   int size[4];   // batch, heads, queries, keys
   int64_t q_first, k_first;
+  bool batched;  // the result has a batch axis
 };
 
 Tensor relative_bias_call(const Tensor& table, const Tensor& q, const Tensor& k, const Tensor& gq, const Tensor& gk, const BiasCall& c,
                           at::ScalarType type) {
   const Tensor t = table.contiguous();
-  Tensor out = at::empty({c.size[0], c.size[1], c.size[2], c.size[3]}, t.options().dtype(type));
+  const int64_t shape[4] = {c.size[0], c.size[1], c.size[2], c.size[3]};
+  Tensor out = at::empty(c10::IntArrayRef(shape + !c.batched, 3 + c.batched), t.options().dtype(type));
   check(ptx_relative_bias_fwd(&c.buckets, ptr(t), ptr(out), c.size[0], c.size[1], c.size[2], c.size[3], (const int64_t*)ptr(q),
                               (const int64_t*)ptr(k), c.q_first, c.k_first, (const int64_t*)ptr(gq), (const int64_t*)ptr(gk),
                               code_of(t.scalar_type()), code_of(type), current_stream(t)), "relative_bias");
@@ -1339,7 +1345,7 @@ struct RelativeBiasFn : torch::autograd::Function<RelativeBiasFn> {
 };
 
 // buckets: the address of a ptx_relative_buckets
-Tensor relative_bias(const Tensor& table, uintptr_t buckets, const std::array<int64_t, 4>& size, const optional<Tensor>& q, const optional<Tensor>& k,
+Tensor relative_bias(const Tensor& table, uintptr_t buckets, const std::array<int64_t, 4>& size, bool batched, const optional<Tensor>& q, const optional<Tensor>& k,
                      const optional<Tensor>& gq, const optional<Tensor>& gk, int64_t q_first, int64_t k_first, at::ScalarType type) {
   BiasCall c;
   c.buckets = *(const ptx_relative_buckets*)buckets;
@@ -1349,6 +1355,7 @@ Tensor relative_bias(const Tensor& table, uintptr_t buckets, const std::array<in
   }
   c.q_first = q_first;
   c.k_first = k_first;
+  c.batched = batched;
   py::gil_scoped_release nogil;
   at::DeviceGuard dev(table.device());
   if (at::GradMode::is_enabled() && table.requires_grad()) {

@@ -376,15 +376,14 @@ __global__ __launch_bounds__(256) void relative_bias_bwd_kernel(Buckets bk, int 
         const f32x4 b = ((const f32x4*)bins)[(v * n_buckets + u) * 16 + (w & 15)];
         s += (b[0] + b[1]) + (b[2] + b[3]);
       }
-#pragma unroll
-    for (int m = 1; m < 16; m <<= 1) s += __shfl_xor(s, m, 64);
+    s = lanes_sum<16>(s);
     if (u < n_buckets && (w & 15) == 0) part[((int64_t)blockIdx.x * n_buckets + u) * heads + h] = s;
   }
 }
 
 // most: vectors a unit may have (64 .. 256); threads: of a workgroup at most, at least `most`; groups: workgroups that share
-// the units of one head (or head group); ahead: queries of a step in a lane.
-static Tiling tiling(int batch, int q_len, int k_len, int most, int threads, int64_t groups, int ahead) {
+// the units of one of `planes` heads (or head groups); ahead: queries of a step in a lane.
+static Tiling tiling(int batch, int q_len, int k_len, int most, int threads, int64_t groups, int planes, int ahead) {
   Tiling t;
   t.q_len = q_len;
   t.k_len = k_len;
@@ -396,9 +395,11 @@ static Tiling tiling(int batch, int q_len, int k_len, int most, int threads, int
   for (int n = 64; n <= threads; n += 64)
     if (n >= t.chunk && (int64_t)(n / t.chunk) * t.threads > (int64_t)(t.threads / t.chunk) * n) t.threads = n;
   t.at_once = t.threads / t.chunk;
-  // a unit for every workgroup where there are rows for it; the blocks of queries no longer than leaves every unit one
-  const int64_t columns = (int64_t)batch * t.chunks;
-  t.row_units = (int)std::min<int64_t>((q_len + t.at_once - 1) / t.at_once, std::max<int64_t>(1, groups / columns));
+  // a unit for every workgroup where there are rows for it: whole steps of them, as long as every compute unit has some; the blocks
+  // of queries no longer than leaves every unit one
+  const int64_t columns = (int64_t)batch * t.chunks, whole = (q_len + t.at_once * ahead - 1) / (t.at_once * ahead);
+  t.row_units = (int)std::min<int64_t>({(q_len + t.at_once - 1) / t.at_once, std::max<int64_t>(1, groups / columns),
+                                        std::max<int64_t>(whole, std::max<int64_t>(1, 256 / (columns * planes)))});
   const int share = (q_len + t.row_units - 1) / t.row_units;
   t.per_lane = std::max(1, std::min({ahead, kUnitRows / t.at_once, (share + t.at_once - 1) / t.at_once}));
   t.block = t.per_lane * t.at_once;
@@ -419,7 +420,7 @@ int relative_bias_fwd(const Buckets& bk, const void* table, int table_type, T* o
   const int n_buckets = bk.count + (q_group != nullptr);
   int at_once = std::min(heads, std::max(1, 16384 / (n_buckets * (int)sizeof(T)))), head_groups = (heads + at_once - 1) / at_once;
   const bool few = (int64_t)batch * q_len * ((k_len + 7) / 8) < kFewVectors;
-  Tiling t = tiling(batch, q_len, k_len, few ? 64 : 256, 256, std::max(1, 2048 / head_groups), 4);
+  Tiling t = tiling(batch, q_len, k_len, few ? 64 : 256, 256, std::max(1, 2048 / head_groups), 8 * head_groups, 1);
   // (fewer rows than a workgroup holds side by side: heads take their place)
   t.by_head = q_len < t.at_once && heads > 1;
   while (at_once > (t.by_head ? t.at_once : 1) && (int64_t)t.units * head_groups < 512) {
@@ -454,7 +455,7 @@ int relative_bias_bwd(const Buckets& bk, const T* dout, void* dtable, int table_
   int slices = 0;
   if (batch > 0 && q_len > 0 && k_len > 0) {
     const int most = bwd_threads(n_buckets);
-    const Tiling t = tiling(batch, q_len, k_len, most, most, bwd_slices(heads, n_buckets), kAhead<T>);
+    const Tiling t = tiling(batch, q_len, k_len, most, most, bwd_slices(heads, n_buckets), heads, kAhead<T>);
     slices = std::min(t.units, bwd_slices(heads, n_buckets));
     const int lds = kStartsBytes + lut_bytes(bk) + t.threads * 4 * n_buckets;
     const Axis qa{q_pos, q_group, q_first}, ka{k_pos, k_group, k_first};

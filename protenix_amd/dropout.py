@@ -9,6 +9,7 @@ launch, and for a captured call's replays as for the call itself.
 from __future__ import annotations
 
 import math
+import operator
 from typing import Optional, Tuple, Union
 
 import torch
@@ -26,6 +27,8 @@ def _rows(x: torch.Tensor, shared_dim: Optional[int]) -> tuple:
         raise RuntimeError("x needs at least one dimension")
     cols = shape[-1]
     rows = math.prod(shape[:-1])
+    if cols >= (1 << 31) - 8:
+        raise RuntimeError(f"rows of {cols} columns: below 2^31 (unsupported shape)")
     if shared_dim is None:
         return rows, cols, 1, 1
     d = shared_dim + len(shape) if shared_dim < 0 else shared_dim
@@ -46,7 +49,7 @@ def _seed(seed: Seed, p: float, x: torch.Tensor) -> tuple:
         if seed.dtype != torch.int64 or seed.numel() != 1 or seed.device != x.device:
             raise RuntimeError(f"a seed tensor holds one int64 on {x.device}, got {seed.dtype} {tuple(seed.shape)} on {seed.device}")
         return 0, seed
-    seed = int(seed)
+    seed = operator.index(seed)
     if not -(1 << 63) <= seed < 1 << 64:
         raise RuntimeError(f"seed={seed} does not fit 64 bits")
     return seed & 0xFFFFFFFFFFFFFFFF, None

@@ -779,12 +779,13 @@ def dropout_add_layer_norm_backward(dy, dh, x, residual, h, stats, weight, param
     return (dres if one else dx), dres, dw, db
 
 
-def relative_bias(buckets, table: torch.Tensor, size: tuple, q: tuple, k: tuple, groups: tuple, dtype: torch.dtype) -> torch.Tensor:
-    """[B, H, Q, K] for size = (B, H, Q, K); q, k = (positions [B, n] or None, first); groups = ([B, Q], [B, K]) or (None, None)."""
+def relative_bias(buckets, table: torch.Tensor, size: tuple, q: tuple, k: tuple, groups: tuple, dtype: torch.dtype,
+                  batched: bool = True) -> torch.Tensor:
+    """[B, H, Q, K] for size = (B, H, Q, K), or without the batch axis; q, k = (positions [B, n] or None, first); groups = ([B, Q], [B, K]) or (None, None)."""
     import ctypes
 
     lib = _lib.load()
-    out = torch.empty(size, dtype=dtype, device=table.device)
+    out = torch.empty(size if batched else size[1:], dtype=dtype, device=table.device)
     with torch.cuda.device(table.device):
         _call("relative_bias", lib.ptx_relative_bias_fwd, ctypes.addressof(buckets), _ptr(table), _ptr(out), *size, _ptr(q[0]),
               _ptr(k[0]), q[1], k[1], _ptr(groups[0]), _ptr(groups[1]), _dt_ln(table), _dt_ln(out), _stream())

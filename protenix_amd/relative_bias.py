@@ -112,11 +112,11 @@ def _whole(t: torch.Tensor, name: str, device: torch.device) -> torch.Tensor:
 
 class _RelativeBias(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, table, buckets, size, q, k, gq, gk, q_first, k_first, dtype):
+    def forward(ctx, table, buckets, size, batched, q, k, gq, gk, q_first, k_first, dtype):
         ctx.buckets, ctx.size, ctx.first = buckets, size, (q_first, k_first)
         ctx.table_shape, ctx.table_dtype = tuple(table.shape), table.dtype
         ctx.save_for_backward(q, k, gq, gk)
-        return ops.relative_bias(buckets._struct, table.contiguous(), size, (q, q_first), (k, k_first), (gq, gk), dtype)
+        return ops.relative_bias(buckets._struct, table.contiguous(), size, (q, q_first), (k, k_first), (gq, gk), dtype, batched)
 
     @staticmethod
     @once_differentiable
@@ -124,7 +124,7 @@ class _RelativeBias(torch.autograd.Function):
         q, k, gq, gk = ctx.saved_tensors
         dtable = ops.relative_bias_backward(ctx.buckets._struct, grad, ctx.table_shape, ctx.table_dtype, ctx.size, (q, ctx.first[0]),
                                             (k, ctx.first[1]), (gq, gk))
-        return (dtable,) + (None,) * 9
+        return (dtable,) + (None,) * 10
 
 
 def relative_position_bias(table: torch.Tensor, buckets: RelativeBuckets, query_positions: Positions, key_positions: Positions, *,
@@ -159,14 +159,15 @@ def relative_position_bias(table: torch.Tensor, buckets: RelativeBuckets, query_
         raise RuntimeError(f"positions and groups of different batch sizes {sorted(batches)}")
     batch = batches.pop() if batches else None
     size = (1 if batch is None else batch, table.shape[1], n_q, n_k)
+    if max(n_q, n_k) > 1 << 30:
+        raise RuntimeError(f"{n_q} queries and {n_k} keys: 2^30 at most (unsupported shape)")
     q, k, gq, gk = (None if t is None else t.expand(size[0], t.shape[-1]).contiguous() for t in (q, k, gq, gk))
     if ops.use_native_operators():
-        out = native.host().relative_bias(table, ctypes.addressof(buckets._struct), size, q, k, gq, gk, q_first, k_first, dtype)
-    elif _wants_grad(table):
-        out = _RelativeBias.apply(table, buckets, size, q, k, gq, gk, q_first, k_first, dtype)
-    else:
-        out = ops.relative_bias(buckets._struct, table.contiguous(), size, (q, q_first), (k, k_first), (gq, gk), dtype)
-    return out[0] if batch is None else out
+        return native.host().relative_bias(table, ctypes.addressof(buckets._struct), size, batch is not None, q, k, gq, gk, q_first,
+                                           k_first, dtype)
+    if _wants_grad(table):
+        return _RelativeBias.apply(table, buckets, size, batch is not None, q, k, gq, gk, q_first, k_first, dtype)
+    return ops.relative_bias(buckets._struct, table.contiguous(), size, (q, q_first), (k, k_first), (gq, gk), dtype, batch is not None)
 
 
 class RelativePositionBias(nn.Module):
