@@ -1,4 +1,5 @@
-// The dropout mask of the residual updates, and 8-column vectors at any alignment: shared by dropout.hip and dropnorm.hip.
+// The dropout mask of the residual updates (dropout.hip, dropnorm.hip), 8-column vectors at any alignment and sums over lanes (those
+// and relbias.hip).
 //
 // The mask is never stored: forward and backward kernels draw it from Philox4x32-10, the counter-based generator of
 // Salmon, Moraes, Dror and Shaw (Parallel random numbers: as easy as 1, 2, 3, 2011).  A mask row's columns lie in

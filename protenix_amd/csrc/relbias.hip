@@ -11,7 +11,12 @@
 //
 // Gradient: sums of millions of elements in a few buckets.  Every lane has bins of its own in LDS, [bucket][lane], and adds to
 // them in its program's order, without waiting for the sums: no two lanes ever meet in a bin (nor, a bin's bank being its lane's, in a
-// bank), so nothing depends on scheduling.  Lanes, waves and workgroups are added in a fixed order at the end.
+// bank), so nothing depends on scheduling.  Lanes, waves and workgroups are added in a fixed order at the end.  An addition takes
+// about two cycles a lane, so a step of 8 queries by 8 keys makes few: one where all its differences share a bucket, one per difference
+// (and not even that where neighbours share one) along the diagonal, one per element only where positions jump.
+//
+// Us of [2, 16, 2048, 2048] bf16, 32 buckets to a distance of 128: forward 53 (5.0 TB/s); gradient with its sums 204 with an addition per
+// element, 103 with one per step or query, 55 (4.9 TB/s) with those along the diagonal.
 #include <algorithm>
 
 #include "../../include/protenix_amd.h"
@@ -242,7 +247,8 @@ __device__ __forceinline__ void bin_add(float* bin, float v) {
   __hip_atomic_fetch_add((__attribute__((address_space(3))) float*)bin, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
 }
 
-// Queries of a step side by side in a lane, requested a step ahead: 128 bytes.
+// Queries of a step in a lane, requested a step ahead: 128 bytes.  Read past the caches (NT): behind the forward pass, whose bias lies
+// there still to be written to memory, reads that take its place wait for that (94 against 55 us at the size above).
 template <typename T> constexpr int kAhead = sizeof(T) == 2 ? 8 : 4;
 
 // bins: [waves][n_buckets][64].  SHORT: fewer than 8 keys.
@@ -410,7 +416,8 @@ static Tiling tiling(int batch, int q_len, int k_len, int most, int threads, int
   return t;
 }
 
-// Fewer vectors than this (a query of a long context): units of 64, and the heads apart until every compute unit has two workgroups.
+// Fewer vectors than this (a query of a long context): units of 64, and the heads apart until every compute unit has two workgroups
+// (16 heads, one query, 4001 keys: 7.9 us with units of up to 256, 5.5 now).
 constexpr int64_t kFewVectors = 16384;
 
 template <typename T>

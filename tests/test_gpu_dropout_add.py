@@ -190,6 +190,10 @@ def test_refusals():
                             ((x, x), {"seed": torch.zeros(1, dtype=torch.int64)}, "seed tensor")]:
         with pytest.raises(RuntimeError, match=match):
             P.dropout_add(*args, **kw)
+    with pytest.raises(RuntimeError, match="unsupported"):
+        P.dropout_add(x[0, 0, :1].expand(1 << 31))
+    with pytest.raises(TypeError):
+        P.dropout_add(x, x, seed=1.5)
 
 
 def _graphed(fn):

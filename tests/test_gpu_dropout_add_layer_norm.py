@@ -132,6 +132,20 @@ def test_one_of_the_two_results_unused(types, which):
     _compare(*args, 0.2, 3, None, 1e-5, *_run(*args, 0.2, 3))
 
 
+@pytest.mark.parametrize("types", [(BF16, BF16), (F16, F32)])
+def test_frozen_inputs(types):
+    """Any subset of the four may want no gradient."""
+    args = _inputs((19, 200), *types)
+    full = _run(*args, 0.2, 3)[2]
+    for mask in range(1, 15):
+        some = [t.detach().requires_grad_(bool(mask >> i & 1)) for i, t in enumerate(args[:4])]
+        y, h = P.dropout_add_layer_norm(*some, 0.2, seed=3)
+        wanted = [n for i, n in enumerate("xrwb") if mask >> i & 1]
+        outs = [(o, g) for o, g in ((y, args[4]), (h, args[5])) if o.requires_grad]
+        grads = torch.autograd.grad([o for o, _ in outs], [t for t in some if t.requires_grad], [g for _, g in outs])
+        assert all(torch.equal(g, full[n]) for n, g in zip(wanted, grads)), wanted
+
+
 def test_rows_far_from_zero_and_of_one_value():
     """A mean a thousand times the deviation; rows of one value, whose variance is 0."""
     x, r, w, b, dy, dh = _inputs((20, 256), F32, F32, shift=2000.0)

@@ -114,6 +114,18 @@ def test_positions_without_order_repeated_and_at_the_ends_of_64_bits():
     _run((100, 254, True), 2, torch.tensor([3, -100], device="cuda", dtype=torch.int32), p)
 
 
+def test_groups_of_any_numbers():
+    """Group numbers that differ by 2^32 and more, or by everything 64 bits hold."""
+    pos, grp = _chains(2, 97, 6)
+    for numbers in ([5, 5 + (1 << 32), -5], [(1 << 63) - 1, -(1 << 63), 0], [0, 1 << 30, -(1 << 30)]):
+        g = torch.tensor(numbers, device="cuda")[grp]
+        _run((8, None, True), 3, pos, pos, (g, g), dtype=BF16)
+    # positions and groups that jump from query to query and from key to key
+    perm = torch.randperm(97, generator=torch.Generator().manual_seed(1)).cuda()
+    _run((128, 32, True), 3, pos[:, perm], pos, (grp[:, perm], grp))
+    _run((128, 32, True), 3, pos, pos[:, perm], (grp, grp[:, perm]))
+
+
 def test_batched_positions_beside_single_ones():
     pos, grp = _chains(3, 40, 1)
     _run((32, None, True), 4, pos, range(25))
@@ -204,7 +216,7 @@ def test_refusals():
                             ((t, b, i, i[:1].expand(3, 5)), {}, "batch sizes"), ((t, b, range(3), range(3)), {"dtype": torch.float64}, "float32"),
                             ((t, b, range(1 << 62, (1 << 62) + 3), range(3)), {}, "positions from"),
                             ((torch.zeros(33, 4, device="cuda"), b, range(3), range(3)), {"groups": (i[0], i[0])}, "groups of"),
-                            ((t, b, range(1 << 31), range(3)), {}, "2\\^31|too large|OverflowError|unsupported")]:
+                            ((t, b, range((1 << 32) + 3), range(1)), {}, "unsupported"), ((t, b, range(1), range((1 << 30) + 1)), {}, "unsupported")]:
         with pytest.raises(RuntimeError, match=match):
             P.relative_position_bias(*args, **kw)
     m = P.RelativePositionBias(4, b, grouped=True).cuda()
