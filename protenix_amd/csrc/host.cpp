@@ -13,7 +13,6 @@
 
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 
-#include <array>
 #include <cstring>
 #include <mutex>
 #include <set>
@@ -1139,7 +1138,8 @@ Tensor tri_attention(const Tensor& q, const Tensor& k, const Tensor& v, const op
 }
 
 // ---- residual dropout, its sum with LayerNorm, the relative position bias ---------------------------------
-// Arguments as dropout.py and relative_bias.py have checked them.
+// Calls with arguments as dropout.py and relative_bias.py document them are taken whole; anything else is handed back (None) to those,
+// which have the checks with their messages.
 struct RowsOf {
   int64_t rows, cols, shared, inner;
 };
@@ -1170,6 +1170,42 @@ void refuse_double_backward() {
 Tensor given(const optional<Tensor>& t) { return t ? *t : Tensor(); }
 Tensor dense(const optional<Tensor>& t) { return t && t->defined() ? t->contiguous() : Tensor(); }
 bool wants(const Tensor& t) { return t.defined() && t.requires_grad(); }
+
+bool float_type(const Tensor& t) {
+  return t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf;
+}
+// A seed as the C ABI takes it; false: not one.
+bool take_seed(const py::object& seed, const Tensor& x, uint64_t& number, optional<Tensor>& tensor) {
+  if (PyLong_CheckExact(seed.ptr())) {
+    int overflow = 0;
+    number = (uint64_t)PyLong_AsLongLongAndOverflow(seed.ptr(), &overflow);
+    return overflow == 0;
+  }
+  if (!THPVariable_Check(seed.ptr())) return false;
+  tensor = THPVariable_Unpack(seed.ptr());
+  return tensor->scalar_type() == at::kLong && tensor->numel() == 1 && tensor->device() == x.device();
+}
+// x, residual, p, shared_dim and the seed; false: not for here.
+bool take_update(const Tensor& x, const optional<Tensor>& residual, double& p, const optional<int64_t>& shared_dim, bool training,
+                 const py::object& seed, RowsOf& r, uint64_t& number, optional<Tensor>& tensor) {
+  if (!x.is_cuda() || !float_type(x) || x.dim() < 1 || x.numel() == 0 || !(p >= 0.0 && p <= 1.0)) return false;
+  if (residual && (residual->device() != x.device() || residual->sizes() != x.sizes() ||
+                   (residual->scalar_type() != x.scalar_type() && residual->scalar_type() != at::kFloat)))
+    return false;
+  r.cols = x.size(-1);
+  r.rows = x.numel() / r.cols;
+  r.shared = r.inner = 1;
+  if (r.cols >= ((int64_t)1 << 31) - 8) return false;
+  if (shared_dim) {
+    const int64_t d = *shared_dim < 0 ? *shared_dim + x.dim() : *shared_dim;
+    if (d < 0 || d >= x.dim() - 1) return false;
+    r.shared = x.size(d);
+    for (int64_t i = d + 1; i < x.dim() - 1; ++i) r.inner *= x.size(i);
+  }
+  if (!training) p = 0.0;
+  number = 0;
+  return p == 0.0 || take_seed(seed, x, number, tensor);
+}
 
 Tensor dropout_add_call(const Tensor& x, const Tensor& res, at::ScalarType out_type, const RowsOf& r, double p, uint64_t number, const Tensor& seed) {
   const Tensor xc = x.contiguous();
@@ -1203,11 +1239,14 @@ struct DropoutAddFn : torch::autograd::Function<DropoutAddFn> {
   }
 };
 
-Tensor dropout_add(const Tensor& x, const optional<Tensor>& residual, int64_t rows, int64_t cols, int64_t shared, int64_t inner, double p,
-                   uint64_t number, const optional<Tensor>& seed) {
+optional<Tensor> dropout_add(const Tensor& x, const optional<Tensor>& residual, double p, const optional<int64_t>& shared_dim, bool training,
+                             const py::object& seed_) {
+  RowsOf r;
+  uint64_t number;
+  optional<Tensor> seed;
+  if (!take_update(x, residual, p, shared_dim, training, seed_, r, number, seed)) return c10::nullopt;
   py::gil_scoped_release nogil;
   at::DeviceGuard dev(x.device());
-  const RowsOf r{rows, cols, shared, inner};
   const Tensor res = given(residual);
   if (at::GradMode::is_enabled() && (wants(x) || wants(res))) {
     refuse_foreign_accumulators(current_stream(x), {&x, &res});
@@ -1282,20 +1321,26 @@ struct DropoutAddLayerNormFn : torch::autograd::Function<DropoutAddLayerNormFn> 
   }
 };
 
-std::tuple<Tensor, Tensor> dropout_add_layer_norm(const Tensor& x, const optional<Tensor>& residual, const optional<Tensor>& weight,
-                                                  const optional<Tensor>& bias, int64_t rows, int64_t cols, int64_t shared, int64_t inner, double p,
-                                                  double eps, uint64_t number, const optional<Tensor>& seed) {
+optional<std::tuple<Tensor, Tensor>> dropout_add_layer_norm(const Tensor& x, const optional<Tensor>& residual, const optional<Tensor>& weight,
+                                                            const optional<Tensor>& bias, double p, double eps,
+                                                            const optional<int64_t>& shared_dim, bool training, const py::object& seed_) {
+  RowsOf r;
+  uint64_t number;
+  optional<Tensor> seed;
+  if (!take_update(x, residual, p, shared_dim, training, seed_, r, number, seed)) return c10::nullopt;
+  for (const auto& t : {&weight, &bias})
+    if (*t && (!float_type(**t) || (*t)->dim() != 1 || (*t)->size(0) != r.cols || (*t)->device() != x.device())) return c10::nullopt;
+  if (weight && bias && weight->scalar_type() != bias->scalar_type()) return c10::nullopt;
   py::gil_scoped_release nogil;
   at::DeviceGuard dev(x.device());
-  const RowsOf r{rows, cols, shared, inner};
   const Tensor res = given(residual), w = given(weight), b = given(bias);
   if (at::GradMode::is_enabled() && (wants(x) || wants(res) || wants(w) || wants(b))) {
     refuse_foreign_accumulators(current_stream(x), {&x, &res, &w, &b});
     const auto out = DropoutAddLayerNormFn::apply(x, residual, weight, bias, seed, r, p, eps, number);
-    return {out[0], out[1]};
+    return std::make_tuple(out[0], out[1]);
   }
   const auto [y, h, stats] = dropnorm_call(x.contiguous(), dense(residual), dense(weight), dense(bias), r, p, eps, number, given(seed), false);
-  return {y, h};
+  return std::make_tuple(y, h);
 }
 
 struct BiasCall {
@@ -1344,25 +1389,72 @@ struct RelativeBiasFn : torch::autograd::Function<RelativeBiasFn> {
   }
 };
 
+// Positions or groups of one side: a range (its first and its length) or whole numbers [n] or [batch, n]; false: not for here.
+struct Side {
+  optional<Tensor> t;
+  int64_t first = 0, n = 0;
+};
+bool take_whole(const py::handle& h, const Tensor& table, Side& s, int64_t& batch) {
+  if (!THPVariable_Check(h.ptr())) return false;
+  s.t = THPVariable_Unpack(h.ptr());
+  if (s.t->scalar_type() != at::kLong || s.t->device() != table.device() || s.t->dim() < 1 || s.t->dim() > 2) return false;
+  s.n = s.t->size(-1);
+  if (s.t->dim() == 2) {
+    if (batch >= 0 && batch != s.t->size(0)) return false;
+    batch = s.t->size(0);
+  }
+  return true;
+}
+bool take_side(const py::handle& h, const Tensor& table, Side& s, int64_t& batch) {
+  if (!PyRange_Check(h.ptr())) return take_whole(h, table, s, batch);
+  int over = 0;
+  const int64_t step = PyLong_AsLongLongAndOverflow(py::object(h.attr("step")).ptr(), &over);
+  if (over || step != 1) return false;
+  s.first = PyLong_AsLongLongAndOverflow(py::object(h.attr("start")).ptr(), &over);
+  if (over || s.first < -((int64_t)1 << 62) || s.first >= (int64_t)1 << 62) return false;
+  const int64_t stop = PyLong_AsLongLongAndOverflow(py::object(h.attr("stop")).ptr(), &over);
+  if (over) return false;
+  s.n = stop > s.first ? stop - s.first : 0;
+  return true;
+}
+
 // buckets: the address of a ptx_relative_buckets
-Tensor relative_bias(const Tensor& table, uintptr_t buckets, const std::array<int64_t, 4>& size, bool batched, const optional<Tensor>& q, const optional<Tensor>& k,
-                     const optional<Tensor>& gq, const optional<Tensor>& gk, int64_t q_first, int64_t k_first, at::ScalarType type) {
+optional<Tensor> relative_bias(const Tensor& table, uintptr_t buckets, const py::object& query_positions, const py::object& key_positions,
+                               const py::object& groups, const optional<at::ScalarType>& dtype) {
   BiasCall c;
   c.buckets = *(const ptx_relative_buckets*)buckets;
-  for (int i = 0; i < 4; ++i) {
-    if (size[i] > 0x7fffffff) throw std::runtime_error("relative_bias: unsupported shape (2): a side of 2^31 or more");
-    c.size[i] = (int)size[i];
+  const at::ScalarType type = dtype ? *dtype : table.scalar_type();
+  const bool grouped = !groups.is_none();
+  if (!table.is_cuda() || !float_type(table) || table.dim() != 2 || table.size(0) != c.buckets.count + grouped || table.size(1) == 0 ||
+      table.size(1) > 32768 || !(type == at::kFloat || type == at::kBFloat16 || type == at::kHalf))
+    return c10::nullopt;
+  Side q, k, gq, gk;
+  int64_t batch = -1;
+  if (!take_side(query_positions, table, q, batch) || !take_side(key_positions, table, k, batch)) return c10::nullopt;
+  if (grouped) {
+    if (!PyTuple_CheckExact(groups.ptr()) || PyTuple_GET_SIZE(groups.ptr()) != 2 ||
+        !take_whole(PyTuple_GET_ITEM(groups.ptr(), 0), table, gq, batch) || !take_whole(PyTuple_GET_ITEM(groups.ptr(), 1), table, gk, batch) ||
+        gq.n != q.n || gk.n != k.n)
+      return c10::nullopt;
   }
-  c.q_first = q_first;
-  c.k_first = k_first;
-  c.batched = batched;
+  c.batched = batch >= 0;
+  if (!c.batched) batch = 1;
+  if (q.n > (int64_t)1 << 30 || k.n > (int64_t)1 << 30 || batch > 0x7fffffff) return c10::nullopt;
+  c.size[0] = (int)batch;
+  c.size[1] = (int)table.size(1);
+  c.size[2] = (int)q.n;
+  c.size[3] = (int)k.n;
+  c.q_first = q.first;
+  c.k_first = k.first;
   py::gil_scoped_release nogil;
   at::DeviceGuard dev(table.device());
+  for (Side* s : {&q, &k, &gq, &gk})
+    if (s->t) s->t = (s->t->dim() == 1 && c.batched ? s->t->expand({batch, s->n}) : *s->t).contiguous();
   if (at::GradMode::is_enabled() && table.requires_grad()) {
     refuse_foreign_accumulators(current_stream(table), {&table});
-    return RelativeBiasFn::apply(table, q, k, gq, gk, c, type);
+    return RelativeBiasFn::apply(table, q.t, k.t, gq.t, gk.t, c, type);
   }
-  return relative_bias_call(table, given(q), given(k), given(gq), given(gk), c, type);
+  return relative_bias_call(table, given(q.t), given(k.t), given(gq.t), given(gk.t), c, type);
 }
 
 }  // namespace
@@ -1395,6 +1487,7 @@ PYBIND11_MODULE(_host, m) {
   py::class_<Mark, std::shared_ptr<Mark>>(m, "Mark").def("elapsed_time", &Mark::elapsed_time);
   m.def("layer_norm", &layer_norm);
   m.def("tri_attention", &tri_attention);
+  // (None: arguments for the Python path)
   m.def("dropout_add", &dropout_add);
   m.def("dropout_add_layer_norm", &dropout_add_layer_norm);
   m.def("relative_bias", &relative_bias);

@@ -37,14 +37,16 @@ def _rows(x: torch.Tensor, shared_dim: Optional[int]) -> tuple:
     return rows, cols, max(shape[d], 1), max(math.prod(shape[d + 1:-1]), 1)
 
 
+def _drawn() -> int:
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("a call recorded into a graph needs its seed: every replay would repeat the mask of a seed drawn now "
+                           "(give a one-element int64 GPU tensor and change it between replays, or a whole number)")
+    return int(torch.empty((), dtype=torch.int64).random_())      # torch's default generator: torch.manual_seed decides
+
+
 def _seed(seed: Seed, p: float, x: torch.Tensor) -> tuple:
     if p == 0.0:
         return 0, None
-    if seed is None:
-        if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("a call recorded into a graph needs its seed: every replay would repeat the mask of a seed drawn now "
-                               "(give a one-element int64 GPU tensor and change it between replays, or a whole number)")
-        return int(torch.empty((), dtype=torch.int64).random_()), None      # torch's default generator: torch.manual_seed decides
     if isinstance(seed, torch.Tensor):
         if seed.dtype != torch.int64 or seed.numel() != 1 or seed.device != x.device:
             raise RuntimeError(f"a seed tensor holds one int64 on {x.device}, got {seed.dtype} {tuple(seed.shape)} on {seed.device}")
@@ -102,13 +104,17 @@ def dropout_add(x: torch.Tensor, residual: Optional[torch.Tensor] = None, p: flo
     seed: a whole number of 64 bits, or one int64 in a GPU tensor, read when the kernels run (a graph's replays then have the masks of
     what the tensor holds at the time; it must not change between a call and its backward pass).  None: drawn from torch's default
     generator.  Two calls with the same seed and shape have the same mask."""
+    if seed is None and training and p != 0.0 and x.is_cuda:
+        seed = _drawn()
+    if ops.use_native_operators():
+        out = native.host().dropout_add(x, residual, p, shared_dim, training, seed)
+        if out is not None:
+            return out
     p = _check(x, residual, p, training)
     rows = _rows(x, shared_dim)
     number, tensor = _seed(seed, p, x)
     if x.numel() == 0:
         return x + x if residual is None else residual + x      # (nothing to launch; shapes and gradients as torch has them)
-    if ops.use_native_operators():
-        return native.host().dropout_add(x, residual, *rows, p, number, tensor)
     if _wants_grad(x, residual):
         return _DropoutAdd.apply(x, residual, rows, p, number, tensor)
     return ops.dropout_add(x, residual, x.dtype if residual is None else residual.dtype, rows, p, (number, tensor))
@@ -150,6 +156,12 @@ def dropout_add_layer_norm(x: torch.Tensor, residual: Optional[torch.Tensor] = N
     the fp32 sum before it is rounded to h, and has x's type; h has the residual's.  weight, bias: [x.shape[-1]], of one of the
     three types, the same for both, either may be None; their gradients have their type and come out of a fixed order of
     additions.  p = 0 (the default): the residual sum and norm of a network in use."""
+    if seed is None and training and p != 0.0 and x.is_cuda:
+        seed = _drawn()
+    if ops.use_native_operators():
+        out = native.host().dropout_add_layer_norm(x, residual, weight, bias, p, eps, shared_dim, training, seed)
+        if out is not None:
+            return out
     p = _check(x, residual, p, training)
     rows = _rows(x, shared_dim)
     cols = rows[1]
@@ -162,8 +174,6 @@ def dropout_add_layer_norm(x: torch.Tensor, residual: Optional[torch.Tensor] = N
             raise RuntimeError(f"weight and bias are [{cols}] on {x.device} and of one type, got "
                                + ", ".join(f"{tuple(u.shape)} {u.dtype} on {u.device}" for u in params))
     number, tensor = _seed(seed, p, x)
-    if ops.use_native_operators():
-        return native.host().dropout_add_layer_norm(x, residual, weight, bias, *rows, p, float(eps), number, tensor)
     if _wants_grad(x, residual, weight, bias):
         return _DropoutAddLayerNorm.apply(x, residual, weight, bias, rows, p, float(eps), number, tensor)
     x, residual, weight, bias = (None if t is None else t.contiguous() for t in (x, residual, weight, bias))

@@ -137,6 +137,10 @@ def relative_position_bias(table: torch.Tensor, buckets: RelativeBuckets, query_
     behind n others), or whole numbers [n] or [B, n]; they may repeat and need no order.
     groups: (of the queries, of the keys), whole numbers of the positions' shapes: tokens of one chain have one number, since residue
     numbers of two chains say nothing about each other.  dtype: of the result (the table's by default)."""
+    if ops.use_native_operators():
+        out = native.host().relative_bias(table, ctypes.addressof(buckets._struct), query_positions, key_positions, groups, dtype)
+        if out is not None:
+            return out
     ops._dev(table, "table")
     ops._dt_ln(table)
     dtype = dtype or table.dtype
@@ -162,9 +166,6 @@ def relative_position_bias(table: torch.Tensor, buckets: RelativeBuckets, query_
     if max(n_q, n_k) > 1 << 30:
         raise RuntimeError(f"{n_q} queries and {n_k} keys: 2^30 at most (unsupported shape)")
     q, k, gq, gk = (None if t is None else t.expand(size[0], t.shape[-1]).contiguous() for t in (q, k, gq, gk))
-    if ops.use_native_operators():
-        return native.host().relative_bias(table, ctypes.addressof(buckets._struct), size, batch is not None, q, k, gq, gk, q_first,
-                                           k_first, dtype)
     if _wants_grad(table):
         return _RelativeBias.apply(table, buckets, size, batch is not None, q, k, gq, gk, q_first, k_first, dtype)
     return ops.relative_bias(buckets._struct, table.contiguous(), size, (q, q_first), (k, k_first), (gq, gk), dtype, batch is not None)

@@ -1,7 +1,9 @@
 """Residual dropout and the relative position bias on the CPU: the oracle's generator against published numbers, the
 buckets, and what the entry points refuse before anything is launched."""
+import copy
 import ctypes
 import math
+import pickle
 
 import numpy as np
 import pytest
@@ -60,6 +62,14 @@ def test_common_buckets_by_value():
 def test_buckets_that_no_kernel_takes_are_refused(args, kw):
     with pytest.raises(ValueError):
         P.RelativeBuckets(*args, **kw)
+
+
+def test_buckets_and_module_are_copied_whole():
+    m = P.RelativePositionBias(4, P.RelativeBuckets(128, 32), grouped=True)
+    for c in (copy.deepcopy(m), pickle.loads(pickle.dumps(m))):
+        assert c.buckets._struct is not m.buckets._struct and bytes(c.buckets._struct) == bytes(m.buckets._struct)
+        assert c.buckets.bucket(50) == m.buckets.bucket(50) and c.weight.shape == (33, 4)
+    assert list(m.state_dict()) == ["weight"]
 
 
 def test_cpu_tensors_are_refused():
