@@ -15,8 +15,8 @@
 // about two cycles a lane, so a step of 8 queries by 8 keys makes few: one where all its differences share a bucket, one per difference
 // (and not even that where neighbours share one) along the diagonal, one per element only where positions jump.
 //
-// Us of [2, 16, 2048, 2048] bf16, 32 buckets to a distance of 128: forward 53 (5.0 TB/s); gradient with its sums 204 with an addition per
-// element, 103 with one per step or query, 55 (4.9 TB/s) with those along the diagonal.
+// Us of [2, 16, 2048, 2048] bf16, 32 buckets to a distance of 128: forward 60 (4.4 TB/s; 48 into memory that is in the caches); gradient
+// with its sums 204 with an addition per element, 103 with one per step or query, 55 (4.9 TB/s) with those along the diagonal.
 #include <algorithm>
 
 #include "../../include/protenix_amd.h"
@@ -420,16 +420,24 @@ static Tiling tiling(int batch, int q_len, int k_len, int most, int threads, int
 // (16 heads, one query, 4001 keys: 7.9 us with units of up to 256, 5.5 now).
 constexpr int64_t kFewVectors = 16384;
 
+// Heads of a workgroup, which share its look-ups.  More write more planes of the bias at one offset at a time, and memory takes writes
+// a power of two apart badly: us of [2, 16, 2048, 2048] bf16 into memory that is not in the caches with 16 heads 99, 8 84, 4 61, 2 65, 1 69.
+constexpr int kHeadsAtOnce = 4;
+
 template <typename T>
 int relative_bias_fwd(const Buckets& bk, const void* table, int table_type, T* out, int batch, int heads, int q_len, int k_len,
                       const int64_t* q_pos, const int64_t* k_pos, int64_t q_first, int64_t k_first, const int64_t* q_group,
                       const int64_t* k_group, hipStream_t stream) {
   const int n_buckets = bk.count + (q_group != nullptr);
-  int at_once = std::min(heads, std::max(1, 16384 / (n_buckets * (int)sizeof(T)))), head_groups = (heads + at_once - 1) / at_once;
+  int at_once = std::min(heads, kHeadsAtOnce), head_groups = (heads + at_once - 1) / at_once;
   const bool few = (int64_t)batch * q_len * ((k_len + 7) / 8) < kFewVectors;
-  Tiling t = tiling(batch, q_len, k_len, few ? 64 : 256, 256, std::max(1, 2048 / head_groups), 8 * head_groups, 1);
-  // (fewer rows than a workgroup holds side by side: heads take their place)
+  Tiling t = tiling(batch, q_len, k_len, few ? 64 : 256, 256, std::max(1, 2048 / head_groups), 8 * head_groups, 4);
+  // (fewer rows than a workgroup holds side by side: heads take their place, as many as keep the threads busy and the table in 16 KB)
   t.by_head = q_len < t.at_once && heads > 1;
+  if (t.by_head) {
+    at_once = std::min({heads, std::max(t.at_once, kHeadsAtOnce), std::max(kHeadsAtOnce, 16384 / (n_buckets * (int)sizeof(T)))});
+    head_groups = (heads + at_once - 1) / at_once;
+  }
   while (at_once > (t.by_head ? t.at_once : 1) && (int64_t)t.units * head_groups < 512) {
     at_once = (at_once + 1) / 2;
     head_groups = (heads + at_once - 1) / at_once;
