@@ -1256,7 +1256,8 @@ static int relative_bias_args(const char* what, const ptx_relative_buckets* bk, 
                            bk->pos_base + (int64_t)bk->pos_step * (bk->side - 1)};
   for (int64_t e : ends) PTX_REQUIRE(e >= 0 && e < bk->count, PTX_ERR_BAD_ARG, "%s: bucket %lld outside 0..%d", what, (long long)e, bk->count - 1);
   PTX_REQUIRE(!q_group == !k_group, PTX_ERR_BAD_ARG, "%s: groups of the queries without the keys' or the reverse", what);
-  PTX_REQUIRE((double)batch * heads * q_len * k_len < 1e11 && heads <= 32768 && q_len <= 1 << 30 && k_len <= 1 << 30,
+  // (units of work are numbered in 31 bits, with room for a grid's step behind the last: one per batch and 512 keys or 128 queries at most)
+  PTX_REQUIRE((double)batch * heads * q_len * k_len < 1e11 && heads <= 32768 && batch <= 1 << 30 && q_len <= 1 << 30 && k_len <= 1 << 30,
               PTX_ERR_UNSUPPORTED, "%s: too large", what);
   return PTX_OK;
 }

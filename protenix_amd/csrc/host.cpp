@@ -1439,7 +1439,7 @@ optional<Tensor> relative_bias(const Tensor& table, uintptr_t buckets, const py:
   }
   c.batched = batch >= 0;
   if (!c.batched) batch = 1;
-  if (q.n > (int64_t)1 << 30 || k.n > (int64_t)1 << 30 || batch > 0x7fffffff) return c10::nullopt;
+  if (q.n > (int64_t)1 << 30 || k.n > (int64_t)1 << 30 || batch > (int64_t)1 << 30) return c10::nullopt;
   c.size[0] = (int)batch;
   c.size[1] = (int)table.size(1);
   c.size[2] = (int)q.n;
@@ -1491,4 +1491,10 @@ PYBIND11_MODULE(_host, m) {
   m.def("dropout_add", &dropout_add);
   m.def("dropout_add_layer_norm", &dropout_add_layer_norm);
   m.def("relative_bias", &relative_bias);
+  m.def("refuse_foreign_accumulators", [](const std::vector<Tensor>& inputs) {
+    for (const Tensor& t : inputs) {
+      at::DeviceGuard dev(t.device());
+      refuse_foreign_accumulators(current_stream(t), {&t});
+    }
+  }, "raises where a call on these GPU tensors is being recorded into a graph that their gradients cannot be recorded into");
 }

@@ -91,6 +91,11 @@ class _DropoutAdd(torch.autograd.Function):
         return dx, grad if ctx.needs_input_grad[1] else None, None, None, None, None
 
 
+def _refuse_foreign_accumulators(*tensors: Optional[torch.Tensor]) -> None:
+    """What the native path asks itself: a gradient recorded into a graph must not reach a leaf that an eager graph holds elsewhere."""
+    native.host().refuse_foreign_accumulators([t for t in tensors if t is not None])
+
+
 def dropout_add(x: torch.Tensor, residual: Optional[torch.Tensor] = None, p: float = 0.1, *, shared_dim: Optional[int] = None,
                 training: bool = True, seed: Seed = None) -> torch.Tensor:
     """residual + dropout(x), or dropout(x) without a residual; differentiable in both.
@@ -116,6 +121,7 @@ def dropout_add(x: torch.Tensor, residual: Optional[torch.Tensor] = None, p: flo
     if x.numel() == 0:
         return x + x if residual is None else residual + x      # (nothing to launch; shapes and gradients as torch has them)
     if _wants_grad(x, residual):
+        _refuse_foreign_accumulators(x, residual)
         return _DropoutAdd.apply(x, residual, rows, p, number, tensor)
     return ops.dropout_add(x, residual, x.dtype if residual is None else residual.dtype, rows, p, (number, tensor))
 
@@ -175,6 +181,7 @@ def dropout_add_layer_norm(x: torch.Tensor, residual: Optional[torch.Tensor] = N
                                + ", ".join(f"{tuple(u.shape)} {u.dtype} on {u.device}" for u in params))
     number, tensor = _seed(seed, p, x)
     if _wants_grad(x, residual, weight, bias):
+        _refuse_foreign_accumulators(x, residual, weight, bias)
         return _DropoutAddLayerNorm.apply(x, residual, weight, bias, rows, p, float(eps), number, tensor)
     x, residual, weight, bias = (None if t is None else t.contiguous() for t in (x, residual, weight, bias))
     return ops.dropout_add_layer_norm(x, residual, weight, bias, rows, p, float(eps), (number, tensor), False)[:2]

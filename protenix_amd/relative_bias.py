@@ -16,7 +16,7 @@ import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
 from . import _lib, native, ops
-from .dropout import _wants_grad
+from .dropout import _refuse_foreign_accumulators, _wants_grad
 
 Positions = Union[range, torch.Tensor]
 MAX_BUCKETS, MAX_DISTANCE = 255, 8192      # as the kernels take them
@@ -163,10 +163,11 @@ def relative_position_bias(table: torch.Tensor, buckets: RelativeBuckets, query_
         raise RuntimeError(f"positions and groups of different batch sizes {sorted(batches)}")
     batch = batches.pop() if batches else None
     size = (1 if batch is None else batch, table.shape[1], n_q, n_k)
-    if max(n_q, n_k) > 1 << 30:
-        raise RuntimeError(f"{n_q} queries and {n_k} keys: 2^30 at most (unsupported shape)")
+    if max(size[0], n_q, n_k) > 1 << 30:
+        raise RuntimeError(f"a batch of {size[0]} with {n_q} queries and {n_k} keys: 2^30 at most (unsupported shape)")
     q, k, gq, gk = (None if t is None else t.expand(size[0], t.shape[-1]).contiguous() for t in (q, k, gq, gk))
     if _wants_grad(table):
+        _refuse_foreign_accumulators(table)
         return _RelativeBias.apply(table, buckets, size, batch is not None, q, k, gq, gk, q_first, k_first, dtype)
     return ops.relative_bias(buckets._struct, table.contiguous(), size, (q, q_first), (k, k_first), (gq, gk), dtype, batch is not None)
 

@@ -263,3 +263,29 @@ def test_side_streams_and_threads():
     assert len(got) == 3
     for g in got.values():
         assert torch.equal(g[0], want) and torch.equal(g[1], want_g[0]) and torch.equal(g[2], want_g[1])
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_recorded_gradients_of_a_leaf_that_an_eager_graph_holds_are_refused(native, monkeypatch):
+    # in each operator and on both host paths (the Python one also takes what the native one hands back: int32 positions, large seeds)
+    monkeypatch.setattr(ops, "native_enabled", native)
+    x, w = (torch.randn(s, device="cuda", requires_grad=True) for s in ((8, 16), (16,)))
+    table, buckets = torch.randn(9, 2, device="cuda", requires_grad=True), P.RelativeBuckets(4)
+    pos = torch.arange(5, device="cuda", dtype=torch.int32)
+    calls = [lambda: P.dropout_add(x, None, 0.5, seed=1), lambda: P.dropout_add(x, None, 0.5, seed=1 << 63),
+             lambda: P.dropout_add_layer_norm(x.detach(), None, w, None, 0.5, seed=1),
+             lambda: P.dropout_add_layer_norm(x.detach(), x, None, None, 0.5, seed=1 << 63),
+             lambda: P.relative_position_bias(table, buckets, range(5), range(5)),
+             lambda: P.relative_position_bias(table, buckets, pos, pos)]
+    alive = [f() for f in calls]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for f in calls:
+            with pytest.raises(RuntimeError, match="eager graph that is still alive"):
+                f()
+        with torch.no_grad():      # (nothing to accumulate: taken)
+            out = [f() for f in calls]
+    graph.replay()
+    torch.cuda.synchronize()
+    flat = lambda l: [t for o in l for t in (o if isinstance(o, tuple) else (o,))]
+    assert all(torch.equal(a, b) for a, b in zip(flat(out), flat(alive)))

@@ -257,3 +257,11 @@ def test_recorded_and_replayed():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, c) for a, c in zip(outs, step())), rep
+
+
+def test_batches_beyond_the_units_a_launch_can_number_are_refused():
+    b, t = P.RelativeBuckets(4), torch.zeros(9, 1, device="cuda")
+    one = torch.zeros(1, 1, dtype=torch.int64, device="cuda")
+    for n in ((1 << 30) + 1, (1 << 32) + 1):
+        with pytest.raises(RuntimeError, match="unsupported"):
+            P.relative_position_bias(t, b, one.expand(n, 1), range(1))

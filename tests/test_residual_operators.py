@@ -138,3 +138,12 @@ def test_c_relative_bias_refuses_before_a_launch():
         assert lib.ptx_relative_bias_bwd(ctypes.addressof(bad), None, None, None, 1, 4, 3, 3, None, None, 0, 0, None, None, 0, 0, None) == rc
     assert lib.ptx_relative_bias_bwd(ctypes.addressof(ok), None, None, None, 1, 4, 3, 3, None, None, 0, 0, None, None, 0, 0, None) == 1
     assert lib.ptx_relative_bias_bwd_workspace_elems(4, 32) >= 4 * 32
+
+
+def test_c_relative_bias_refuses_batches_whose_units_it_cannot_number():
+    lib = _lib.load()
+    buckets = P.RelativeBuckets(32)._struct
+    for batch in ((1 << 30) + 1, (1 << 31) - 1):
+        args = (batch, 1, 1, 1, None, None, 0, 0, None, None, 0, 0, None)
+        assert lib.ptx_relative_bias_fwd(ctypes.addressof(buckets), None, None, *args) == 2
+        assert lib.ptx_relative_bias_bwd(ctypes.addressof(buckets), None, None, None, *args) == 2
