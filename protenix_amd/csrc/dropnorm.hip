@@ -11,7 +11,7 @@
 // The backward pass takes h from memory where it is fp32, and forms it again from x and the residual where the stream
 // has 16 bits: xh of a rounded h would leave dgamma with an error of 2^-8 instead of 2^-24, for the sake of one
 // 16-bit read.  Bound by memory: 16384 rows of 2048 bf16 forward 54 us (5.0 TB/s), backward 80 and 5 for the sums (5.0 TB/s of its
-// 12 bytes an element; 50 and 75 where its tensors are partly in the caches); 147456 rows of 128 bf16 on fp32 45 and 51 us; a plain
+// 12 bytes an element; 50 and 75 where its tensors are partly in the caches); 147456 rows of 128 bf16 on fp32 47 and 51 us; a plain
 // copy reaches 5.8 TB/s.  dgamma and dbeta: column sums in registers over the rows a workgroup walks, one row of fp32 partial sums per
 // workgroup, added in a fixed order by layernorm_bwd_reduce (no atomics).
 #include <algorithm>
