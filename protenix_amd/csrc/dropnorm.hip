@@ -6,7 +6,7 @@
 //              dgamma = sum_rows dy xh,  dbeta = sum_rows dy
 //
 // A row lies over its lanes in registers, one block of 8 columns per lane (= one draw of the mask, see dropout.h), two for
-// rows of more than 8192 columns: G lanes of a wave for up to 512 columns, as many waves of a workgroup as hold it
+// rows of more than 8192 columns: 1 to 64 lanes of a wave for up to 512 columns, as many waves of a workgroup as hold it
 // beyond, whose sums meet in LDS.  Statistics are fp32 and taken in two passes over the registers, from the sum before it is rounded to h.
 // The backward pass takes h from memory where it is fp32, and forms it again from x and the residual where the stream
 // has 16 bits: xh of a rounded h would leave dgamma with an error of 2^-8 instead of 2^-24, for the sake of one
@@ -286,7 +286,7 @@ __global__ __launch_bounds__((Lay<G, WAVES>::kThreads)) void dropnorm_bwd_kernel
 
 // The first layout that holds a row's blocks of 8 columns: (lanes, waves at most, blocks per lane, fewer than 8 columns).
 #define PTX_DN_LAYOUTS(X) \
-  X(8, 1, 1, true) X(8, 1, 1, false) X(16, 1, 1, false) X(32, 1, 1, false) X(64, 1, 1, false) X(64, 8, 1, false) X(64, 16, 1, false) \
+  X(1, 1, 1, true) X(1, 1, 1, false) X(2, 1, 1, false) X(4, 1, 1, false) X(8, 1, 1, false) X(16, 1, 1, false) X(32, 1, 1, false) X(64, 1, 1, false) X(64, 8, 1, false) X(64, 16, 1, false) \
   X(64, 16, 2, false)
 constexpr int kDropnormCols = 16384;
 
@@ -301,7 +301,7 @@ template <int G, int WAVES, int NC> static Walk walk(int64_t rows, int n_vec, in
   Walk w;
   w.threads = WAVES == 1 ? 256 : (n_vec + 64 * NC - 1) / (64 * NC) * 64;
   const int64_t batches = (rows + Lay<G, WAVES>::kRows - 1) / Lay<G, WAVES>::kRows;
-  w.groups = (int)std::min<int64_t>({batches, std::max<int64_t>(256, batches / turns), std::max(1, 256 * waves_per_cu / (w.threads / 64))});
+  w.groups = (int)std::min<int64_t>({batches, std::max<int64_t>(256, batches / turns), std::max(256, 256 * waves_per_cu / (w.threads / 64))});
   return w;
 }
 #define PTX_DN_FITS(G, WAVES, NC, SHORT) (SHORT ? cols < 8 : n_vec <= G * WAVES * NC)

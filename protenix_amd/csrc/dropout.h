@@ -90,10 +90,10 @@ template <int CTRL> __device__ __forceinline__ float lane_move(float v) {
   return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true));
 }
 template <int G> __device__ __forceinline__ float lanes_sum(float v) {
-  static_assert(G == 8 || G == 16 || G == 32 || G == 64, "8, 16, 32 or 64 lanes");
-  v += lane_move<0xB1>(v);      // lane ^ 1 (within four: 1 0 3 2)
-  v += lane_move<0x4E>(v);      // lane ^ 2 (2 3 0 1)
-  v += lane_move<0x141>(v);     // 7 - lane within 8: the other four
+  static_assert(G >= 1 && G <= 64 && (G & (G - 1)) == 0, "a power of two of lanes");
+  if constexpr (G >= 2) v += lane_move<0xB1>(v);       // lane ^ 1 (within four: 1 0 3 2)
+  if constexpr (G >= 4) v += lane_move<0x4E>(v);       // lane ^ 2 (2 3 0 1)
+  if constexpr (G >= 8) v += lane_move<0x141>(v);      // 7 - lane within 8: the other four
   if constexpr (G >= 16) v += lane_move<0x140>(v);      // 15 - lane within 16: the other eight
   // (the results by way of variables: a cast of a vector's element takes the first one)
   if constexpr (G >= 32) {
@@ -161,9 +161,14 @@ template <bool NT = false, typename T> __device__ __forceinline__ void store_col
     const Raw8<T> o = rounded<T>(v);
     if (NT) __builtin_nontemporal_store(o, to); else *to = o;
   } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (e < n) p[e] = (T)v[e];
+    // four, two and one of them, as n has them (a wave that stores its last lane's up to 7 one by one waits for 7 stores)
+    typedef T T4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+    typedef T T2 __attribute__((ext_vector_type(2), aligned(sizeof(T))));
+    const bool behind4 = n & 4, behind2 = n & 2;
+    if (n & 4) *reinterpret_cast<T4*>(p) = T4{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+    if (n & 2) *reinterpret_cast<T2*>(p + (n & 4)) = T2{(T)(behind4 ? v[4] : v[0]), (T)(behind4 ? v[5] : v[1])};
+    const float last = behind4 ? (behind2 ? v[6] : v[4]) : behind2 ? v[2] : v[0];
+    if (n & 1) p[n & 6] = (T)last;
   }
 }
 
