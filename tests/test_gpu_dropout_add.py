@@ -289,3 +289,12 @@ def test_recorded_gradients_of_a_leaf_that_an_eager_graph_holds_are_refused(nati
     torch.cuda.synchronize()
     flat = lambda l: [t for o in l for t in (o if isinstance(o, tuple) else (o,))]
     assert all(torch.equal(a, b) for a, b in zip(flat(out), flat(alive)))
+
+
+@pytest.mark.parametrize("types", TYPES)
+@pytest.mark.parametrize("shared_dim", [None, 0])
+def test_rows_that_end_anywhere_in_a_block(types, shared_dim):
+    for cols in range(1, 24):
+        x, r, d = _inputs((6, 3, cols), *types, seed=cols)
+        out = P.dropout_add(x, r, 0.2, shared_dim=shared_dim, seed=cols)
+        _compare(x, r, d, 0.2, cols, shared_dim, out, torch.autograd.grad(out, [x, r], d))

@@ -280,3 +280,18 @@ def test_recorded_and_replayed():
         want = step()
         assert all(torch.equal(a, c) for a, c in zip(outs, want)), rep
         assert all(torch.equal(a, c) for a, c in zip(outs2, want)), rep
+
+
+@pytest.mark.parametrize("types", TYPES)
+def test_few_columns(types):
+    # one, two and four lanes to a row, every length of its last block
+    for cols in (*range(2, 7), *range(9, 20), 23, 25, 31, 32, 33):
+        args = _inputs((3, 101, cols), *types, seed=cols)
+        _compare(*args, 0.15, cols, None, 1e-5, *_run(*args, 0.15, cols))
+
+
+@pytest.mark.parametrize("types", [(BF16, BF16), (BF16, F32)])
+@pytest.mark.parametrize("rows,cols", [(300001, 5), (70001, 27), (2600, 1500), (1900, 2800), (1100, 5001), (800, 7000)])
+def test_walks_of_several_turns(types, rows, cols):
+    args = _inputs((rows, cols), *types, seed=cols)
+    _compare(*args, 0.1, 3, None, 1e-5, *_run(*args, 0.1, 3))

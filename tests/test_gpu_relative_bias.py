@@ -265,3 +265,17 @@ def test_batches_beyond_the_units_a_launch_can_number_are_refused():
     for n in ((1 << 30) + 1, (1 << 32) + 1):
         with pytest.raises(RuntimeError, match="unsupported"):
             P.relative_position_bias(t, b, one.expand(n, 1), range(1))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("heads", [1, 5])
+def test_rows_that_end_anywhere_in_a_block(dtype, heads):
+    for k in range(1, 24):
+        _run((5, None, False), heads, range(7, 20), range(k), dtype=dtype, seed=k)
+
+
+@pytest.mark.parametrize("batch,heads,q", [(700, 16, 1), (300, 40, 3), (1, 300, 2)])
+def test_heads_side_by_side(batch, heads, q):
+    g = torch.Generator().manual_seed(batch)
+    pos = torch.randint(-40, 40, (batch, 65), generator=g).cuda()
+    _run((32, None, True), heads, pos[:, :q].contiguous(), pos, dtype=BF16)
