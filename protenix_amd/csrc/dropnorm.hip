@@ -10,8 +10,8 @@
 // beyond, whose sums meet in LDS.  Statistics are fp32 and taken in two passes over the registers, from the sum before it is rounded to h.
 // The backward pass takes h from memory where it is fp32, and forms it again from x and the residual where the stream
 // has 16 bits: xh of a rounded h would leave dgamma with an error of 2^-8 instead of 2^-24, for the sake of one
-// 16-bit read.  Bound by memory: 16384 rows of 2048 bf16 forward 54 us (5.0 TB/s), backward 80 and 5 for the sums (5.0 TB/s of its
-// 12 bytes an element; 50 and 75 where its tensors are partly in the caches); 147456 rows of 128 bf16 on fp32 47 and 51 us; a plain
+// 16-bit read.  Bound by memory: 16384 rows of 2048 bf16 forward 48 us (5.6 TB/s), backward 80 and 5 for the sums (5.0 TB/s of its
+// 12 bytes an element; 75 where its tensors are partly in the caches); 147456 rows of 128 bf16 on fp32 44 and 51 us; a plain
 // copy reaches 5.8 TB/s.  dgamma and dbeta: column sums in registers over the rows a workgroup walks, one row of fp32 partial sums per
 // workgroup, added in a fixed order by layernorm_bwd_reduce (no atomics).
 #include <algorithm>
@@ -293,21 +293,27 @@ constexpr int kDropnormCols = 16384;
 int dropnorm_max_cols() { return kDropnormCols; }
 
 // A launch's shape: workgroups of one row in the fewest waves that hold it, or of four waves of rows, which walk the rows: the same number
-// of them for each of the 256 compute units, or as have `turns` turns to make (but one per compute unit).  That number holds `waves` waves
-// at most (`fill`: or is the first that holds as many): with 256 waves / w of them, whatever that leaves over, some units walk two shares
-// one after the other (64 M bf16 elements in rows of 5000 forward 3.9 TB/s, with 3 for each 4.4; of 2800 backward 4.0, with 2 4.9).
+// of them for each of the 256 compute units, the first that holds `waves` waves, or as have `turns` turns to make (but one per compute
+// unit).  (With 256 waves / w of them, whatever that leaves over, some units walk two shares one after the other: 64 M bf16
+// elements in rows of 2800 backward 4.0 TB/s, with 2 for each 4.9.)
 struct Walk {
   int groups, threads;
 };
-template <int G, int WAVES, int NC> static Walk walk(int64_t rows, int n_vec, int waves, bool fill, int turns) {
+template <int G, int WAVES, int NC> static Walk walk(int64_t rows, int n_vec, int waves, int turns) {
   Walk w;
   w.threads = WAVES == 1 ? 256 : (n_vec + 64 * NC - 1) / (64 * NC) * 64;
   const int64_t batches = (rows + Lay<G, WAVES>::kRows - 1) / Lay<G, WAVES>::kRows;
-  const int own = w.threads / 64, per_cu = std::max(1, (waves + (fill ? own - 1 : 0)) / own);
-  w.groups = (int)std::min<int64_t>({batches, std::max<int64_t>(256, batches / turns), 256 * per_cu});
+  const int own = w.threads / 64, per_cu = (waves + own - 1) / own;
+  w.groups = (int)std::min<int64_t>({batches, std::max<int64_t>(256, batches / turns), (int64_t)256 * per_cu});
   return w;
 }
 #define PTX_DN_FITS(G, WAVES, NC, SHORT) (SHORT ? cols < 8 : n_vec <= G * WAVES * NC)
+
+// Waves of a compute unit that walk the forward pass (24 fit).  TB/s of 64 M bf16 elements with 16, 32 and 64 of them, and with as many
+// as there are rows: rows of 128 4.9, 4.9, 5.0 and 5.6, of 512 5.1, 5.0, 4.9 and 5.6, but of 384 (lanes without columns) 4.8, 4.6, 4.9
+// and 4.4, of 65 3.0, 3.0, 3.2 and 2.0; several waves to a row: of 2048 5.3, 5.0, 5.3 and 5.2, of 4096 5.5, 4.9, 5.2 and 5.2, of 5000
+// with two, three, six workgroups and all 5.0, 4.3, 4.3 and 3.7.
+template <int G, int WAVES> static int fwd_waves(int cols) { return WAVES > 1 ? 16 : cols == 8 * G ? 1 << 15 : 64; }
 
 template <typename TX, typename TR>
 int dropnorm_fwd(const TX* x, const TR* res, const void* gamma, const void* beta, int param_type, TX* y, TR* h, float* mean,
@@ -316,7 +322,7 @@ int dropnorm_fwd(const TX* x, const TR* res, const void* gamma, const void* beta
   const int n_vec = (cols + 7) / 8;
 #define PTX_DN_CASE(G, WAVES, NC, SHORT)                                                                              \
   if (PTX_DN_FITS(G, WAVES, NC, SHORT)) {                                                                             \
-    const Walk w = walk<G, WAVES, NC>(rows, n_vec, 32, false, 1);                                                       \
+    const Walk w = walk<G, WAVES, NC>(rows, n_vec, fwd_waves<G, WAVES>(cols), 1);                                    \
     auto* kernel = res ? dropnorm_fwd_kernel<TX, TR, G, WAVES, NC, SHORT, true> : dropnorm_fwd_kernel<TX, TR, G, WAVES, NC, SHORT, false>; \
     kernel<<<dim3(w.groups), dim3(w.threads), 0, stream>>>(x, res, NormParam{gamma, param_type}, NormParam{beta, param_type}, y, h,    \
                                                            mean, rstd, rows, cols, eps, drop);                        \
@@ -347,7 +353,7 @@ int dropnorm_bwd(const TX* dy, const TR* dh, const TX* x, const TR* res, const T
   auto launch = [&]() {
 #define PTX_DN_CASE(G, WAVES, NC, SHORT)                                                               \
   if (PTX_DN_FITS(G, WAVES, NC, SHORT)) {                                                              \
-    const Walk w = walk<G, WAVES, NC>(rows, n_vec, kDropnormBwdWaves, true, kDropnormBwdTurns);        \
+    const Walk w = walk<G, WAVES, NC>(rows, n_vec, kDropnormBwdWaves, kDropnormBwdTurns);        \
     parts = w.groups;                                                                                  \
     dropnorm_bwd_kernel<TX, TR, G, WAVES, NC, SHORT><<<dim3(parts), dim3(w.threads), 0, stream>>>(     \
         dy, dh, x, res, h, mean, rstd, NormParam{gamma, param_type}, dx, dres, part, rows, cols, drop); \
