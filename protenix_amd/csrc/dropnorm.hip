@@ -333,9 +333,11 @@ int dropnorm_fwd(const TX* x, const TR* res, const void* gamma, const void* beta
   return 1;
 }
 
-// Backward: waves per compute unit, and turns of a workgroup at the least, which leaves a row of partial sums each.  Us of
-// 16384 rows of 2048 bf16 with its sums: 16 waves 89, 12 85, 8 82; of 2055 rows of 1024 fp32: 22, 19, 17, with four turns 16.
-constexpr int kDropnormBwdWaves = 8, kDropnormBwdTurns = 4;
+// Backward: waves per compute unit, and turns of a workgroup at the least, which leaves a row of partial sums each.  Us with the sums
+// of 16384 rows of 2048 bf16: 16 waves 89, 12 85, 8 82, 4 106; of 700 rows of 2048 fp32 with at least one turn 16.5, two 14.7, four 13.4; but
+// where a wave holds whole rows, of 6000 rows of 384 with one 13.2, two 13.2, four 15.4.
+constexpr int kDropnormBwdWaves = 8;
+template <int WAVES> constexpr int kDropnormBwdTurns = WAVES == 1 ? 1 : 4;
 
 int64_t dropnorm_bwd_workspace_elems(int64_t rows, int cols) {
   if (rows <= 0 || cols <= 0) return 0;
@@ -353,7 +355,7 @@ int dropnorm_bwd(const TX* dy, const TR* dh, const TX* x, const TR* res, const T
   auto launch = [&]() {
 #define PTX_DN_CASE(G, WAVES, NC, SHORT)                                                               \
   if (PTX_DN_FITS(G, WAVES, NC, SHORT)) {                                                              \
-    const Walk w = walk<G, WAVES, NC>(rows, n_vec, kDropnormBwdWaves, kDropnormBwdTurns);        \
+    const Walk w = walk<G, WAVES, NC>(rows, n_vec, kDropnormBwdWaves, kDropnormBwdTurns<WAVES>);        \
     parts = w.groups;                                                                                  \
     dropnorm_bwd_kernel<TX, TR, G, WAVES, NC, SHORT><<<dim3(parts), dim3(w.threads), 0, stream>>>(     \
         dy, dh, x, res, h, mean, rstd, NormParam{gamma, param_type}, dx, dres, part, rows, cols, drop); \
