@@ -141,7 +141,10 @@ __global__ __launch_bounds__((Lay<G, WAVES>::kThreads)) void dropnorm_fwd_kernel
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         v[c][e] -= mean;
-        q[0] = __builtin_fmaf(v[c][e], e < n[c] ? v[c][e] : 0.0f, q[0]);
+        // (selected, then squared: a lane without columns holds the row's last ones under another block's mask, and an infinity that is
+        // dropped there times 0 is NaN)
+        const float t = e < n[c] ? v[c][e] : 0.0f;
+        q[0] = __builtin_fmaf(t, t, q[0]);
       }
     row_sums<G, WAVES>(q, slots, turn);
     const float rstd = rsqrtf(q[0] * inv_n + eps);

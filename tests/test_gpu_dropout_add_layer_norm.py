@@ -295,3 +295,19 @@ def test_few_columns(types):
 def test_walks_of_several_turns(types, rows, cols):
     args = _inputs((rows, cols), *types, seed=cols)
     _compare(*args, 0.1, 3, None, 1e-5, *_run(*args, 0.1, 3))
+
+
+@pytest.mark.parametrize("types", [(F32, F32), (BF16, BF16), (F16, F32)])
+@pytest.mark.parametrize("cols", [7, 24, 67, 128, 136, 384, 768, 1035, 2056, 8200, 9000])
+def test_dropped_values_do_not_matter(types, cols):
+    """Infinities, NaN and values that the factor would carry beyond the type, in all dropped places: the results and gradients are, bit by
+    bit, those of zeros there.  Lanes of a row without columns of their own hold its last 8 columns under another block's mask."""
+    for shared_dim in (None, 0):
+        x, r, w, b, dy, dh = _inputs((3, 37 if cols < 2000 else 5, cols), *types, seed=cols)
+        keep = R.keep_mask(x.shape, 0.25, 31, shared_dim).cuda()
+        odd = torch.tensor([float("inf"), float("nan"), float("-inf"), torch.finfo(types[0]).max], device="cuda").to(types[0])
+        odd = odd[torch.arange(x.numel(), device="cuda") % 4].view(x.shape)
+        runs = [_run(torch.where(keep, x.detach(), there).requires_grad_(), r, w, b, dy, dh, 0.25, 31, shared_dim)
+                for there in (torch.zeros_like(odd), odd)]
+        for name, want, got in zip(("y", "h", *"xrwb"), *((y, h, *(g[n] for n in "xrwb")) for y, h, g in runs)):
+            assert want.isfinite().all() and torch.equal(want, got), (name, shared_dim)
