@@ -213,8 +213,8 @@ __global__ __launch_bounds__((Lay<G, WAVES>::kThreads)) void dropnorm_bwd_kernel
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       keeps[c] = dropout_keeps(drop, mask_row_of(drop, (uint32_t)row), c * span + lane);
-      // (columns and rows beyond the end: dy = 0 and a deviation of 0 keep them out of every sum)
-      const int have = ok ? n[c] : 0, have_d = have_dy ? have : 0;
+      // (columns and rows beyond the end, and all of them without dy: dy = 0 and a deviation of 0 keep them out of every sum)
+      const int have = ok && have_dy ? n[c] : 0;
       xh[c] = used_cols<SHORT, TR>(raw_stream[c], n[c]);
       d[c] = used_cols<SHORT, TX>(raw_dy[c], n[c]);
       if (AGAIN) {
@@ -226,7 +226,7 @@ __global__ __launch_bounds__((Lay<G, WAVES>::kThreads)) void dropnorm_bwd_kernel
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         xh[c][e] = e < have ? (xh[c][e] - mu) * rs : 0.0f;
-        d[c][e] = e < have_d ? d[c][e] : 0.0f;
+        d[c][e] = e < have ? d[c][e] : 0.0f;
         const float g = gm[c][e] * d[c][e];
         s[0] += g;
         s[1] = __builtin_fmaf(g, xh[c][e], s[1]);
@@ -242,7 +242,11 @@ __global__ __launch_bounds__((Lay<G, WAVES>::kThreads)) void dropnorm_bwd_kernel
       const int64_t at = row * cols + (c * span + lane) * 8;
       const f32x8 up = used_cols<SHORT, TR>(raw_dh[c], n[c]);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) d[c][e] = __builtin_fmaf(gm[c][e] * d[c][e] - a - xh[c][e] * b, rs, have_dh ? up[e] : 0.0f);
+      for (int e = 0; e < 8; ++e) {
+        const float of_h = have_dh ? up[e] : 0.0f;
+        // (without dy dh alone: a zero times the rstd of a row that has none would be NaN)
+        d[c][e] = have_dy ? __builtin_fmaf(gm[c][e] * d[c][e] - a - xh[c][e] * b, rs, of_h) : of_h;
+      }
       if (dres) store_cols(dres + at, d[c], n[c]);
       if (dx) {
 #pragma unroll

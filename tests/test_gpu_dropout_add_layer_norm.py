@@ -311,3 +311,20 @@ def test_dropped_values_do_not_matter(types, cols):
                 for there in (torch.zeros_like(odd), odd)]
         for name, want, got in zip(("y", "h", *"xrwb"), *((y, h, *(g[n] for n in "xrwb")) for y, h, g in runs)):
             assert want.isfinite().all() and torch.equal(want, got), (name, shared_dim)
+
+
+@pytest.mark.parametrize("types", [(F32, F32), (BF16, BF16), (F16, F32)])
+@pytest.mark.parametrize("cols", [64, 136, 1035])
+def test_the_sum_alone_asks_nothing_of_the_norm(types, cols):
+    """Where y is not used, h's gradient goes on as it is: through rows without a norm (an infinity in them, or one value and
+    eps = 0) and columns whose weight is infinite too."""
+    x, r, w, b, _, dh = _inputs((6, cols), *types)
+    with torch.no_grad():
+        x[1, 3], r[2, cols - 1], r[3, 0] = float("inf"), float("-inf"), float("nan")
+        x[4], r[4] = 0.0, 2.0
+        w[5] = float("inf")
+    _, _, grads = _run(x, r, w, b, None, dh, 0.5, 7, eps=0.0)
+    keep = R.keep_mask(x.shape, 0.5, 7).cuda()
+    assert torch.equal(grads["r"], dh)
+    assert torch.equal(grads["x"], torch.where(keep, dh.float() * 2, 0.0).to(types[0]))
+    assert (grads["w"] == 0).all() and (grads["b"] == 0).all()
