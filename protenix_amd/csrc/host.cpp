@@ -12,6 +12,7 @@
 #include <torch/extension.h>
 
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/core/AutogradState.h>
 
 #include <cstring>
 #include <mutex>
@@ -1164,6 +1165,14 @@ void refuse_foreign_accumulators(hipStream_t st, std::initializer_list<const Ten
                                "accumulates on another stream; drop the results of the eager calls first");
   }
 }
+// The operators have no forward-mode derivatives: a result without a tangent would say that it is zero.  (Not where these are
+// switched off, as in the forward of a function that has a rule of its own.)
+void refuse_tangents(std::initializer_list<const Tensor*> inputs) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const Tensor* t : inputs)
+    if (t->defined() && t->_fw_grad(0).defined())
+      throw std::runtime_error("protenix_amd: this operator has no forward-mode derivative (an input is a dual tensor)");
+}
 void refuse_double_backward() {
   if (at::GradMode::is_enabled()) throw std::runtime_error("protenix_amd: this operator's gradient is not differentiable (create_graph=True)");
 }
@@ -1248,6 +1257,7 @@ optional<Tensor> dropout_add(const Tensor& x, const optional<Tensor>& residual, 
   py::gil_scoped_release nogil;
   at::DeviceGuard dev(x.device());
   const Tensor res = given(residual);
+  refuse_tangents({&x, &res});
   if (at::GradMode::is_enabled() && (wants(x) || wants(res))) {
     refuse_foreign_accumulators(current_stream(x), {&x, &res});
     return DropoutAddFn::apply(x, residual, seed, r, p, number);
@@ -1334,6 +1344,7 @@ optional<std::tuple<Tensor, Tensor>> dropout_add_layer_norm(const Tensor& x, con
   py::gil_scoped_release nogil;
   at::DeviceGuard dev(x.device());
   const Tensor res = given(residual), w = given(weight), b = given(bias);
+  refuse_tangents({&x, &res, &w, &b});
   if (at::GradMode::is_enabled() && (wants(x) || wants(res) || wants(w) || wants(b))) {
     refuse_foreign_accumulators(current_stream(x), {&x, &res, &w, &b});
     const auto out = DropoutAddLayerNormFn::apply(x, residual, weight, bias, seed, r, p, eps, number);
@@ -1448,6 +1459,7 @@ optional<Tensor> relative_bias(const Tensor& table, uintptr_t buckets, const py:
   c.k_first = k.first;
   py::gil_scoped_release nogil;
   at::DeviceGuard dev(table.device());
+  refuse_tangents({&table});
   for (Side* s : {&q, &k, &gq, &gk})
     if (s->t) s->t = (s->t->dim() == 1 && c.batched ? s->t->expand({batch, s->n}) : *s->t).contiguous();
   if (at::GradMode::is_enabled() && table.requires_grad()) {
@@ -1491,6 +1503,9 @@ PYBIND11_MODULE(_host, m) {
   m.def("dropout_add", &dropout_add);
   m.def("dropout_add_layer_norm", &dropout_add_layer_norm);
   m.def("relative_bias", &relative_bias);
+  m.def("refuse_tangents", [](const std::vector<Tensor>& inputs) {
+    for (const Tensor& t : inputs) refuse_tangents({&t});
+  }, "raises where one of the tensors carries a forward-mode tangent");
   m.def("refuse_foreign_accumulators", [](const std::vector<Tensor>& inputs) {
     for (const Tensor& t : inputs) {
       at::DeviceGuard dev(t.device());

@@ -91,6 +91,11 @@ class _DropoutAdd(torch.autograd.Function):
         return dx, grad if ctx.needs_input_grad[1] else None, None, None, None, None
 
 
+def _refuse_tangents(*tensors: Optional[torch.Tensor]) -> None:
+    """What the native path asks itself: the operators have no forward-mode derivatives."""
+    native.host().refuse_tangents([t for t in tensors if t is not None])
+
+
 def _refuse_foreign_accumulators(*tensors: Optional[torch.Tensor]) -> None:
     """What the native path asks itself: a gradient recorded into a graph must not reach a leaf that an eager graph holds elsewhere."""
     native.host().refuse_foreign_accumulators([t for t in tensors if t is not None])
@@ -98,7 +103,7 @@ def _refuse_foreign_accumulators(*tensors: Optional[torch.Tensor]) -> None:
 
 def dropout_add(x: torch.Tensor, residual: Optional[torch.Tensor] = None, p: float = 0.1, *, shared_dim: Optional[int] = None,
                 training: bool = True, seed: Seed = None) -> torch.Tensor:
-    """residual + dropout(x), or dropout(x) without a residual; differentiable in both.
+    """residual + dropout(x), or dropout(x) without a residual; differentiable in both (backward, once; forward-mode is refused).
 
     x: float32, bfloat16 or float16, any shape; residual: the same shape, in x's type or float32 (an update of 16 bits onto
     the fp32 residual stream).  The result has the residual's type; the sum is formed in fp32 and rounded once.
@@ -120,6 +125,7 @@ def dropout_add(x: torch.Tensor, residual: Optional[torch.Tensor] = None, p: flo
     number, tensor = _seed(seed, p, x)
     if x.numel() == 0:
         return x + x if residual is None else residual + x      # (nothing to launch; shapes and gradients as torch has them)
+    _refuse_tangents(x, residual)
     if _wants_grad(x, residual):
         _refuse_foreign_accumulators(x, residual)
         return _DropoutAdd.apply(x, residual, rows, p, number, tensor)
@@ -156,7 +162,8 @@ def dropout_add_layer_norm(x: torch.Tensor, residual: Optional[torch.Tensor] = N
                            bias: Optional[torch.Tensor] = None, p: float = 0.0, eps: float = 1e-5, *,
                            shared_dim: Optional[int] = None, training: bool = True,
                            seed: Seed = None) -> Tuple[torch.Tensor, torch.Tensor]:
-    """(LayerNorm(h), h) with h = residual + dropout(x), in one pass; differentiable in x, residual, weight and bias.
+    """(LayerNorm(h), h) with h = residual + dropout(x), in one pass; differentiable in x, residual, weight and bias
+    (backward, once; forward-mode is refused).
 
     x, residual, p, shared_dim, training and seed as in `dropout_add`; the norm is over the last dimension (at most 16384), of
     the fp32 sum before it is rounded to h, and has x's type; h has the residual's.  weight, bias: [x.shape[-1]], of one of the
@@ -180,6 +187,7 @@ def dropout_add_layer_norm(x: torch.Tensor, residual: Optional[torch.Tensor] = N
             raise RuntimeError(f"weight and bias are [{cols}] on {x.device} and of one type, got "
                                + ", ".join(f"{tuple(u.shape)} {u.dtype} on {u.device}" for u in params))
     number, tensor = _seed(seed, p, x)
+    _refuse_tangents(x, residual, weight, bias)
     if _wants_grad(x, residual, weight, bias):
         _refuse_foreign_accumulators(x, residual, weight, bias)
         return _DropoutAddLayerNorm.apply(x, residual, weight, bias, rows, p, float(eps), number, tensor)

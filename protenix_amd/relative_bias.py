@@ -16,7 +16,7 @@ import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
 from . import _lib, native, ops
-from .dropout import _refuse_foreign_accumulators, _wants_grad
+from .dropout import _refuse_foreign_accumulators, _refuse_tangents, _wants_grad
 
 Positions = Union[range, torch.Tensor]
 MAX_BUCKETS, MAX_DISTANCE = 255, 8192      # as the kernels take them
@@ -130,7 +130,8 @@ class _RelativeBias(torch.autograd.Function):
 def relative_position_bias(table: torch.Tensor, buckets: RelativeBuckets, query_positions: Positions, key_positions: Positions, *,
                            groups: Optional[Tuple[torch.Tensor, torch.Tensor]] = None,
                            dtype: Optional[torch.dtype] = None) -> torch.Tensor:
-    """[H, Q, K], or [B, H, Q, K] where any of the positions or groups is [B, n]; differentiable in the table.
+    """[H, Q, K], or [B, H, Q, K] where any of the positions or groups is [B, n]; differentiable in the table (backward, once;
+    forward-mode is refused).
 
     table: [buckets.num_buckets, H], float32, bfloat16 or float16 - with one row more, for pairs of different groups, where groups are
     given.  query_positions, key_positions: a `range` of step 1 (range(n, n + 1): the one query of a token
@@ -166,6 +167,7 @@ def relative_position_bias(table: torch.Tensor, buckets: RelativeBuckets, query_
     if max(size[0], n_q, n_k) > 1 << 30:
         raise RuntimeError(f"a batch of {size[0]} with {n_q} queries and {n_k} keys: 2^30 at most (unsupported shape)")
     q, k, gq, gk = (None if t is None else t.expand(size[0], t.shape[-1]).contiguous() for t in (q, k, gq, gk))
+    _refuse_tangents(table)
     if _wants_grad(table):
         _refuse_foreign_accumulators(table)
         return _RelativeBias.apply(table, buckets, size, batch is not None, q, k, gq, gk, q_first, k_first, dtype)
