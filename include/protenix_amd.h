@@ -624,7 +624,8 @@ PTX_API int ptx_dropout_add_layernorm_bwd(const void* dy, const void* dh, const 
  *   out[b][h][i][j] = table[bucket(k_pos[b][j] - q_pos[b][i])][h]
  * The bucket of a difference d with n = min(|d|, max_distance): with s the last of `side` buckets whose start is
  * at most n, neg_base + neg_step s for d <= 0 and pos_base + pos_step s for d > 0; pairs whose groups differ have bucket
- * `count` (a further row of the table, there exactly when groups are given).
+ * `count` (a further row of the table, there exactly when groups are given).  The differences of a bucket have to be
+ * one interval (buckets of |d|, which have a difference on either side of the query, are refused).
  */
 #define PTX_RELATIVE_BUCKETS_MAX 255    /* largest count */
 #define PTX_RELATIVE_DISTANCE_MAX 8192  /* largest max_distance */

@@ -1238,6 +1238,27 @@ PTX_API int ptx_dropout_add_layernorm_bwd(const void* dy, const void* dh, const 
 }
 
 // ---- learned bias by buckets of relative position ---------------------------------------------------
+// Whether the differences -max_distance .. max_distance of every bucket are one interval: each is met once on the way from one end to the
+// other.
+static bool buckets_are_intervals(const ptx_relative_buckets& bk) {
+  bool met[PTX_RELATIVE_BUCKETS_MAX] = {};
+  int last = -1;
+  auto visit = [&](int bucket) {
+    if (bucket == last) return true;
+    last = bucket;
+    const bool first = !met[bucket];
+    met[bucket] = true;
+    return first;
+  };
+  // (bucket s of a side has the n from starts[s] to the next start, if any)
+  auto end = [&](int s) { return s + 1 < bk.side ? std::min<int>(bk.starts[s + 1] - 1, bk.max_distance) : bk.max_distance; };
+  for (int s = bk.side - 1; s >= 0; --s)
+    if (end(s) >= bk.starts[s] && !visit(bk.neg_base + bk.neg_step * s)) return false;
+  for (int s = 0; s < bk.side; ++s)
+    if (end(s) >= std::max<int>(bk.starts[s], 1) && !visit(bk.pos_base + bk.pos_step * s)) return false;
+  return true;
+}
+
 static int relative_bias_args(const char* what, const ptx_relative_buckets* bk, int batch, int heads, int q_len, int k_len,
                               const int64_t* q_group, const int64_t* k_group, int table_dtype, int out_dtype) {
   PTX_REQUIRE(dtype_ok_ln(table_dtype) && dtype_ok_ln(out_dtype), PTX_ERR_BAD_ARG, "%s: unknown dtype %d or %d", what, table_dtype, out_dtype);
@@ -1255,6 +1276,7 @@ static int relative_bias_args(const char* what, const ptx_relative_buckets* bk, 
   const int64_t ends[4] = {bk->neg_base, bk->neg_base + (int64_t)bk->neg_step * (bk->side - 1), bk->pos_base,
                            bk->pos_base + (int64_t)bk->pos_step * (bk->side - 1)};
   for (int64_t e : ends) PTX_REQUIRE(e >= 0 && e < bk->count, PTX_ERR_BAD_ARG, "%s: bucket %lld outside 0..%d", what, (long long)e, bk->count - 1);
+  PTX_REQUIRE(buckets_are_intervals(*bk), PTX_ERR_UNSUPPORTED, "%s: a bucket whose differences are not one interval", what);
   PTX_REQUIRE(!q_group == !k_group, PTX_ERR_BAD_ARG, "%s: groups of the queries without the keys' or the reverse", what);
   // (units of work are numbered in 31 bits, with room for a grid's step behind the last: one per batch and 512 keys or 128 queries at most)
   PTX_REQUIRE((double)batch * heads * q_len * k_len < 1e11 && heads <= 32768 && batch <= 1 << 30 && q_len <= 1 << 30 && k_len <= 1 << 30,

@@ -5,9 +5,9 @@
 // Bound by the memory of the bias (written, and its gradient read); the buckets cost no memory.  A workgroup has a
 // byte per distance in LDS (differences beyond max_distance stand for it), made from the distances at which the buckets start.
 // A thread owns 8 neighbouring keys, kept as 32-bit offsets from a query of the workgroup's (whole 64-bit differences where some
-// position is 2^30 or more away), and walks the rows of queries.  The differences that share a bucket are an
-// interval, whatever the scheme: where a thread's keys are consecutive numbers of one group and the first and the last of them fall into
-// the same bucket, all do, and two look-ups stand for eight.  The rest is a look-up per element, shared by the heads.
+// position is 2^30 or more away), and walks the rows of queries.  The differences that share a bucket are an interval (schemes of
+// other buckets are refused at the C entry): where a thread's keys are consecutive numbers of one group and the first and the last of
+// them fall into the same bucket, all do, and two look-ups stand for eight.  The rest is a look-up per element, shared by the heads.
 //
 // Gradient: sums of millions of elements in a few buckets.  Every lane has bins of its own in LDS, [bucket][lane], and adds to
 // them in its program's order, without waiting for the sums: no two lanes ever meet in a bin (nor, a bin's bank being its lane's, in a

@@ -147,3 +147,34 @@ def test_c_relative_bias_refuses_batches_whose_units_it_cannot_number():
         args = (batch, 1, 1, 1, None, None, 0, 0, None, None, 0, 0, None)
         assert lib.ptx_relative_bias_fwd(ctypes.addressof(buckets), None, None, *args) == 2
         assert lib.ptx_relative_bias_bwd(ctypes.addressof(buckets), None, None, None, *args) == 2
+
+
+def test_c_relative_bias_refuses_buckets_that_come_back():
+    """The kernels take the differences of a bucket for an interval: |d| in buckets of its own has 2 1 0 1 2 around the query."""
+    lib = _lib.load()
+
+    def rc(buckets):
+        args = (1, 4, 0, 3, None, None, 0, 0, None, None, 0, 0, None)      # (no query: nothing to launch)
+        fwd = lib.ptx_relative_bias_fwd(ctypes.addressof(buckets), None, None, *args)
+        text = lib.ptx_last_error_string()
+        if fwd:
+            assert lib.ptx_relative_bias_bwd(ctypes.addressof(buckets), None, None, None, *args) == fwd
+        return fwd, text
+
+    both = dict(neg_base=0, neg_step=1, pos_base=0, pos_step=1)
+    singles = {i: i for i in range(16)}
+    for bad in (_buckets(max_distance=2, side=3, starts=singles, **both), _buckets(**both), _buckets(neg_base=5, neg_step=0, pos_base=2),
+                _buckets(max_distance=1, side=2, starts=singles, neg_base=0, neg_step=1, pos_base=1, pos_step=0, count=2),
+                _buckets(max_distance=2, side=3, starts=singles, neg_base=2, neg_step=-1, pos_base=2, pos_step=-1)):
+        got, text = rc(bad)
+        assert got == 2 and b"interval" in text, (got, text)
+    # the same numbers where each is met once: beyond max_distance, in empty buckets, in the query's own or on one side only
+    for good in (_buckets(max_distance=2, side=16, starts={**singles, 1: 3, 2: 3}, **both),
+                 _buckets(neg_base=3, neg_step=0, pos_base=3, pos_step=0), _buckets(neg_base=5, neg_step=0, pos_base=4),
+                 _buckets(max_distance=4, side=5, starts=singles, neg_base=4, neg_step=-1, pos_base=4, pos_step=1),
+                 _buckets(max_distance=1, side=2, starts=singles, neg_base=0, neg_step=1, pos_base=0, pos_step=0),
+                 _buckets(max_distance=8, side=2, starts={1: 0}, **both)):
+        assert rc(good)[0] == 0, rc(good)
+    for scheme in ((1, None, True), (120, None, True), (254, None, False), (128, 32, True), (128, 32, False), (8192, 254, True), (8192, 255, False),
+                   (2, 2, False), (2, 4, True), (3, 4, True)):
+        assert rc(P.RelativeBuckets(scheme[0], scheme[1], bidirectional=scheme[2])._struct)[0] == 0, scheme
