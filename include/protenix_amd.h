@@ -628,7 +628,7 @@ PTX_API int ptx_dropout_add_layernorm_bwd(const void* dy, const void* dh, const 
  * one interval (buckets of |d|, which have a difference on either side of the query, are refused).
  */
 #define PTX_RELATIVE_BUCKETS_MAX 255    /* largest count */
-#define PTX_RELATIVE_DISTANCE_MAX 8192  /* largest max_distance */
+#define PTX_RELATIVE_DISTANCE_MAX 8192  /* largest max_distance (the smallest is 1) */
 typedef struct ptx_relative_buckets {
   int32_t max_distance, count, side;
   int32_t neg_base, neg_step, pos_base, pos_step;

@@ -1265,9 +1265,9 @@ static int relative_bias_args(const char* what, const ptx_relative_buckets* bk, 
   PTX_REQUIRE(batch >= 0 && heads > 0 && q_len >= 0 && k_len >= 0, PTX_ERR_BAD_ARG, "%s: batch=%d heads=%d q_len=%d k_len=%d", what,
               batch, heads, q_len, k_len);
   PTX_REQUIRE(bk, PTX_ERR_BAD_ARG, "%s: null buckets", what);
-  PTX_REQUIRE(bk->count >= 1 && bk->count <= PTX_RELATIVE_BUCKETS_MAX && bk->max_distance >= 0 &&
+  PTX_REQUIRE(bk->count >= 1 && bk->count <= PTX_RELATIVE_BUCKETS_MAX && bk->max_distance >= 1 &&
                   bk->max_distance <= PTX_RELATIVE_DISTANCE_MAX,
-              PTX_ERR_UNSUPPORTED, "%s: %d buckets up to distance %d (%d and %d at most)", what, bk->count, bk->max_distance,
+              PTX_ERR_UNSUPPORTED, "%s: %d buckets up to distance %d (1 at least, %d and %d at most)", what, bk->count, bk->max_distance,
               PTX_RELATIVE_BUCKETS_MAX, PTX_RELATIVE_DISTANCE_MAX);
   PTX_REQUIRE(bk->side >= 1 && bk->side <= 256 && bk->starts[0] == 0, PTX_ERR_BAD_ARG, "%s: %d buckets of a side", what, bk->side);
   for (int s = 1; s < bk->side; ++s)

@@ -178,3 +178,13 @@ def test_c_relative_bias_refuses_buckets_that_come_back():
     for scheme in ((1, None, True), (120, None, True), (254, None, False), (128, 32, True), (128, 32, False), (8192, 254, True), (8192, 255, False),
                    (2, 2, False), (2, 4, True), (3, 4, True)):
         assert rc(P.RelativeBuckets(scheme[0], scheme[1], bidirectional=scheme[2])._struct)[0] == 0, scheme
+
+
+def test_c_relative_bias_refuses_a_distance_of_zero():
+    """Every d > 0 would have n = 0 and the first bucket of its side, which a look-up by min(|d|, max_distance) cannot tell from d = 0's."""
+    lib = _lib.load()
+    args = (1, 4, 0, 3, None, None, 0, 0, None, None, 0, 0, None)
+    for most, rc in ((0, 2), (1, 0)):
+        s = _buckets(max_distance=most, count=2, side=1, neg_base=0, neg_step=0, pos_base=1, pos_step=0)
+        assert lib.ptx_relative_bias_fwd(ctypes.addressof(s), None, None, *args) == rc
+        assert lib.ptx_relative_bias_bwd(ctypes.addressof(s), None, None, None, *args) == (rc or 1)      # (1: null pointers, refused later)
