@@ -1425,8 +1425,10 @@ bool take_side(const py::handle& h, const Tensor& table, Side& s, int64_t& batch
   if (over || s.first < -((int64_t)1 << 62) || s.first >= (int64_t)1 << 62) return false;
   const int64_t stop = PyLong_AsLongLongAndOverflow(py::object(h.attr("stop")).ptr(), &over);
   if (over) return false;
-  s.n = stop > s.first ? stop - s.first : 0;
-  return true;
+  // (the two may be further apart than 63 bits say; the Python path refuses lengths that no kernel takes)
+  const uint64_t n = stop > s.first ? (uint64_t)stop - (uint64_t)s.first : 0;
+  s.n = (int64_t)n;
+  return n <= (uint64_t)1 << 30;
 }
 
 // buckets: the address of a ptx_relative_buckets

@@ -97,7 +97,7 @@ def _axis(p: Positions, name: str, device: torch.device) -> Tuple[Optional[torch
             raise RuntimeError(f"{name}: a range of positions has step 1, got {p}")
         if not -(1 << 62) <= p.start < 1 << 62:
             raise RuntimeError(f"{name}: positions from {p.start} on")
-        return None, p.start, len(p), None
+        return None, p.start, max(p.stop - p.start, 0), None      # (its len() stops at 63 bits)
     return _whole(p, name, device), 0, p.shape[-1], p.shape[0] if p.dim() == 2 else None
 
 

@@ -279,3 +279,13 @@ def test_heads_side_by_side(batch, heads, q):
     g = torch.Generator().manual_seed(batch)
     pos = torch.randint(-40, 40, (batch, 65), generator=g).cuda()
     _run((32, None, True), heads, pos[:, :q].contiguous(), pos, dtype=BF16)
+
+
+def test_ranges_whose_length_passes_63_bits_are_refused():
+    b, t = P.RelativeBuckets(4), torch.zeros(9, 2, device="cuda")
+    for far in (range(-(1 << 62), 1 << 62), range(-(1 << 62), (1 << 63) - 1), range(-(1 << 62), (1 << 62) + 3), range(0, 1 << 70)):
+        for sides in ((far, range(3)), (range(3), far)):
+            with pytest.raises(RuntimeError, match="unsupported"):
+                P.relative_position_bias(t, b, *sides)
+    assert P.relative_position_bias(t, b, range(5, 3), range(3)).shape == (2, 0, 3)
+    assert P.relative_position_bias(t, b, range(5, -(1 << 70)), range(3)).shape == (2, 0, 3)
