@@ -37,8 +37,10 @@ def _rows(x: torch.Tensor, shared_dim: Optional[int]) -> tuple:
     return rows, cols, max(shape[d], 1), max(math.prod(shape[d + 1:-1]), 1)
 
 
-def _drawn() -> int:
-    if torch.cuda.is_current_stream_capturing():
+def _drawn(x: torch.Tensor) -> int:
+    with torch.cuda.device(x.device):
+        recorded = torch.cuda.is_current_stream_capturing()
+    if recorded:
         raise RuntimeError("a call recorded into a graph needs its seed: every replay would repeat the mask of a seed drawn now "
                            "(give a one-element int64 GPU tensor and change it between replays, or a whole number)")
     return int(torch.empty((), dtype=torch.int64).random_())      # torch's default generator: torch.manual_seed decides
@@ -115,7 +117,7 @@ def dropout_add(x: torch.Tensor, residual: Optional[torch.Tensor] = None, p: flo
     what the tensor holds at the time; it must not change between a call and its backward pass).  None: drawn from torch's default
     generator.  Two calls with the same seed and shape have the same mask."""
     if seed is None and training and p != 0.0 and x.is_cuda:
-        seed = _drawn()
+        seed = _drawn(x)
     if ops.use_native_operators():
         out = native.host().dropout_add(x, residual, p, shared_dim, training, seed)
         if out is not None:
@@ -170,7 +172,7 @@ def dropout_add_layer_norm(x: torch.Tensor, residual: Optional[torch.Tensor] = N
     three types, the same for both, either may be None; their gradients have their type and come out of a fixed order of
     additions.  p = 0 (the default): the residual sum and norm of a network in use."""
     if seed is None and training and p != 0.0 and x.is_cuda:
-        seed = _drawn()
+        seed = _drawn(x)
     if ops.use_native_operators():
         out = native.host().dropout_add_layer_norm(x, residual, weight, bias, p, eps, shared_dim, training, seed)
         if out is not None:

@@ -188,3 +188,27 @@ def test_c_relative_bias_refuses_a_distance_of_zero():
         s = _buckets(max_distance=most, count=2, side=1, neg_base=0, neg_step=0, pos_base=1, pos_step=0)
         assert lib.ptx_relative_bias_fwd(ctypes.addressof(s), None, None, *args) == rc
         assert lib.ptx_relative_bias_bwd(ctypes.addressof(s), None, None, None, *args) == (rc or 1)      # (1: null pointers, refused later)
+
+
+def test_a_drawn_seed_asks_the_updates_device_whether_it_records(monkeypatch):
+    """The recording may be on the stream of another device than the current one."""
+    current = [0]
+
+    class Device:
+        def __init__(self, d):
+            self.index = d.index
+
+        def __enter__(self):
+            current.append(self.index)
+
+        def __exit__(self, *_):
+            current.pop()
+
+    class Update:      # (what a tensor on the second GPU says of itself)
+        is_cuda, device = True, torch.device("cuda", 1)
+
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: current[-1] == 1)
+    for call in (P.dropout_add, P.dropout_add_layer_norm):
+        with pytest.raises(RuntimeError, match="needs its seed"):
+            call(Update(), p=0.5)
