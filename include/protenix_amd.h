@@ -609,7 +609,8 @@ PTX_API int ptx_dropout_add_layernorm_fwd(const void* x, const void* residual, c
  * Its gradients, from dy (x_dtype) and dh (stream_dtype; either may be NULL: zero).  dx (x_dtype), dresidual (stream_dtype),
  * dgamma and dbeta (param_dtype) are written where given; dgamma / dbeta need the workspace (uninitialised fp32).
  * An fp32 stream takes the forward's h (x and residual are not read); a 16-bit one x and the residual (NULL: none), from which h is
- * formed again: its rounded value would cost dgamma its accuracy.  No atomics: the sums' order is fixed.
+ * formed again: its rounded value would cost dgamma its accuracy.  dgamma and dbeta are summed in fp32, in a fixed order (no atomics).
+ * Without dy, dresidual is dh and dx its share under the mask, whatever the norm of the row is.
  */
 PTX_API int64_t ptx_dropout_add_layernorm_bwd_workspace_elems(int64_t rows, int cols);
 PTX_API int ptx_dropout_add_layernorm_bwd(const void* dy, const void* dh, const void* x, const void* residual,

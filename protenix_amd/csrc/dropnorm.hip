@@ -10,7 +10,7 @@
 // beyond, whose sums meet in LDS.  Statistics are fp32 and taken in two passes over the registers, from the sum before it is rounded to h.
 // The backward pass takes h from memory where it is fp32, and forms it again from x and the residual where the stream
 // has 16 bits: xh of a rounded h would leave dgamma with an error of 2^-8 instead of 2^-24, for the sake of one
-// 16-bit read.  Bound by memory: 16384 rows of 2048 bf16 forward 48 us (5.6 TB/s), backward 80 and 5 for the sums (5.0 TB/s of its
+// 16-bit read.  Bound by memory: 16384 rows of 2048 bf16 forward 49 us (5.5 TB/s), backward 83 and 5 for the sums (4.9 TB/s of its
 // 12 bytes an element; 75 where its tensors are partly in the caches); 147456 rows of 128 bf16 on fp32 44 and 51 us; a plain
 // copy reaches 5.8 TB/s.  dgamma and dbeta: column sums in registers over the rows a workgroup walks, one row of fp32 partial sums per
 // workgroup, added in a fixed order by layernorm_bwd_reduce (no atomics).
@@ -340,9 +340,9 @@ int dropnorm_fwd(const TX* x, const TR* res, const void* gamma, const void* beta
   return 1;
 }
 
-// Backward: waves per compute unit, and turns of a workgroup at the least, which leaves a row of partial sums each.  Us with the sums
-// of 16384 rows of 2048 bf16: 16 waves 89, 12 85, 8 82, 4 106; of 700 rows of 2048 fp32 with at least one turn 16.5, two 14.7, four 13.4; but
-// where a wave holds whole rows, of 6000 rows of 384 with one 13.2, two 13.2, four 15.4.
+// Backward: waves per compute unit, and turns of a workgroup at the least, which leaves a row of partial sums each.  Us with the sums, the
+// same tensors again and again, of 16384 rows of 2048 bf16: 16 waves 89, 12 85, 8 82, 4 106; of 700 rows of 2048 fp32 with at least one
+// turn 16.5, two 14.7, four 13.4; but where a wave holds whole rows, of 6000 rows of 384 with one 13.2, two 13.2, four 15.4.
 constexpr int kDropnormBwdWaves = 8;
 template <int WAVES> constexpr int kDropnormBwdTurns = WAVES == 1 ? 1 : 4;
 

@@ -2,7 +2,7 @@
 //
 // One pass: x, the residual and the sum are moved once, the mask costs no memory.  A thread owns one block of 8 columns of a mask
 // row and four of the rows that share it (one, where a row has a mask row of its own): the mask is drawn once for them.  Bound by
-// memory; [768, 768, 128] bf16 onto fp32 rows 128 us, its gradient 83 (5.9 and 5.5 TB/s), 65536 x 768 bf16 with a mask for
+// memory; [768, 768, 128] bf16 onto fp32 rows 127 us, its gradient 82 (5.9 and 5.5 TB/s), 65536 x 768 bf16 with a mask for
 // every row 51 and 37 us (5.9 and 5.5), where a plain copy reaches 5.8.
 #include <algorithm>
 
@@ -52,7 +52,7 @@ __global__ __launch_bounds__(256) void dropout_add_kernel(const TI* __restrict__
 
 template <typename TI, typename TO, bool RES>
 static void launch(const TI* x, const TO* res, TO* out, int64_t rows, int cols, const Dropout& drop, hipStream_t stream) {
-  constexpr int kRows = 4;      // us of the pair tensor above, forward and gradient: two 126 and 84, four 127 and 83, eight 137 and 87
+  constexpr int kRows = 4;      // us of the pair tensor above, forward and gradient, in one sweep: two 126 and 84, four 127 and 83, eight 137 and 87
   const uint32_t n_vec = (uint32_t)((cols + 7) / 8);
   const int64_t n_blocks = rows / drop.shared * n_vec;
   // (2^32 threads at most along a grid's axis)

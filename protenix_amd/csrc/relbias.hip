@@ -15,7 +15,7 @@
 // about two cycles a lane, so a step of 8 queries by 8 keys makes few: one where all its differences share a bucket, one per difference
 // (and not even that where neighbours share one) along the diagonal, one per element only where positions jump.
 //
-// Us of [2, 16, 2048, 2048] bf16, 32 buckets to a distance of 128: forward 60 (4.4 TB/s; 48 into memory that is in the caches); gradient
+// Us of [2, 16, 2048, 2048] bf16, 32 buckets to a distance of 128: forward 59 (4.5 TB/s; 48 into memory that is in the caches); gradient
 // with its sums 204 with an addition per element, 103 with one per step or query, 55 (4.9 TB/s) with those along the diagonal.
 #include <algorithm>
 
@@ -448,11 +448,12 @@ int relative_bias_fwd(const Buckets& bk, const void* table, int table_type, T* o
   return 0;
 }
 
-// Bins of a workgroup take at most this beside the look-up, so that a compute unit holds two workgroups at least.
+// Bins of a workgroup take at most this, so that a compute unit (160 KB) holds two workgroups at least, beside the queries (2 KB) and a
+// look-up of two bytes per distance: up to distances of some 2800.  Beyond, one of many bins may be alone.
 constexpr int kBinBytes = 72 * 1024;
 static int bwd_threads(int n_buckets) { return 64 * std::min(4, std::max(1, kBinBytes / (n_buckets * 256))); }
 // Workgroups of one head, a row of partial sums each: as many as the machine's LDS holds at a time (four waves to a SIMD at most) of all
-// heads together.
+// heads together.  Counted by their bins alone, as the workspace is: behind look-ups of thousands of distances some wait for others to end.
 static int bwd_slices(int heads, int n_buckets) {
   const int per_cu = std::max(1, std::min(1024 / bwd_threads(n_buckets), 150 * 1024 / (bwd_threads(n_buckets) * 4 * n_buckets)));
   return std::max(1, 256 * per_cu / heads);

@@ -169,8 +169,8 @@ def dropout_add_layer_norm(x: torch.Tensor, residual: Optional[torch.Tensor] = N
 
     x, residual, p, shared_dim, training and seed as in `dropout_add`; the norm is over the last dimension (at most 16384), of
     the fp32 sum before it is rounded to h, and has x's type; h has the residual's.  weight, bias: [x.shape[-1]], of one of the
-    three types, the same for both, either may be None; their gradients have their type and come out of a fixed order of
-    additions.  p = 0 (the default): the residual sum and norm of a network in use."""
+    three types, the same for both, either may be None; their gradients have their type and are summed in fp32, in a fixed
+    order.  p = 0 (the default): the residual sum and norm of a network in use."""
     if seed is None and training and p != 0.0 and x.is_cuda:
         seed = _drawn(x)
     if ops.use_native_operators():

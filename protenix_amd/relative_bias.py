@@ -131,7 +131,7 @@ def relative_position_bias(table: torch.Tensor, buckets: RelativeBuckets, query_
                            groups: Optional[Tuple[torch.Tensor, torch.Tensor]] = None,
                            dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """[H, Q, K], or [B, H, Q, K] where any of the positions or groups is [B, n]; differentiable in the table (backward, once;
-    forward-mode is refused).
+    forward-mode is refused), whose gradient is summed in fp32, in a fixed order.
 
     table: [buckets.num_buckets, H], float32, bfloat16 or float16 - with one row more, for pairs of different groups, where groups are
     given.  query_positions, key_positions: a `range` of step 1 (range(n, n + 1): the one query of a token
