@@ -34,7 +34,7 @@
 extern "C" {
 #endif
 
-#define PTX_ABI_VERSION 8
+#define PTX_ABI_VERSION 9
 #define PTX_API __attribute__((visibility("default")))
 
 /*
@@ -51,7 +51,7 @@ extern "C" {
 enum ptx_dtype { PTX_F32 = 0, PTX_BF16 = 1, PTX_MIXED = 2, PTX_F16 = 3 };
 /* PTX_F16 (IEEE half) is taken by the LayerNorm entry points, which dispatch on float /
  * Half / BFloat16 like the reference's kernel (layer_norm_cuda_kernel.cu:304-330), and by the
- * dropout and relative position bias entry points. */
+ * dropout, relative position bias, RMS norm and 8-bit entry points. */
 
 enum ptx_status {
   PTX_OK = 0,
@@ -653,6 +653,66 @@ PTX_API int ptx_relative_bias_bwd(const ptx_relative_buckets* buckets, const voi
                                   int batch, int heads, int q_len, int k_len, const int64_t* q_pos,
                                   const int64_t* k_pos, int64_t q_first, int64_t k_first, const int64_t* q_group,
                                   const int64_t* k_group, int table_dtype, int out_dtype, void* stream);
+
+/*
+ * Matrices in 8-bit blocks: e4m3 values (OCP: 1 sign, 4 exponent, 3 mantissa bits, largest 448, no infinities) with a scale per 128
+ * values of a row or, square, per 128 x 128.  A block with the largest magnitude a has s = max(a / 448, 2^-126) and, with
+ * i = 1 / s, q = e4m3(v i) to the nearest, ties to even; s, i and v i are each rounded to fp32.  A block with a value that
+ * is not finite has such a scale, and so has every product of it.
+ *   values  [rows][ptx_fp8_pitch(cols)] bytes (cols rounded up to 128), zeros behind the last column
+ *   scales  fp32 [blocks of cols][ptx_fp8_scale_pitch(rows)] (rows rounded up to 4; what is behind the last row is not used), or
+ *           square [blocks of rows][blocks of cols]; ptx_fp8_scale_elems() elements
+ * Values, scales and x are 16-byte aligned (x: to its element), dense otherwise.
+ */
+PTX_API int64_t ptx_fp8_pitch(int64_t cols);
+PTX_API int64_t ptx_fp8_scale_pitch(int64_t rows);
+PTX_API int64_t ptx_fp8_scale_elems(int64_t rows, int64_t cols, int square);
+/*
+ * x [rows][cols] (dtype: PTX_F32, PTX_BF16 or PTX_F16) -> q, scales: the matrix; and / or qt, scales_t: the transposed matrix [cols][rows],
+ * blocks along x's rows, as a product over the rows takes it.  Either pair may be NULL.
+ *   col_sums   sums of x over its rows [cols], col_sums_dtype, or NULL (summed in fp32, in a fixed order); needs the workspace of
+ *              ptx_fp8_col_sums_workspace_elems(rows, cols) fp32 elements, uninitialised
+ * Fewer than 2^28 blocks of 128 values of a row.
+ */
+PTX_API int64_t ptx_fp8_col_sums_workspace_elems(int64_t rows, int64_t cols);
+PTX_API int ptx_fp8_quantize(const void* x, void* q, float* scales, void* qt, float* scales_t, void* col_sums,
+                             float* workspace, int64_t rows, int64_t cols, int square, int dtype, int col_sums_dtype,
+                             void* stream);
+/*
+ * out [m][n] (out_dtype) = a b^T + bias: a [m][k] with a scale per 128 values of a row, b [n][k] with the same or, b_square, with
+ * one per 128 x 128; products of a block and sums over blocks in fp32, in a fixed order, rounded once.
+ *   bias       [n], bias_dtype, or NULL
+ *   workspace  ptx_fp8_matmul_workspace_elems(m, n, k, b_square) fp32 elements, uninitialised (none: NULL)
+ * 0 < k < 2^22, (m / 64 + 1) (n / 64 + 1) < 2^23.
+ */
+PTX_API int64_t ptx_fp8_matmul_workspace_elems(int64_t m, int64_t n, int64_t k, int b_square);
+PTX_API int ptx_fp8_matmul(const void* a, const float* a_scales, const void* b, const float* b_scales, int b_square,
+                           const void* bias, void* out, float* workspace, int64_t m, int64_t n, int64_t k,
+                           int out_dtype, int bias_dtype, void* stream);
+
+/*
+ * A residual sum and its root-mean-square norm in one pass:
+ *   h = residual + x,   y = h r gamma,   r = 1 / sqrt(mean(h^2) + eps)
+ *   x         [rows][cols], x_dtype;  residual, h [rows][cols], stream_dtype (x_dtype, or PTX_F32 beside 16-bit x)
+ *   residual  NULL: h is x, and is not written
+ *   gamma     [cols], param_dtype, or NULL
+ *   y         [rows][cols], x_dtype; with y_scales given 8-bit values [rows][ptx_fp8_pitch(cols)] and y_scales as above
+ *   rstd      fp32 [rows] or NULL: r, of the sum before it is rounded to h
+ * At most 16384 columns.  y may alias x (not in 8 bits), h the residual; every other pair must not overlap.
+ */
+PTX_API int ptx_add_rms_norm_fwd(const void* x, const void* residual, const void* gamma, void* y, float* y_scales,
+                                 void* h, float* rstd, int64_t rows, int cols, float eps, int x_dtype,
+                                 int stream_dtype, int param_dtype, void* stream);
+/*
+ * Its gradients, from dy (x_dtype) and dh (stream_dtype; either may be NULL: zero): dx (x_dtype) and dresidual (stream_dtype), which
+ * are the same numbers, and dgamma (param_dtype), written where given; dgamma needs the workspace (uninitialised fp32) and is summed
+ * in fp32, in a fixed order.  An fp32 stream takes h (x itself where there was no residual), a 16-bit one x and the residual.
+ */
+PTX_API int64_t ptx_add_rms_norm_bwd_workspace_elems(int64_t rows, int cols);
+PTX_API int ptx_add_rms_norm_bwd(const void* dy, const void* dh, const void* x, const void* residual, const void* h,
+                                 const float* rstd, const void* gamma, void* dx, void* dresidual, void* dgamma,
+                                 float* workspace, int64_t rows, int cols, int x_dtype, int stream_dtype,
+                                 int param_dtype, void* stream);
 
 #ifdef __cplusplus
 }

@@ -14,7 +14,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libprotenix_amd.so")
 
 PTX_F32, PTX_BF16, PTX_MIXED, PTX_F16 = 0, 1, 2, 3
-ABI_VERSION = 8
+ABI_VERSION = 9
 
 _p = ctypes.c_void_p
 _i = ctypes.c_int
@@ -103,6 +103,16 @@ SIGNATURES = {
     "ptx_relative_bias_fwd": (_i, [_p, _p, _p, _i, _i, _i, _i, _p, _p, _l, _l, _p, _p, _i, _i, _p]),
     "ptx_relative_bias_bwd_workspace_elems": (_l, [_i, _i]),
     "ptx_relative_bias_bwd": (_i, [_p, _p, _p, _p, _i, _i, _i, _i, _p, _p, _l, _l, _p, _p, _i, _i, _p]),
+    "ptx_fp8_pitch": (_l, [_l]),
+    "ptx_fp8_scale_pitch": (_l, [_l]),
+    "ptx_fp8_scale_elems": (_l, [_l, _l, _i]),
+    "ptx_fp8_col_sums_workspace_elems": (_l, [_l, _l]),
+    "ptx_fp8_quantize": (_i, [_p] * 7 + [_l, _l, _i, _i, _i, _p]),
+    "ptx_fp8_matmul_workspace_elems": (_l, [_l, _l, _l, _i]),
+    "ptx_fp8_matmul": (_i, [_p] * 4 + [_i] + [_p] * 3 + [_l, _l, _l, _i, _i, _p]),
+    "ptx_add_rms_norm_fwd": (_i, [_p] * 7 + [_l, _i, _f, _i, _i, _i, _p]),
+    "ptx_add_rms_norm_bwd_workspace_elems": (_l, [_l, _i]),
+    "ptx_add_rms_norm_bwd": (_i, [_p] * 11 + [_l, _i, _i, _i, _i, _p]),
     "ptx_hbm_stream": (_i, [_p, _p, _l, _i, _p]),
 }
 

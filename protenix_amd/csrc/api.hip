@@ -10,6 +10,7 @@
 #include "../../include/protenix_amd.h"
 #include "common.h"
 #include "dropout.h"
+#include "fp8.h"
 #include "kernels.h"
 
 namespace {
@@ -1310,6 +1311,100 @@ PTX_API int ptx_relative_bias_bwd(const ptx_relative_buckets* buckets, const voi
   PTX_DISPATCH_LN(out_dtype, ptx::relative_bias_bwd<T>(*buckets, (const T*)dout, dtable, table_dtype, workspace, batch, heads, q_len, k_len,
                                                        q_pos, k_pos, q_first, k_first, q_group, k_group, (hipStream_t)stream));
   return after_launch("relative_bias_bwd");
+}
+
+// ---- 8-bit blocks and the norm in front of them ------------------------------------------------------
+PTX_API int64_t ptx_fp8_pitch(int64_t cols) { return ptx::fp8_pitch(cols); }
+PTX_API int64_t ptx_fp8_scale_pitch(int64_t rows) { return ptx::fp8_scale_pitch(rows); }
+PTX_API int64_t ptx_fp8_scale_elems(int64_t rows, int64_t cols, int square) {
+  return (square ? ptx::fp8_blocks(rows) : ptx::fp8_scale_pitch(rows)) * ptx::fp8_blocks(cols);
+}
+PTX_API int64_t ptx_fp8_col_sums_workspace_elems(int64_t rows, int64_t cols) { return ptx::fp8_blocks(rows) * cols; }
+
+PTX_API int ptx_fp8_quantize(const void* x, void* q, float* scales, void* qt, float* scales_t, void* col_sums, float* workspace,
+                             int64_t rows, int64_t cols, int square, int dtype, int col_sums_dtype, void* stream) {
+  PTX_REQUIRE(dtype_ok_ln(dtype) && (!col_sums || dtype_ok_ln(col_sums_dtype)), PTX_ERR_BAD_ARG, "fp8_quantize: unknown dtype %d or %d", dtype,
+              col_sums_dtype);
+  PTX_REQUIRE(rows >= 0 && cols >= 0, PTX_ERR_BAD_ARG, "fp8_quantize: rows=%lld cols=%lld", (long long)rows, (long long)cols);
+  // (a launch has fewer than 2^32 threads: 16 per block, 256 per 128 x 128)
+  PTX_REQUIRE(rows < 0x7fffff00 && cols < 0x7fffff00 && (double)(rows + 127) * (double)ptx::fp8_blocks(cols) < 268435456.0, PTX_ERR_UNSUPPORTED,
+              "fp8_quantize: %lld rows of %lld columns are too many", (long long)rows, (long long)cols);
+  PTX_REQUIRE(!q == !scales && !qt == !scales_t, PTX_ERR_BAD_ARG, "fp8_quantize: values without scales or the reverse");
+  PTX_REQUIRE(!col_sums || workspace || rows == 0 || cols == 0, PTX_ERR_BAD_ARG, "fp8_quantize: column sums need the workspace");
+  if (cols == 0 || (rows == 0 && !col_sums)) return PTX_OK;
+  if (rows > 0) {
+    PTX_REQUIRE(x && (q || qt || col_sums), PTX_ERR_BAD_ARG, "fp8_quantize: null pointer");
+    PTX_REQUIRE(aligned16(q) && aligned16(qt), PTX_ERR_BAD_ARG, "fp8_quantize: values must be 16-byte aligned");
+    PTX_DISPATCH_LN(dtype, ptx::fp8_quantize<T>((const T*)x, q, scales, qt, scales_t, col_sums ? workspace : nullptr, rows, (int)cols,
+                                                square != 0, (hipStream_t)stream));
+  }
+  // (no rows: the sums are zero, and written by the same kernel)
+  if (col_sums)
+    ptx::column_sums(workspace, (int)ptx::fp8_blocks(rows), (int)cols, col_sums_dtype, col_sums, nullptr, (hipStream_t)stream);
+  return after_launch("fp8_quantize");
+}
+
+PTX_API int64_t ptx_fp8_matmul_workspace_elems(int64_t m, int64_t n, int64_t k, int b_square) {
+  return ptx::fp8_matmul_workspace_elems(m, n, ptx::fp8_blocks(k), b_square != 0);
+}
+
+PTX_API int ptx_fp8_matmul(const void* a, const float* a_scales, const void* b, const float* b_scales, int b_square, const void* bias,
+                           void* out, float* workspace, int64_t m, int64_t n, int64_t k, int out_dtype, int bias_dtype, void* stream) {
+  PTX_REQUIRE(dtype_ok_ln(out_dtype) && (!bias || dtype_ok_ln(bias_dtype)), PTX_ERR_BAD_ARG, "fp8_matmul: unknown dtype %d or %d", out_dtype,
+              bias_dtype);
+  PTX_REQUIRE(m >= 0 && n >= 0 && k > 0, PTX_ERR_BAD_ARG, "fp8_matmul: m=%lld n=%lld k=%lld", (long long)m, (long long)n, (long long)k);
+  // (a launch has fewer than 2^32 threads, 512 per tile at most, and a tile's rows are addressed in 32 bits)
+  PTX_REQUIRE(m < 0x7fffff00 && n < 0x7fffff00 && k < 1 << 22 && (double)(m / 64 + 1) * (double)(n / 64 + 1) < 8388608.0,
+              PTX_ERR_UNSUPPORTED, "fp8_matmul: m=%lld n=%lld k=%lld is too large", (long long)m, (long long)n, (long long)k);
+  if (m == 0 || n == 0) return PTX_OK;
+  PTX_REQUIRE(a && a_scales && b && b_scales && out, PTX_ERR_BAD_ARG, "fp8_matmul: null pointer");
+  PTX_REQUIRE(aligned16(a) && aligned16(b) && aligned16(a_scales) && aligned16(b_scales), PTX_ERR_BAD_ARG,
+              "fp8_matmul: values and scales must be 16-byte aligned");
+  PTX_REQUIRE(workspace || ptx_fp8_matmul_workspace_elems(m, n, k, b_square) == 0, PTX_ERR_BAD_ARG, "fp8_matmul: needs the workspace");
+  PTX_DISPATCH_LN(out_dtype, ptx::fp8_matmul<T>(a, a_scales, b, b_scales, b_square != 0, bias, bias_dtype, (T*)out, workspace, (int)m, (int)n,
+                                                (int)ptx::fp8_blocks(k), (hipStream_t)stream));
+  return after_launch("fp8_matmul");
+}
+
+static int rmsnorm_args(const char* what, int64_t rows, int cols, int x_dtype, int stream_dtype, int param_dtype) {
+  PTX_REQUIRE(dtype_ok_ln(x_dtype) && dtype_ok_ln(stream_dtype) && dtype_ok_ln(param_dtype), PTX_ERR_BAD_ARG,
+              "%s: unknown dtype among %d, %d, %d", what, x_dtype, stream_dtype, param_dtype);
+  PTX_REQUIRE(x_dtype == stream_dtype || stream_dtype == PTX_F32, PTX_ERR_UNSUPPORTED, "%s: the stream has x's type or is fp32", what);
+  PTX_REQUIRE(rows >= 0 && cols > 0, PTX_ERR_BAD_ARG, "%s: rows=%lld cols=%d", what, (long long)rows, cols);
+  PTX_REQUIRE(rows < ((int64_t)1 << 31) && cols <= ptx::rmsnorm_max_cols(), PTX_ERR_UNSUPPORTED, "%s: %lld rows of %d columns (%d at most)",
+              what, (long long)rows, cols, ptx::rmsnorm_max_cols());
+  return PTX_OK;
+}
+
+PTX_API int ptx_add_rms_norm_fwd(const void* x, const void* residual, const void* gamma, void* y, float* y_scales, void* h, float* rstd,
+                                 int64_t rows, int cols, float eps, int x_dtype, int stream_dtype, int param_dtype, void* stream) {
+  const int rc = rmsnorm_args("add_rms_norm", rows, cols, x_dtype, stream_dtype, param_dtype);
+  if (rc != PTX_OK) return rc;
+  if (rows == 0) return PTX_OK;
+  PTX_REQUIRE(residual || x_dtype == stream_dtype, PTX_ERR_BAD_ARG, "add_rms_norm: without a residual the stream has x's type");
+  PTX_REQUIRE(x && y && (h || !residual), PTX_ERR_BAD_ARG, "add_rms_norm: null x, y or h");
+  PTX_REQUIRE(!y_scales || aligned16(y), PTX_ERR_BAD_ARG, "add_rms_norm: 8-bit values must be 16-byte aligned");
+  PTX_DISPATCH_STREAM(x_dtype, stream_dtype,
+                      (ptx::rmsnorm_fwd<TX, TR>)((const TX*)x, (const TR*)residual, gamma, param_dtype, y, y_scales, (TR*)h, rstd, rows, cols,
+                                                 eps, (hipStream_t)stream));
+  return after_launch("add_rms_norm");
+}
+
+PTX_API int64_t ptx_add_rms_norm_bwd_workspace_elems(int64_t rows, int cols) { return ptx::rmsnorm_bwd_workspace_elems(rows, cols); }
+
+PTX_API int ptx_add_rms_norm_bwd(const void* dy, const void* dh, const void* x, const void* residual, const void* h, const float* rstd,
+                                 const void* gamma, void* dx, void* dresidual, void* dgamma, float* workspace, int64_t rows, int cols,
+                                 int x_dtype, int stream_dtype, int param_dtype, void* stream) {
+  const int rc = rmsnorm_args("add_rms_norm_bwd", rows, cols, x_dtype, stream_dtype, param_dtype);
+  if (rc != PTX_OK) return rc;
+  PTX_REQUIRE(rows == 0 || !dgamma || workspace, PTX_ERR_BAD_ARG, "add_rms_norm_bwd: dgamma needs the workspace");
+  if (rows == 0 && !dgamma) return PTX_OK;
+  PTX_REQUIRE(rows == 0 || ((stream_dtype == PTX_F32 ? h : x) && rstd), PTX_ERR_BAD_ARG,
+              "add_rms_norm_bwd: null pointer (an fp32 stream needs h, a 16-bit one x)");
+  PTX_DISPATCH_STREAM(x_dtype, stream_dtype,
+                      (ptx::rmsnorm_bwd<TX, TR>)((const TX*)dy, (const TR*)dh, (const TX*)x, (const TR*)residual, (const TR*)h, rstd, gamma,
+                                                 param_dtype, (TX*)dx, (TR*)dresidual, dgamma, workspace, rows, cols, (hipStream_t)stream));
+  return after_launch("add_rms_norm_bwd");
 }
 
 }  // extern "C"

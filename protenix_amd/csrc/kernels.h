@@ -250,6 +250,26 @@ int dropnorm_bwd(const TX* dy, const TR* dh, const TX* x, const TR* res, const T
                  int cols, const Dropout& drop, hipStream_t stream);
 // Column sums of fp32 partial rows, [2][parts][cols] -> a, b of param_type (either may be null): layernorm_bwd's second launch.
 void column_sums(const float* part, int parts, int cols, int param_type, void* a, void* b, hipStream_t stream);
+// y = RMSNorm(h) of h = res + x (res null: of x, and no h), and the gradients (see rmsnorm.hip).  scales null: y [rows][cols] of type TX;
+// else 8-bit values and their scales as fp8.h lays them out.  Rows of up to rmsnorm_max_cols() columns.
+int rmsnorm_max_cols();
+template <typename TX, typename TR>
+int rmsnorm_fwd(const TX* x, const TR* res, const void* gamma, int param_type, void* y, float* scales, TR* h, float* rstd,
+                int64_t rows, int cols, float eps, hipStream_t stream);
+int64_t rmsnorm_bwd_workspace_elems(int64_t rows, int cols);
+template <typename TX, typename TR>
+int rmsnorm_bwd(const TX* dy, const TR* dh, const TX* x, const TR* res, const TR* h, const float* rstd, const void* gamma,
+                int param_type, TX* dx, TR* dres, void* dgamma, float* workspace, int64_t rows, int cols, hipStream_t stream);
+// x [rows][cols] into 8-bit blocks along its rows (q, scales) and / or along its columns (qt, scales_t: the transposed matrix); square: a
+// scale per 128 x 128.  part: null, or column sums of x per 128 rows, [tiles of rows][cols].
+template <typename T>
+int fp8_quantize(const T* x, void* q, float* scales, void* qt, float* scales_t, float* part, int64_t rows, int cols, bool square,
+                 hipStream_t stream);
+// out [m][n] = a b^T (+ bias) of such operands of `blocks` blocks; square: b's scales.  workspace: fp8_matmul_workspace_elems() floats.
+int64_t fp8_matmul_workspace_elems(int64_t m, int64_t n, int64_t blocks, bool square);
+template <typename O>
+int fp8_matmul(const void* a, const float* sa, const void* b, const float* sb, bool square, const void* bias, int bias_type, O* out,
+               float* workspace, int m, int n, int blocks, hipStream_t stream);
 // Learned bias by buckets of relative position, and its table's gradient (see relbias.hip).
 template <typename T>
 int relative_bias_fwd(const ptx_relative_buckets& bk, const void* table, int table_type, T* out, int batch, int heads, int q_len,

@@ -1,0 +1,198 @@
+"""Linear layers in 8 bits: matrices as e4m3 values with a scale per block of 128, their product, and `linear_fp8` with its gradients.
+
+Where `Linear` multiplies in bf16 or fp32, these multiply at the 8-bit rate of the matrix cores.  A block is 128 values along the axis
+that is summed over (activations, gradients), or 128 x 128 (`square`: weights, whose transpose then has the same numbers); its scale
+is its largest magnitude over 448, and a product's sums are fp32.  The scheme is written down in include/protenix_amd.h.
+"""
+from __future__ import annotations
+
+import math
+from typing import Optional, Tuple, Union
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import ops
+from .dropout import _refuse_foreign_accumulators, _refuse_tangents, _wants_grad
+
+BLOCK = 128
+
+
+class Fp8Tensor:
+    """A matrix [*, k] in 8-bit blocks along its last dimension, as `quantize_fp8`, `add_rms_norm(quantize=True)` and this class make it.
+
+    values: float8_e4m3fn [*, k]; scales: float32 [*, ceil(k / 128)], or with square=True [ceil(n / 128), ceil(k / 128)] for values
+    [n, k].  `values` and `scales` are views of the operand's own memory, whose layout is the kernels'; what is given here is copied
+    into that layout (weights of a checkpoint, say)."""
+
+    def __init__(self, values: torch.Tensor, scales: torch.Tensor, *, square: bool = False) -> None:
+        ops._dev(values, "values")
+        if values.dtype != torch.float8_e4m3fn or scales.dtype != torch.float32 or scales.device != values.device:
+            raise RuntimeError(f"values are float8_e4m3fn and scales float32 on their device, got {values.dtype} and {scales.dtype} on "
+                               f"{values.device} and {scales.device}")
+        if values.dim() < 1 or values.shape[-1] == 0 or (square and values.dim() != 2):
+            raise RuntimeError(f"values are [*, k] with k > 0, [n, k] with square scales, got {tuple(values.shape)}")
+        *lead, k = values.shape
+        want = (-(-lead[0] // BLOCK), -(-k // BLOCK)) if square else (*lead, -(-k // BLOCK))
+        if tuple(scales.shape) != want:
+            raise RuntimeError(f"values {tuple(values.shape)} have scales {want}{' (square)' if square else ''}, got {tuple(scales.shape)}")
+        rows = math.prod(lead)
+        with torch.cuda.device(values.device):
+            operand = ops.fp8_buffers(rows, k, bool(square), values.device)
+            data = operand[0].view(torch.uint8)
+            data[:, :k] = values.reshape(rows, k).view(torch.uint8)
+            data[:, k:] = 0
+            if square:
+                operand[1].copy_(scales)
+            else:
+                operand[1][:, :rows] = scales.reshape(rows, -1).t()
+        self._operand, self.shape = operand, torch.Size(values.shape)
+
+    @classmethod
+    def _of(cls, operand: tuple, shape) -> "Fp8Tensor":
+        t = cls.__new__(cls)
+        t._operand, t.shape = operand, torch.Size(shape)
+        return t
+
+    @property
+    def values(self) -> torch.Tensor:
+        return self._operand[0][:, :self.shape[-1]].view(self.shape)
+
+    @property
+    def scales(self) -> torch.Tensor:
+        _, scales, rows, _, square = self._operand
+        return scales if square else scales.t()[:rows].view(*self.shape[:-1], scales.shape[0])
+
+    @property
+    def square(self) -> bool:
+        return self._operand[4]
+
+    @property
+    def device(self) -> torch.device:
+        return self._operand[0].device
+
+    def __repr__(self) -> str:
+        return f"Fp8Tensor({tuple(self.shape)}, {'a scale per 128 x 128' if self.square else 'a scale per 128'}, {self.device})"
+
+
+Operand = Union[torch.Tensor, Fp8Tensor]
+
+
+def _matrix(x: torch.Tensor, name: str) -> torch.Tensor:
+    ops._dev(x, name)
+    ops._dt_ln(x)
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise RuntimeError(f"{name} is [*, k] with k > 0, got {tuple(x.shape)}")
+    return x.reshape(math.prod(x.shape[:-1]), x.shape[-1])
+
+
+def quantize_fp8(x: torch.Tensor, *, square: bool = False, along: Union[int, Tuple[int, int]] = -1):
+    """x [*, k], float32, bfloat16 or float16, in 8-bit blocks (no gradient: a rounding has none; `linear_fp8` has its own).
+
+    along=-1: blocks of the last dimension; the result has x's shape.  along=-2: the rows (all other dimensions as one) are the axis
+    that will be summed over: the transposed matrix [k, rows], blocks along its rows.  along=(-1, -2): both, from one pass over x.
+    square: a scale per 128 x 128, for x [n, k]: a weight, laid out once for serving."""
+    matrix = _matrix(x, "x")
+    if along not in (-1, -2, (-1, -2)):
+        raise RuntimeError(f"along={along}: -1, -2 or (-1, -2)")
+    if square and x.dim() != 2:
+        raise RuntimeError(f"square blocks are of a matrix [n, k], got {tuple(x.shape)}")
+    if along != -1 and matrix.shape[0] == 0:
+        raise RuntimeError("along=-2: no rows to sum over")
+    q, qt, _ = ops.fp8_quantize(matrix.detach(), bool(square), along != -2, along != -1)
+    got = [Fp8Tensor._of(q, x.shape) if q else None, Fp8Tensor._of(qt, (matrix.shape[1], matrix.shape[0])) if qt else None]
+    return tuple(got) if along == (-1, -2) else got[along == -2]
+
+
+def _check_bias(bias: Optional[torch.Tensor], n: int, device: torch.device) -> None:
+    if bias is None:
+        return
+    ops._dt_ln(bias)
+    if bias.shape != (n,) or bias.device != device:
+        raise RuntimeError(f"the bias is [{n}] on {device}, got {tuple(bias.shape)} on {bias.device}")
+
+
+def _out_type(dtype: torch.dtype) -> torch.dtype:
+    if dtype not in ops._LN_DTYPES:
+        raise RuntimeError(f"a product is float32, bfloat16 or float16, got {dtype}")
+    return dtype
+
+
+def matmul_fp8(a: Fp8Tensor, b: Fp8Tensor, bias: Optional[torch.Tensor] = None, *, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """a b^T + bias, [*, n] of type dtype, for a [*, k] and b [n, k]; sums in fp32, rounded once.
+
+    a has a scale per 128 values; b the same, or square ones (a weight).  bias: [n], float32, bfloat16 or float16."""
+    if not isinstance(a, Fp8Tensor) or not isinstance(b, Fp8Tensor):
+        raise RuntimeError(f"matmul_fp8 takes two Fp8Tensors, got {type(a).__name__} and {type(b).__name__}")
+    if len(b.shape) != 2 or a.shape[-1] != b.shape[1] or a.device != b.device:
+        raise RuntimeError(f"a [*, k] and b [n, k] on one device, got {tuple(a.shape)} and {tuple(b.shape)} on {a.device} and {b.device}")
+    if a.square:
+        raise RuntimeError("a has a scale per 128 values of a row (square scales are b's)")
+    _check_bias(bias, b.shape[0], b.device)
+    _refuse_wanted(bias)
+    bias = None if bias is None else bias.contiguous()
+    out = ops.fp8_matmul(a._operand, b._operand, bias, _out_type(dtype))
+    return out.view(*a.shape[:-1], b.shape[0])
+
+
+def _refuse_wanted(*tensors: Optional[torch.Tensor]) -> None:
+    if _wants_grad(*tensors):
+        raise RuntimeError("operands in 8 bits have no gradients: give linear_fp8 the tensors themselves, or call under torch.no_grad()")
+
+
+class _LinearFp8(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, dtype):
+        need = ctx.needs_input_grad
+        matrix = x.reshape(-1, x.shape[-1])
+        xq, xt, _ = ops.fp8_quantize(matrix, False, True, need[1])
+        wq, wt, _ = ops.fp8_quantize(weight, True, True, need[0])
+        ctx.x_shape, ctx.types = x.shape, (x.dtype, weight.dtype, None if bias is None else bias.dtype)
+        # what the gradients take, in 8 bits: neither x nor the weight is kept
+        ctx.saved = [None if t is None else t[2:] for t in (xt, wt)]
+        ctx.save_for_backward(*(u for t in (xt, wt) for u in (t[:2] if t else (None, None))))
+        return ops.fp8_matmul(xq, wq, None if bias is None else bias.contiguous(), dtype).view(*x.shape[:-1], weight.shape[0])
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        t = ctx.saved_tensors
+        xt, wt = (None if s is None else (t[2 * i], t[2 * i + 1], *s) for i, s in enumerate(ctx.saved))
+        need = ctx.needs_input_grad
+        q, qt, db = ops.fp8_quantize(dy.reshape(math.prod(ctx.x_shape[:-1]), dy.shape[-1]), False, need[0], need[1], ctx.types[2] if need[2] else None)
+        dx = ops.fp8_matmul(q, wt, None, ctx.types[0]).view(ctx.x_shape) if need[0] else None
+        dw = ops.fp8_matmul(qt, xt, None, ctx.types[1]) if need[1] else None
+        return dx, dw, db, None
+
+
+def linear_fp8(x: Operand, weight: Operand, bias: Optional[torch.Tensor] = None, *, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """x W^T + bias with both in 8-bit blocks: [*, n] for x [*, k], weight [n, k], bias [n]; differentiable (backward, once;
+    forward-mode is refused).
+
+    x, weight: float32, bfloat16 or float16 tensors, each of its own type, or `Fp8Tensor`s (in use without gradients: a weight laid out
+    once by `quantize_fp8(weight, square=True)`, what `add_rms_norm(quantize=True)` left of x).  dtype: of the result (x's by
+    default, bfloat16 for x in 8 bits).
+    Training: x and dy in blocks of 128 along the axis each product sums over, the weight in blocks of 128 x 128; dx = dy W and
+    dW = dy^T x are products of such operands too, with the rounding to 8 bits taken as the identity, and db is summed in fp32,
+    in a fixed order.  Gradients have their inputs' types.  Neither x nor the weight is kept, only their 8-bit forms."""
+    if not isinstance(weight, Fp8Tensor):
+        _matrix(weight, "weight")
+    if weight.shape.__len__() != 2:
+        raise RuntimeError(f"the weight is [n, k], got {tuple(weight.shape)}")
+    n, k = weight.shape
+    if not isinstance(x, Fp8Tensor):
+        _matrix(x, "x")
+    if x.shape[-1] != k or x.device != weight.device:
+        raise RuntimeError(f"x [*, k] and weight [n, k] on one device, got {tuple(x.shape)} and {tuple(weight.shape)} on {x.device} and {weight.device}")
+    _check_bias(bias, n, weight.device)
+    dtype = _out_type(dtype or (torch.bfloat16 if isinstance(x, Fp8Tensor) else x.dtype))
+    plain = [t for t in (x, weight, bias) if isinstance(t, torch.Tensor)]
+    _refuse_tangents(*plain)
+    if isinstance(x, torch.Tensor) and isinstance(weight, torch.Tensor) and _wants_grad(*plain):
+        _refuse_foreign_accumulators(*plain)
+        return _LinearFp8.apply(x, weight, bias, dtype)
+    if isinstance(x, Fp8Tensor) or isinstance(weight, Fp8Tensor):
+        _refuse_wanted(*plain)
+    a = x if isinstance(x, Fp8Tensor) else quantize_fp8(x)
+    b = weight if isinstance(weight, Fp8Tensor) else quantize_fp8(weight, square=True)
+    return matmul_fp8(a, b, None if bias is None else bias.detach(), dtype=dtype)

@@ -805,3 +805,87 @@ def relative_bias_backward(buckets, dout: torch.Tensor, table_shape, table_dtype
         _call("relative_bias_bwd", lib.ptx_relative_bias_bwd, ctypes.addressof(buckets), _ptr(dout), _ptr(dtable), _ptr(ws), *size,
               _ptr(q[0]), _ptr(k[0]), q[1], k[1], _ptr(groups[0]), _ptr(groups[1]), _dt_ln(dtable), _dt_ln(dout), _stream())
     return dtable
+
+
+# ---- 8-bit blocks, their product, and the RMS norm in front of them --------------------------------------
+# (arguments as the modules fp8.py and rms_norm.py have checked them; an operand is (values [rows, pitch], scales as the C ABI lays
+# them out, rows, columns, whether a scale stands for 128 x 128))
+def fp8_buffers(rows: int, cols: int, square: bool, device) -> tuple:
+    """An operand with its memory as it comes."""
+    lib = _lib.load()
+    blocks = -(-cols // 128)
+    values = torch.empty((rows, blocks * 128), dtype=torch.float8_e4m3fn, device=device)
+    lead = -(-rows // 128) if square else lib.ptx_fp8_scale_pitch(rows)
+    scales = torch.empty((lead, blocks) if square else (blocks, lead), dtype=torch.float32, device=device)
+    return values, scales, rows, cols, square
+
+
+def fp8_quantize(x: torch.Tensor, square: bool, rows_too: bool, columns_too: bool, col_sums_dtype: Optional[torch.dtype] = None) -> tuple:
+    """(operand of the matrix x, operand of its transpose, sums over its rows), those asked for."""
+    lib = _lib.load()
+    x = x.contiguous()
+    rows, cols = x.shape
+    q = fp8_buffers(rows, cols, square, x.device) if rows_too else None
+    qt = fp8_buffers(cols, rows, square, x.device) if columns_too else None
+    sums = ws = None
+    if col_sums_dtype is not None:
+        sums = torch.empty((cols,), dtype=col_sums_dtype, device=x.device)
+        ws = _workspace((lib.ptx_fp8_col_sums_workspace_elems(rows, cols),), torch.float32, x.device)
+    with torch.cuda.device(x.device):
+        _call("fp8_quantize", lib.ptx_fp8_quantize, _ptr(x), *((_ptr(q[0]), _ptr(q[1])) if q else (None, None)),
+              *((_ptr(qt[0]), _ptr(qt[1])) if qt else (None, None)), _ptr(sums), _ptr(ws), rows, cols, int(square), _dt_ln(x),
+              _lib.PTX_F32 if sums is None else _dt_ln(sums), _stream())
+    return q, qt, sums
+
+
+def fp8_matmul(a: tuple, b: tuple, bias: Optional[torch.Tensor], dtype: torch.dtype) -> torch.Tensor:
+    """a b^T + bias, [rows of a, rows of b]."""
+    lib = _lib.load()
+    m, n, k = a[2], b[2], a[3]
+    if k == 0:
+        out = torch.zeros((m, n), dtype=dtype, device=a[0].device)
+        return out if bias is None else out + bias.to(dtype)
+    out = torch.empty((m, n), dtype=dtype, device=a[0].device)
+    elems = lib.ptx_fp8_matmul_workspace_elems(m, n, k, int(b[4]))
+    ws = _workspace((elems,), torch.float32, out.device) if elems else None
+    with torch.cuda.device(out.device):
+        _call("fp8_matmul", lib.ptx_fp8_matmul, _ptr(a[0]), _ptr(a[1]), _ptr(b[0]), _ptr(b[1]), int(b[4]), _ptr(bias), _ptr(out), _ptr(ws),
+              m, n, k, _dt_ln(out), _lib.PTX_F32 if bias is None else _dt_ln(bias), _stream())
+    return out
+
+
+def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: Optional[torch.Tensor], eps: float, quantize: bool,
+                 return_rstd: bool) -> tuple:
+    """(y or an operand, h or None without a residual, rstd [rows] or None) of contiguous x and residual."""
+    lib = _lib.load()
+    cols = x.shape[-1]
+    rows = x.numel() // cols
+    y = fp8_buffers(rows, cols, False, x.device) if quantize else torch.empty_like(x)
+    h = None if residual is None else torch.empty_like(residual)
+    rstd = torch.empty((rows,), dtype=torch.float32, device=x.device) if return_rstd else None
+    with torch.cuda.device(x.device):
+        _call("add_rms_norm", lib.ptx_add_rms_norm_fwd, _ptr(x), _ptr(residual), _ptr(weight), _ptr(y[0] if quantize else y),
+              _ptr(y[1]) if quantize else None, _ptr(h), _ptr(rstd), rows, cols, eps, _dt_ln(x), _dt_ln(x if h is None else h),
+              _lib.PTX_F32 if weight is None else _dt_ln(weight), _stream())
+    return y, h, rstd
+
+
+def add_rms_norm_backward(dy, dh, x, residual, h, rstd, weight, x_dtype, need: tuple):
+    """Gradients (x, residual, weight), those of `need`; x and residual given (16-bit streams) or h (fp32 ones)."""
+    lib = _lib.load()
+    like = x if x is not None else h
+    cols = like.shape[-1]
+    rows = like.numel() // cols
+    empty = lambda dtype: torch.empty(like.shape, dtype=dtype, device=like.device)
+    one = x_dtype == like.dtype and need[0] and need[1]      # (the two gradients are the same values)
+    dres = empty(like.dtype) if need[1] else None
+    dx = empty(x_dtype) if need[0] and not one else None
+    dw = torch.empty_like(weight) if need[2] else None
+    ws = None
+    if dw is not None:
+        ws = _workspace((lib.ptx_add_rms_norm_bwd_workspace_elems(max(rows, 1), cols),), torch.float32, like.device)
+    with torch.cuda.device(like.device):
+        _call("add_rms_norm_bwd", lib.ptx_add_rms_norm_bwd, _ptr(dy), _ptr(dh), _ptr(x), _ptr(residual), _ptr(h), _ptr(rstd), _ptr(weight),
+              _ptr(dx), _ptr(dres), _ptr(dw), _ptr(ws), rows, cols, _LN_DTYPES[x_dtype], _dt_ln(like),
+              _lib.PTX_F32 if weight is None else _dt_ln(weight), _stream())
+    return (dres if one else dx), dres, dw
