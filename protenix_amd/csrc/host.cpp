@@ -1471,6 +1471,253 @@ optional<Tensor> relative_bias(const Tensor& table, uintptr_t buckets, const py:
   return relative_bias_call(table, given(q.t), given(k.t), given(gq.t), given(gk.t), c, type);
 }
 
+// ---- 8-bit blocks, their product, and the RMS norm in front of them -----------------------------------------
+// Calls with arguments as fp8.py and rms_norm.py document them, with something in every tensor; anything else is handed back (None).
+struct Fp8Operand {
+  Tensor values, scales;
+  int64_t rows = 0, cols = 0;
+  bool square = false;
+};
+typedef std::tuple<Tensor, Tensor, int64_t, int64_t, bool> OperandTuple;      // as Python has it
+OperandTuple tuple_of(const Fp8Operand& t) { return {t.values, t.scales, t.rows, t.cols, t.square}; }
+Fp8Operand operand_of(const OperandTuple& t) { return {std::get<0>(t), std::get<1>(t), std::get<2>(t), std::get<3>(t), std::get<4>(t)}; }
+
+Fp8Operand fp8_buffers(int64_t rows, int64_t cols, bool square, const at::TensorOptions& like) {
+  const int64_t blocks = (cols + 127) / 128, lead = square ? (rows + 127) / 128 : ptx_fp8_scale_pitch(rows);
+  return {at::empty({rows, blocks * 128}, like.dtype(at::kFloat8_e4m3fn)),
+          at::empty(square ? std::initializer_list<int64_t>{lead, blocks} : std::initializer_list<int64_t>{blocks, lead}, like.dtype(at::kFloat)),
+          rows, cols, square};
+}
+// x [.., cols], dense, as a matrix of `rows` rows
+void fp8_quantize_call(const Tensor& x, int64_t rows, bool square, Fp8Operand* q, Fp8Operand* qt, Tensor* sums, at::ScalarType sums_type) {
+  const int64_t cols = x.numel() / rows;
+  const auto like = at::TensorOptions().device(x.device());
+  Tensor ws;
+  if (q) *q = fp8_buffers(rows, cols, square, like);
+  if (qt) *qt = fp8_buffers(cols, rows, square, like);
+  if (sums) {
+    *sums = at::empty({cols}, like.dtype(sums_type));
+    ws = at::empty({ptx_fp8_col_sums_workspace_elems(rows, cols)}, like.dtype(at::kFloat));
+  }
+  check(ptx_fp8_quantize(ptr(x), q ? ptr(q->values) : nullptr, q ? (float*)ptr(q->scales) : nullptr, qt ? ptr(qt->values) : nullptr,
+                         qt ? (float*)ptr(qt->scales) : nullptr, sums ? ptr(*sums) : nullptr, (float*)ptr(ws), rows, cols, square,
+                         code_of(x.scalar_type()), sums ? code_of(sums_type) : PTX_F32, current_stream(x)), "fp8_quantize");
+}
+Tensor fp8_matmul_call(const Fp8Operand& a, const Fp8Operand& b, const Tensor& bias, at::ScalarType type, at::IntArrayRef shape) {
+  Tensor out = at::empty(shape, a.values.options().dtype(type)), ws;
+  const int64_t elems = ptx_fp8_matmul_workspace_elems(a.rows, b.rows, a.cols, b.square);
+  if (elems) ws = at::empty({elems}, out.options().dtype(at::kFloat));
+  check(ptx_fp8_matmul(ptr(a.values), (const float*)ptr(a.scales), ptr(b.values), (const float*)ptr(b.scales), b.square, ptr(bias), ptr(out),
+                       (float*)ptr(ws), a.rows, b.rows, a.cols, code_of(type), bias.defined() ? code_of(bias.scalar_type()) : PTX_F32,
+                       current_stream(out)), "fp8_matmul");
+  return out;
+}
+bool product_type(at::ScalarType t) { return t == at::kFloat || t == at::kBFloat16 || t == at::kHalf; }
+bool fits_bias(const optional<Tensor>& bias, int64_t n, const at::Device& device) {
+  return !bias || (float_type(*bias) && bias->dim() == 1 && bias->size(0) == n && bias->device() == device);
+}
+std::vector<int64_t> with_last(at::IntArrayRef shape, int64_t last) {
+  auto s = shape.vec();
+  s.back() = last;
+  return s;
+}
+
+optional<std::tuple<optional<OperandTuple>, optional<OperandTuple>>> quantize_fp8(const Tensor& x_, bool square, bool rows_too, bool columns_too) {
+  if (!x_.is_cuda() || !float_type(x_) || x_.dim() < 1 || x_.numel() == 0 || (square && x_.dim() != 2)) return c10::nullopt;
+  optional<OperandTuple> first, second;
+  {
+    py::gil_scoped_release nogil;
+    at::DeviceGuard dev(x_.device());
+    at::NoGradGuard no_grad;
+    const Tensor x = x_.contiguous();
+    Fp8Operand q, qt;
+    fp8_quantize_call(x, x.numel() / x.size(-1), square, rows_too ? &q : nullptr, columns_too ? &qt : nullptr, nullptr, at::kFloat);
+    if (rows_too) first = tuple_of(q);
+    if (columns_too) second = tuple_of(qt);
+  }
+  return std::make_tuple(first, second);
+}
+
+// a, b: operands; lead: the result's shape but for its last dimension.  x in a's place: quantized first.
+optional<Tensor> matmul_fp8(const OperandTuple& a_, const OperandTuple& b_, const optional<Tensor>& bias, at::ScalarType type,
+                            const std::vector<int64_t>& a_shape) {
+  const Fp8Operand a = operand_of(a_), b = operand_of(b_);
+  if (a.square || a.cols != b.cols || !a.rows || !b.rows || a.values.device() != b.values.device() || !product_type(type) ||
+      !fits_bias(bias, b.rows, b.values.device()) || (at::GradMode::is_enabled() && bias && wants(*bias)))
+    return c10::nullopt;
+  py::gil_scoped_release nogil;
+  at::DeviceGuard dev(a.values.device());
+  return fp8_matmul_call(a, b, dense(bias), type, with_last(a_shape, b.rows));
+}
+
+struct LinearFp8Fn : torch::autograd::Function<LinearFp8Fn> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x_, const Tensor& weight, const optional<Tensor>& bias,
+                        at::ScalarType type) {
+    const Tensor x = x_.contiguous(), w = weight.contiguous();
+    Fp8Operand xq, xt, wq, wt;
+    const bool need_x = x_.requires_grad(), need_w = weight.requires_grad();
+    fp8_quantize_call(x, x.numel() / x.size(-1), false, &xq, need_w ? &xt : nullptr, nullptr, at::kFloat);
+    fp8_quantize_call(w, w.size(0), true, &wq, need_x ? &wt : nullptr, nullptr, at::kFloat);
+    // what the gradients take, in 8 bits: neither x nor the weight is kept
+    ctx->save_for_backward({xt.values, xt.scales, wt.values, wt.scales});
+    ctx->saved_data["shape"] = x.sizes().vec();
+    ctx->saved_data["n"] = std::vector<int64_t>{w.size(0), (int64_t)x.scalar_type(), (int64_t)w.scalar_type(),
+                                                bias ? (int64_t)bias->scalar_type() : (int64_t)-1};
+    return fp8_matmul_call(xq, wq, dense(bias), type, with_last(x.sizes(), w.size(0)));
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    refuse_double_backward();
+    const auto t = ctx->get_saved_variables();
+    const auto shape = ctx->saved_data["shape"].toIntVector(), v = ctx->saved_data["n"].toIntVector();
+    const int64_t k = shape.back(), n = v[0];
+    const Tensor dy = grads[0].contiguous();
+    const int64_t m = dy.numel() / n;
+    at::DeviceGuard dev(dy.device());
+    const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1), need_b = v[3] >= 0 && ctx->needs_input_grad(2);
+    Fp8Operand q, qt;
+    Tensor dx, dw, db;
+    if (need_x || need_w || need_b)
+      fp8_quantize_call(dy, m, false, need_x ? &q : nullptr, need_w ? &qt : nullptr, need_b ? &db : nullptr, need_b ? (at::ScalarType)v[3] : at::kFloat);
+    if (need_x) dx = fp8_matmul_call(q, {t[2], t[3], k, n, true}, Tensor(), (at::ScalarType)v[1], shape);
+    if (need_w) dw = fp8_matmul_call(qt, {t[0], t[1], k, m, false}, Tensor(), (at::ScalarType)v[2], {n, k});
+    return {dx, dw, db, Tensor()};
+  }
+};
+
+optional<Tensor> linear_fp8(const Tensor& x_, const Tensor& weight, const optional<Tensor>& bias, const optional<at::ScalarType>& type_) {
+  if (!x_.is_cuda() || !float_type(x_) || !float_type(weight) || x_.dim() < 1 || weight.dim() != 2 || x_.numel() == 0 || weight.numel() == 0 ||
+      weight.device() != x_.device() || x_.size(-1) != weight.size(1) || !fits_bias(bias, weight.size(0), x_.device()))
+    return c10::nullopt;
+  const auto type = type_ ? *type_ : x_.scalar_type();
+  if (!product_type(type)) return c10::nullopt;
+  py::gil_scoped_release nogil;
+  at::DeviceGuard dev(x_.device());
+  const Tensor b = given(bias);
+  refuse_tangents({&x_, &weight, &b});
+  if (at::GradMode::is_enabled() && (wants(x_) || wants(weight) || wants(b))) {
+    refuse_foreign_accumulators(current_stream(x_), {&x_, &weight, &b});
+    return LinearFp8Fn::apply(x_, weight, bias, type);
+  }
+  at::NoGradGuard no_grad;
+  const Tensor x = x_.contiguous(), w = weight.contiguous();
+  Fp8Operand xq, wq;
+  fp8_quantize_call(x, x.numel() / x.size(-1), false, &xq, nullptr, nullptr, at::kFloat);
+  fp8_quantize_call(w, w.size(0), true, &wq, nullptr, nullptr, at::kFloat);
+  return fp8_matmul_call(xq, wq, dense(bias), type, with_last(x.sizes(), w.size(0)));
+}
+
+// The same with a weight laid out before.
+optional<Tensor> linear_fp8_ready(const Tensor& x_, const OperandTuple& w, const optional<Tensor>& bias, const optional<at::ScalarType>& type_) {
+  const Fp8Operand b = operand_of(w);
+  if (!x_.is_cuda() || !float_type(x_) || x_.dim() < 1 || x_.numel() == 0 || !b.rows || b.values.device() != x_.device() || x_.size(-1) != b.cols ||
+      !fits_bias(bias, b.rows, x_.device()) || (at::GradMode::is_enabled() && (wants(x_) || (bias && wants(*bias)))))
+    return c10::nullopt;
+  const auto type = type_ ? *type_ : x_.scalar_type();
+  if (!product_type(type)) return c10::nullopt;
+  py::gil_scoped_release nogil;
+  at::DeviceGuard dev(x_.device());
+  const Tensor bi = given(bias);
+  refuse_tangents({&x_, &bi});
+  at::NoGradGuard no_grad;
+  const Tensor x = x_.contiguous();
+  Fp8Operand xq;
+  fp8_quantize_call(x, x.numel() / x.size(-1), false, &xq, nullptr, nullptr, at::kFloat);
+  return fp8_matmul_call(xq, b, dense(bias), type, with_last(x.sizes(), b.rows));
+}
+
+// y (or into `quant`), h (undefined without a residual) and, for a backward pass, rstd [rows]
+std::tuple<Tensor, Tensor, Tensor> rms_norm_call(const Tensor& x, const Tensor& res, const Tensor& w, double eps, Fp8Operand* quant, bool want_rstd) {
+  const int64_t cols = x.size(-1), rows = x.numel() / cols;
+  Tensor y, h, rstd;
+  if (quant) *quant = fp8_buffers(rows, cols, false, at::TensorOptions().device(x.device()));
+  else y = at::empty_like(x);
+  if (res.defined()) h = at::empty_like(res);
+  if (want_rstd) rstd = at::empty({rows}, x.options().dtype(at::kFloat));
+  check(ptx_add_rms_norm_fwd(ptr(x), ptr(res), ptr(w), quant ? ptr(quant->values) : ptr(y), quant ? (float*)ptr(quant->scales) : nullptr, ptr(h),
+                             (float*)ptr(rstd), rows, (int)cols, (float)eps, code_of(x.scalar_type()),
+                             code_of((res.defined() ? res : x).scalar_type()), w.defined() ? code_of(w.scalar_type()) : PTX_F32,
+                             current_stream(x)), "add_rms_norm");
+  return {y, h, rstd};
+}
+
+struct AddRmsNormFn : torch::autograd::Function<AddRmsNormFn> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& x_, const optional<Tensor>& residual,
+                                                const optional<Tensor>& weight, double eps) {
+    ctx->set_materialize_grads(false);
+    const Tensor x = x_.contiguous(), res = dense(residual), w = dense(weight);
+    auto [y, h, rstd] = rms_norm_call(x, res, w, eps, nullptr, true);
+    // the sum itself where the stream is fp32 (x without a residual); else what it is formed from (see ptx_add_rms_norm_bwd)
+    const Tensor& stream = h.defined() ? h : x;
+    const bool wide = stream.scalar_type() == at::kFloat;
+    ctx->save_for_backward({wide ? Tensor() : x, wide ? Tensor() : res, wide ? stream : Tensor(), rstd, w});
+    ctx->saved_data["given"] = std::vector<int64_t>{(int64_t)x.scalar_type(), res.defined(), w.defined()};
+    // (without a residual x comes back as a second result, so that its gradient is added before the rounding)
+    return {y, h.defined() ? h : x_};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    refuse_double_backward();
+    torch::autograd::variable_list out(4);
+    if (!grads[0].defined() && !grads[1].defined()) return out;
+    const auto t = ctx->get_saved_variables();
+    const Tensor &x = t[0], &res = t[1], &h = t[2], &rstd = t[3], &w = t[4];
+    const auto v = ctx->saved_data["given"].toIntVector();
+    const auto x_type = (at::ScalarType)v[0];
+    const Tensor& like = h.defined() ? h : x;
+    const int64_t cols = like.size(-1), rows = like.numel() / cols;
+    at::DeviceGuard dev(like.device());
+    const Tensor dy = dense(grads[0]), dh = dense(grads[1]);
+    int next = 0;   // (needs_input_grad counts the tensors that were given)
+    auto needs = [&](bool was_given) { return was_given && ctx->needs_input_grad(next++); };
+    const bool need_x = needs(true), need_res = needs(v[1]), need_w = needs(v[2]);
+    const bool one = x_type == like.scalar_type() && need_x && need_res;   // (the two gradients are the same values)
+    Tensor dx, dres, dw, ws;
+    if (need_res) dres = at::empty_like(like);
+    if (need_x && !one) dx = at::empty(like.sizes(), like.options().dtype(x_type));
+    if (need_w) {
+      dw = at::empty_like(w);
+      ws = at::empty({ptx_add_rms_norm_bwd_workspace_elems(std::max<int64_t>(rows, 1), (int)cols)}, like.options().dtype(at::kFloat));
+    }
+    check(ptx_add_rms_norm_bwd(ptr(dy), ptr(dh), ptr(x), ptr(res), ptr(h), (const float*)ptr(rstd), ptr(w), ptr(dx), ptr(dres), ptr(dw),
+                               (float*)ptr(ws), rows, (int)cols, code_of(x_type), code_of(like.scalar_type()),
+                               w.defined() ? code_of(w.scalar_type()) : PTX_F32, current_stream(like)), "add_rms_norm_bwd");
+    out[0] = one ? dres : dx;
+    out[1] = dres;
+    out[2] = dw;
+    return out;
+  }
+};
+
+// (y, h), or (an operand, h) with quantize
+py::object add_rms_norm(const Tensor& x, const optional<Tensor>& residual, const optional<Tensor>& weight, double eps, bool quantize) {
+  if (!x.is_cuda() || !float_type(x) || x.dim() < 1 || x.numel() == 0) return py::none();
+  if (residual && (residual->device() != x.device() || residual->sizes() != x.sizes() ||
+                   (residual->scalar_type() != x.scalar_type() && residual->scalar_type() != at::kFloat)))
+    return py::none();
+  if (weight && (!float_type(*weight) || weight->dim() != 1 || weight->size(0) != x.size(-1) || weight->device() != x.device())) return py::none();
+  const Tensor res = given(residual), w = given(weight);
+  const bool grad = at::GradMode::is_enabled() && (wants(x) || wants(res) || wants(w));
+  if (grad && quantize) return py::none();
+  Tensor y, h, rstd;
+  Fp8Operand q;
+  {
+    py::gil_scoped_release nogil;
+    at::DeviceGuard dev(x.device());
+    refuse_tangents({&x, &res, &w});
+    if (grad) {
+      refuse_foreign_accumulators(current_stream(x), {&x, &res, &w});
+      const auto out = AddRmsNormFn::apply(x, residual, weight, eps);
+      y = out[0];
+      h = out[1];
+    } else {
+      at::NoGradGuard no_grad;
+      std::tie(y, h, rstd) = rms_norm_call(x.contiguous(), dense(residual), dense(weight), eps, quantize ? &q : nullptr, false);
+      if (!h.defined()) h = x;
+    }
+  }
+  if (quantize) return py::cast(std::make_tuple(tuple_of(q), h));
+  return py::cast(std::make_tuple(y, h));
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_host, m) {
@@ -1505,6 +1752,11 @@ PYBIND11_MODULE(_host, m) {
   m.def("dropout_add", &dropout_add);
   m.def("dropout_add_layer_norm", &dropout_add_layer_norm);
   m.def("relative_bias", &relative_bias);
+  m.def("quantize_fp8", &quantize_fp8);
+  m.def("matmul_fp8", &matmul_fp8);
+  m.def("linear_fp8", &linear_fp8);
+  m.def("linear_fp8_ready", &linear_fp8_ready);
+  m.def("add_rms_norm", &add_rms_norm);
   m.def("refuse_tangents", [](const std::vector<Tensor>& inputs) {
     for (const Tensor& t : inputs) refuse_tangents({&t});
   }, "raises where one of the tensors carries a forward-mode tangent");

@@ -12,7 +12,7 @@ from typing import Optional, Tuple, Union
 import torch
 from torch.autograd.function import once_differentiable
 
-from . import ops
+from . import native, ops
 from .dropout import _refuse_foreign_accumulators, _refuse_tangents, _wants_grad
 
 BLOCK = 128
@@ -51,12 +51,13 @@ class Fp8Tensor:
     @classmethod
     def _of(cls, operand: tuple, shape) -> "Fp8Tensor":
         t = cls.__new__(cls)
-        t._operand, t.shape = operand, torch.Size(shape)
+        t._operand, t.shape = operand, shape if type(shape) is torch.Size else torch.Size(shape)
         return t
 
     @property
     def values(self) -> torch.Tensor:
-        return self._operand[0][:, :self.shape[-1]].view(self.shape)
+        data, k = self._operand[0], self.shape[-1]
+        return (data if data.shape[1] == k else data[:, :k]).view(self.shape)
 
     @property
     def scales(self) -> torch.Tensor:
@@ -92,6 +93,15 @@ def quantize_fp8(x: torch.Tensor, *, square: bool = False, along: Union[int, Tup
     along=-1: blocks of the last dimension; the result has x's shape.  along=-2: the rows (all other dimensions as one) are the axis
     that will be summed over: the transposed matrix [k, rows], blocks along its rows.  along=(-1, -2): both, from one pass over x.
     square: a scale per 128 x 128, for x [n, k]: a weight, laid out once for serving."""
+    if ops.use_native_operators():
+        both = along == (-1, -2)
+        if both or along == -1 or along == -2:
+            out = native.host().quantize_fp8(x, square, along != -2, along != -1)
+            if out is not None:
+                q, qt = out
+                first = None if q is None else Fp8Tensor._of(q, x.shape)
+                second = None if qt is None else Fp8Tensor._of(qt, (qt[2], qt[3]))
+                return (first, second) if both else second if first is None else first
     matrix = _matrix(x, "x")
     if along not in (-1, -2, (-1, -2)):
         raise RuntimeError(f"along={along}: -1, -2 or (-1, -2)")
@@ -122,6 +132,10 @@ def matmul_fp8(a: Fp8Tensor, b: Fp8Tensor, bias: Optional[torch.Tensor] = None, 
     """a b^T + bias, [*, n] of type dtype, for a [*, k] and b [n, k]; sums in fp32, rounded once.
 
     a has a scale per 128 values; b the same, or square ones (a weight).  bias: [n], float32, bfloat16 or float16."""
+    if ops.use_native_operators() and isinstance(a, Fp8Tensor) and isinstance(b, Fp8Tensor) and len(b.shape) == 2:
+        out = native.host().matmul_fp8(a._operand, b._operand, bias, dtype, a.shape)
+        if out is not None:
+            return out
     if not isinstance(a, Fp8Tensor) or not isinstance(b, Fp8Tensor):
         raise RuntimeError(f"matmul_fp8 takes two Fp8Tensors, got {type(a).__name__} and {type(b).__name__}")
     if len(b.shape) != 2 or a.shape[-1] != b.shape[1] or a.device != b.device:
@@ -175,9 +189,17 @@ def linear_fp8(x: Operand, weight: Operand, bias: Optional[torch.Tensor] = None,
     Training: x and dy in blocks of 128 along the axis each product sums over, the weight in blocks of 128 x 128; dx = dy W and
     dW = dy^T x are products of such operands too, with the rounding to 8 bits taken as the identity, and db is summed in fp32,
     in a fixed order.  Gradients have their inputs' types.  Neither x nor the weight is kept, only their 8-bit forms."""
+    if ops.use_native_operators() and isinstance(x, torch.Tensor):
+        out = None
+        if isinstance(weight, torch.Tensor):
+            out = native.host().linear_fp8(x, weight, bias, dtype)
+        elif len(weight.shape) == 2:
+            out = native.host().linear_fp8_ready(x, weight._operand, bias, dtype)
+        if out is not None:
+            return out
     if not isinstance(weight, Fp8Tensor):
         _matrix(weight, "weight")
-    if weight.shape.__len__() != 2:
+    if len(weight.shape) != 2:
         raise RuntimeError(f"the weight is [n, k], got {tuple(weight.shape)}")
     n, k = weight.shape
     if not isinstance(x, Fp8Tensor):

@@ -6,7 +6,7 @@ from typing import Optional, Tuple, Union
 import torch
 from torch.autograd.function import once_differentiable
 
-from . import ops
+from . import native, ops
 from .dropout import _refuse_foreign_accumulators, _refuse_tangents, _wants_grad
 from .fp8 import Fp8Tensor
 
@@ -46,6 +46,10 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor] = None, weigh
     types, or None; its gradient is summed in fp32, in a fixed order.
     quantize: y as an `Fp8Tensor`, blocks along the last dimension, straight from the fp32 values, for `matmul_fp8` and `linear_fp8`
     in use (no gradients)."""
+    if ops.use_native_operators():
+        out = native.host().add_rms_norm(x, residual, weight, eps, quantize)
+        if out is not None:
+            return (Fp8Tensor._of(out[0], x.shape), out[1]) if quantize else out
     ops._dev(x, "x")
     ops._dt_ln(x)
     if x.dim() < 1 or x.shape[-1] == 0:

@@ -259,6 +259,26 @@ def test_workspaces_hold_nothing(monkeypatch):
     assert all(torch.equal(a, c) for a, c in zip(first, torch.autograd.grad(P.linear_fp8(x, w, b), (x, w, b), dy)))
 
 
+def test_python_and_native_paths_give_the_same_bits(monkeypatch):
+    for types in ((BF16, F32, F32), (F32, F32, None), (F16, F16, F16)):
+        x, w, b, dy = _train(90, 200, 60, *types, lead=(3, 5, 6))
+
+        def every():
+            y = P.linear_fp8(x, w, b)
+            wq = P.quantize_fp8(w, square=True)
+            pair = P.quantize_fp8(x, along=(-1, -2))
+            with torch.no_grad():
+                served = P.linear_fp8(x, wq, b, dtype=F16), P.matmul_fp8(pair[0], wq, b), P.linear_fp8(x, w)
+            return (y, *torch.autograd.grad(y, [t for t in (x, w, b) if t is not None], dy), *served,
+                    *(u for t in (wq, *pair) for u in (t.values.view(torch.uint8), t.scales)))
+
+        first = every()
+        with monkeypatch.context() as m:
+            m.setattr(ops, "native_enabled", False)
+            second = every()
+        assert len(first) == len(second) and all(a.shape == c.shape and a.dtype == c.dtype and torch.equal(a, c) for a, c in zip(first, second))
+
+
 def test_rows_behind_the_last_are_left_alone():
     """Nothing outside the results is written."""
     lib, dev = ops._lib.load(), "cuda"
@@ -387,6 +407,5 @@ def test_refusals():
         with pytest.raises(RuntimeError):
             bad()
     y = P.linear_fp8(grad, w)
-    g = torch.autograd.grad(y, grad, torch.ones_like(y), create_graph=True)[0]
-    with pytest.raises(RuntimeError):
-        g.sum().backward()
+    with pytest.raises(RuntimeError, match="differentiable"):
+        torch.autograd.grad(y, grad, torch.ones_like(y), create_graph=True)[0].sum().backward()

@@ -249,6 +249,24 @@ def test_workspaces_graphs_and_streams(monkeypatch):
         assert torch.equal(t.scales, eager.scales) and torch.equal(t.values.view(torch.uint8), eager.values.view(torch.uint8))
 
 
+def test_python_and_native_paths_give_the_same_bits(monkeypatch):
+    for types in ((BF16, F32), (BF16, BF16), (F32, None), (F16, None)):
+        x, r, w, dy, dh = _inputs((5, 31, 200), *types)
+
+        def every():
+            y, h, grads = _run(x, r, w, dy, dh)
+            with torch.no_grad():
+                t, h2 = P.add_rms_norm(x, r, w, quantize=True)
+                plain = P.add_rms_norm(x, r, w)
+            return (y, h, *(grads[n] for n in "xrw" if n in grads), t.values.view(torch.uint8), t.scales, h2, *plain)
+
+        first = every()
+        with monkeypatch.context() as m:
+            m.setattr(ops, "native_enabled", False)
+            second = every()
+        assert len(first) == len(second) and all(a.shape == c.shape and a.dtype == c.dtype and torch.equal(a, c) for a, c in zip(first, second))
+
+
 def test_refusals():
     x, r, w, _, _ = _inputs((4, 200), BF16, F32)
     with pytest.raises(RuntimeError, match="no gradients"):
