@@ -1329,9 +1329,9 @@ PTX_API int ptx_fp8_quantize(const void* x, void* q, float* scales, void* qt, fl
   // (a launch has fewer than 2^32 threads: 16 per block, 256 per 128 x 128)
   PTX_REQUIRE(rows < 0x7fffff00 && cols < 0x7fffff00 && (double)(rows + 127) * (double)ptx::fp8_blocks(cols) < 268435456.0, PTX_ERR_UNSUPPORTED,
               "fp8_quantize: %lld rows of %lld columns are too many", (long long)rows, (long long)cols);
-  PTX_REQUIRE(!q == !scales && !qt == !scales_t, PTX_ERR_BAD_ARG, "fp8_quantize: values without scales or the reverse");
-  PTX_REQUIRE(!col_sums || workspace || rows == 0 || cols == 0, PTX_ERR_BAD_ARG, "fp8_quantize: column sums need the workspace");
   if (cols == 0 || (rows == 0 && !col_sums)) return PTX_OK;
+  PTX_REQUIRE(rows == 0 || (!q == !scales && !qt == !scales_t), PTX_ERR_BAD_ARG, "fp8_quantize: values without scales or the reverse");
+  PTX_REQUIRE(!col_sums || workspace || rows == 0, PTX_ERR_BAD_ARG, "fp8_quantize: column sums need the workspace");
   if (rows > 0) {
     PTX_REQUIRE(x && (q || qt || col_sums), PTX_ERR_BAD_ARG, "fp8_quantize: null pointer");
     PTX_REQUIRE(aligned16(q) && aligned16(qt), PTX_ERR_BAD_ARG, "fp8_quantize: values must be 16-byte aligned");

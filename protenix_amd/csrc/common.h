@@ -129,6 +129,10 @@ __device__ __forceinline__ void load_to_lds16_s(uint64_t sbase, uint32_t voff, u
                : "v"(voff), "s"(sbase), "s"(lds_base), "n"(IMM)
                : "m0");
 }
+// The same for 4 bytes a lane, to lds_base + 4 * lane.
+__device__ __forceinline__ void load_to_lds4_s(uint64_t sbase, uint32_t voff, uint32_t lds_base) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" : : "v"(voff), "s"(sbase), "s"(lds_base) : "m0");
+}
 // A 64-bit value that is the same in all lanes, moved to scalar registers.
 __device__ __forceinline__ uint64_t uniform64(uint64_t v) {
   const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v);

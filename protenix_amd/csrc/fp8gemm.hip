@@ -11,6 +11,7 @@
 // (2^-9 and 2^-12 at most), which take it.  Results in fp32 do not: for those the values, which f16 holds exactly, are widened in registers
 // and multiplied by the f16 MFMA, whose sums are fp32 (1e-8 on the same data), at half of the 8-bit rate.
 #include <algorithm>
+#include <type_traits>
 
 #include "fp8.h"
 #include "dropout.h"
@@ -26,10 +27,12 @@ typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 // A lane's 32 values of 16 rows x 128: pieces of 16 bytes from 16 q and 64 + 16 q on (q = lane / 16), as the MFMA takes them.
 template <bool WIDE> struct Fragment {
   i32x8 v;
+  Fragment() = default;
   __device__ __forceinline__ Fragment(const i32x4& lo, const i32x4& hi) : v(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7)) {}
 };
 template <> struct Fragment<true> {
   f16x8 v[4];
+  Fragment() = default;
   __device__ __forceinline__ Fragment(const i32x4& lo, const i32x4& hi) {
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
@@ -96,131 +99,233 @@ __device__ __forceinline__ void tile_of(uint32_t id, int tiles_m, int tiles_n, i
   tn = (int)(in / high);
 }
 
-// Tiles of TM x TN, WM x WN waves of TM / WM x 64 each.  Both operands' 128 columns of a block go to LDS (direct loads, two buffers: one
-// block is loaded while the other is multiplied), rows of 128 bytes whose 16-byte pieces lie at place piece ^ (row % 8).  Rows of b
-// lie in LDS so that a lane's results of four MFMAs are 16 neighbouring n: row 16 t + i of 64 holds n = 16 (i / 4) + 4 t + i % 4.
-template <int TM, int TN, int WM, int WN> struct Fp8Tile {
+// Tiles of TM x TN, WM x WN waves of TM / WM x 64 each.  Both operands' 128 columns of a block go to LDS (direct loads into a ring of NB
+// buffers: NB - 1 blocks are on their way or there while one is multiplied), rows of 128 bytes whose 16-byte pieces lie at place piece ^ (row % 8).  Rows of b
+// lie in LDS so that what a wave stores at a time are runs of 64 bytes: with 16-bit results row 16 u + i of 64 holds
+// n = 32 (u / 2) + 8 (i / 4) + 4 (u % 2) + i % 4, and a lane's results of two MFMAs are 8 neighbours; with fp32 ones n = 16 u + i.
+template <int TM, int TN, int WM, int WN, int NB, bool PAIRS> struct Fp8Tile {
   static constexpr int W = WM * WN, MT = TM / WM / 16;
-  static constexpr int kB = 0, kA = TN * 128, kSa = kA + TM * 128, kSb = kSa + 1024, kStage = kSb + 1024;
+  static constexpr int kSa = 0, kSb = 1024, kB = 2048, kA = kB + TN * 128, kStage = kA + TM * 128;
   static constexpr int PER = (TM + TN) / 8 / W;      // loads of 1 KB per wave and block
   static constexpr int PER_B = TN / 8 / W;
-  static_assert(TN == 64 * WN && (TN / 8) % W == 0 && (TM / 8) % W == 0 && TM <= 256 && TN <= 256, "whole loads per wave");
+  // The row of b (of 64) that a group s of 8 rows of LDS has for its row e, and how many rows lie between a wave's first load and its load j.
+  static __device__ __forceinline__ int b_row(int s, int e) {
+    return PAIRS ? 32 * (s >> 2) + 8 * (2 * (s & 1) + (e >> 2)) + 4 * ((s >> 1) & 1) + (e & 3) : 8 * s + e;
+  }
+  static constexpr int b_rows(int j) { return W == 4 ? 32 * (j & 1) + 64 * (j >> 1) : 8 * W * j; }
+  // the first of the 4 columns that lane group q has of MFMA u
+  static __device__ __forceinline__ int col(int u, int q) { return PAIRS ? 32 * (u >> 1) + 8 * q + 4 * (u & 1) : 16 * u + 4 * q; }
+  static_assert((W == 4 || W % 8 == 0) && TN == 64 * WN && (TN / 8) % W == 0 && (TM / 8) % W == 0 && TM <= 256 && TN <= 256, "whole loads per wave");
 };
 
-template <int TM, int TN, int WM, int WN, bool ROWB, typename O>
-__global__ __launch_bounds__(64 * WM * WN) void fp8_tile_product(Fp8Args p) {
-  typedef Fp8Tile<TM, TN, WM, WN> C;
-  __shared__ __align__(16) uint8_t lds[2 * C::kStage];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+template <int TM, int TN, int WM, int WN, int WK, int NB, bool ROWB, typename O>
+__global__ __launch_bounds__(64 * WM * WN * WK) void fp8_tile_product(Fp8Args p) {
+  typedef Fp8Tile<TM, TN, WM, WN, NB, sizeof(O) == 2> C;
+  __shared__ __align__(16) uint8_t lds_all[WK * NB * C::kStage];
+  const int lane = threadIdx.x & 63, wave_of_all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int group = WK > 1 ? wave_of_all / C::W : 0, wave = wave_of_all - group * C::W;
+  uint8_t* lds = lds_all + group * NB * C::kStage;
   const int wm = wave / WN, wn = wave % WN, i = lane & 15, q = lane >> 4;
   const int split = blockIdx.y;
   int tm, tn;
   tile_of(blockIdx.x, p.tiles_m, p.tiles_n, tm, tn);
   const int m0 = tm * TM, n0 = tn * TN;
-  const int first = (int)((int64_t)p.blocks * split / p.splits), last = (int)((int64_t)p.blocks * (split + 1) / p.splits);
+  // this group's blocks first .. last - 1; all groups of waves make `steps` steps, those with a block less none in the last one
+  const int begin = (int)((int64_t)p.blocks * split / p.splits), count = (int)((int64_t)p.blocks * (split + 1) / p.splits) - begin;
+  const int first = begin + count * group / WK, last = begin + count * (group + 1) / WK, steps = (count + WK - 1) / WK;
   const uint32_t pitch = (uint32_t)p.blocks * kFp8Block;
-  // what this lane loads: rows beyond the end are the last one once more
+  // What this lane loads: its row of the first load and the last row there is, as offsets (a later load's row lies a number of rows
+  // behind; rows beyond the end are the last one once more).
   const int e = lane >> 3;
   const uint32_t piece = (uint32_t)((lane & 7) ^ e) * 16;
-  uint32_t off[C::PER];
-#pragma unroll
-  for (int j = 0; j < C::PER; ++j) {
-    if (j < C::PER_B) {
-      const int g = wave + C::W * j, s = g & 7;
-      const int row = 64 * (g >> 3) + 16 * (2 * (s & 1) + (e >> 2)) + 4 * (s >> 1) + (e & 3);
-      off[j] = (uint32_t)min(row, p.n - 1 - n0) * pitch + piece;
-    } else {
-      const int row = 8 * (wave + C::W * (j - C::PER_B)) + e;
-      off[j] = (uint32_t)min(row, p.m - 1 - m0) * pitch + piece;
-    }
-  }
+  uint32_t first_b = (uint32_t)(64 * (wave >> 3) + C::b_row(wave & 7, e)) * pitch + piece;
+  uint32_t first_a = (uint32_t)(8 * wave + e) * pitch + piece;
+  const uint32_t last_b = (uint32_t)(min(TN, p.n - n0) - 1) * pitch + piece, last_a = (uint32_t)(min(TM, p.m - m0) - 1) * pitch + piece;
   const uint64_t base_a = uniform64((uint64_t)(p.a + (int64_t)m0 * pitch)), base_b = uniform64((uint64_t)(p.b + (int64_t)n0 * pitch));
   const int64_t sp_a = fp8_scale_pitch(p.m), sp_b = fp8_scale_pitch(p.n);
   const uint64_t base_sa = uniform64((uint64_t)(p.sa + m0));
   const uint32_t off_sa = 4u * (uint32_t)min((int64_t)4 * lane, sp_a - 4 - m0);
-  const uint64_t base_sb = uniform64((uint64_t)(p.sb + (ROWB ? n0 : 0)));
-  const uint32_t off_sb = ROWB ? 4u * (uint32_t)min((int64_t)4 * lane, sp_b - 4 - n0) : 0u;
+  // b's scales: of this tile's rows, or of the waves' 64 columns each (lane l: wave l of a row of them)
+  const int block_n = ROWB ? 0 : n0 / kFp8Block;
+  const uint64_t base_sb = uniform64((uint64_t)(p.sb + (ROWB ? n0 : (int64_t)block_n * p.blocks)));
+  const uint32_t off_sb = ROWB ? 4u * (uint32_t)min((int64_t)4 * lane, sp_b - 4 - n0)
+                               : 4u * (uint32_t)(min(n0 + 64 * min(lane, WN - 1), p.n - 1) / kFp8Block - block_n) * (uint32_t)p.blocks;
   const uint32_t lds0 = lds_address(lds);
-  auto load = [&](int block, int buf) {
+  // one of a wave's PER + 1 loads of a block: a KB of an operand each, and the scales
+  auto load = [&](int step, int buf, int j) {
     const uint32_t to = lds0 + buf * C::kStage;
+    const int block = WK > 1 ? max(min(first + step, last - 1), first) : first + step;
     const uint64_t k = (uint64_t)block * kFp8Block;
-#pragma unroll
-    for (int j = 0; j < C::PER; ++j) {
-      if (j < C::PER_B) load_to_lds16_s<0>(base_b + k, off[j], to + C::kB + 1024 * (wave + C::W * j));
-      else load_to_lds16_s<0>(base_a + k, off[j], to + C::kA + 1024 * (wave + C::W * (j - C::PER_B)));
+    if (j < C::PER_B) {
+      asm volatile("" : "+v"(first_b));      // (the offset is formed here: kept, they would take as many registers as there are loads)
+      load_to_lds16_s<0>(base_b + k, min(first_b + C::b_rows(j) * pitch, last_b), to + C::kB + 1024 * (wave + C::W * j));
+    } else if (j < C::PER) {
+      asm volatile("" : "+v"(first_a));
+      const int r = j - C::PER_B;
+      load_to_lds16_s<0>(base_a + k, min(first_a + 8 * C::W * r * pitch, last_a), to + C::kA + 1024 * (wave + C::W * r));
+    } else if (wave == 0) {
+      load_to_lds16_s<0>(base_sa + 4 * (uint64_t)block * sp_a, off_sa, to + C::kSa);
+    } else if (wave == C::W - 1) {
+      if (ROWB) load_to_lds16_s<0>(base_sb + 4 * (uint64_t)block * sp_b, off_sb, to + C::kSb);
+      else load_to_lds4_s(base_sb + 4 * (uint64_t)block, off_sb, to + C::kSb);
     }
-    if (wave == 0) load_to_lds16_s<0>(base_sa + 4 * (uint64_t)block * sp_a, off_sa, to + C::kSa);
-    if (ROWB && wave == C::W - 1) load_to_lds16_s<0>(base_sb + 4 * (uint64_t)block * sp_b, off_sb, to + C::kSb);
   };
-  // this wave's scale of b per block
-  const float* sb = p.sb + (ROWB ? 0 : (int64_t)__builtin_amdgcn_readfirstlane(min(n0 + 64 * wn, p.n - 1) / kFp8Block) * p.blocks);
   f32x4 acc[C::MT][4];
 #pragma unroll
   for (int t = 0; t < C::MT; ++t)
 #pragma unroll
     for (int u = 0; u < 4; ++u) acc[t][u] = f32x4{};
-  const int at = i * 128 + ((q ^ (i & 7)) << 4);
+  const int at = i * 128 + ((q ^ (i & 7)) << 4), row0 = wm * (TM / WM);
   typedef Fragment<sizeof(O) == 4> F;
   auto fragment = [&](const uint8_t* tile) {      // 16 rows of 128 bytes
     return F(*reinterpret_cast<const i32x4*>(tile + at), *reinterpret_cast<const i32x4*>(tile + (at ^ 64)));
   };
-  load(first, 0);
-  float next_sb = ROWB ? 1.0f : sb[first];
-  for (int block = first; block < last; ++block) {
-    const int buf = (block - first) & 1;
-    ring_barrier<0>();
-    if (block + 1 < last) load(block + 1, buf ^ 1);
-    const float scale_b = next_sb;
-    if (!ROWB && block + 1 < last) next_sb = sb[block + 1];
-    const uint8_t* st = lds + buf * C::kStage;
+  struct B {
+    F f[4];
+  };
+  auto read_b = [&](const uint8_t* st) {
     const uint8_t* tb = st + C::kB + 64 * wn * 128;
-    const F fb[4] = {fragment(tb), fragment(tb + 16 * 128), fragment(tb + 32 * 128), fragment(tb + 48 * 128)};
+    return B{{fragment(tb), fragment(tb + 16 * 128), fragment(tb + 32 * 128), fragment(tb + 48 * 128)}};
+  };
+  auto read_a = [&](const uint8_t* st, int t) { return fragment(st + C::kA + (row0 + 16 * t) * 128); };
+  // (the scale of b by way of LDS too: a load that the compiler knows of would wait for all of these)
+  auto read_scale_b = [&](const uint8_t* st) { return ROWB ? 1.0f : *reinterpret_cast<const float*>(st + C::kSb + 4 * wn); };
+  auto read_s = [&](const uint8_t* st, int t) { return *reinterpret_cast<const float*>(st + C::kSa + 4 * (row0 + 16 * t + i)); };
+  // A wave's stages overlap: the loads of a later block are spread over this one's first row tiles, a row tile's fragments are read while
+  // the one before is multiplied, and its results scaled and added while the next one is.  The waves meet once a block, behind the last
+  // multiplications, which still run while the next block's first fragments are read.
+  // Before the next block is read: this wave's loads of it have landed (all but those of the AFTER youngest blocks), and all waves' have.
+  auto meet = [&](auto after) {
+    constexpr int AFTER = after.value;
+    if (wave == 0 || wave == C::W - 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(AFTER * (C::PER + 1)) : "memory");
+    else asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(AFTER * C::PER) : "memory");
+  };
+#pragma unroll
+  for (int k = 0; k < NB - 1; ++k)
+    if (k == 0 || k < steps)
+#pragma unroll
+      for (int j = 0; j <= C::PER; ++j) load(k, k, j);
+  if (NB - 1 <= steps) meet(std::integral_constant<int, NB - 2>{});
+  else meet(std::integral_constant<int, 0>{});
+  B fb = read_b(lds);
+  F fa = read_a(lds, 0);
+  float scale_b = read_scale_b(lds), sa = read_s(lds, 0), s_before = 0.0f;
+  f32x4 d[4] = {f32x4{}, f32x4{}, f32x4{}, f32x4{}};
+  int buf = 0;
+  // loads: of the block NB - 1 behind this one; next: there is one behind this one
+  auto multiply = [&](int step, auto loads, auto next) {
+    const uint8_t* st = lds + buf * C::kStage;
+    const int buf_next = buf + 1 == NB ? 0 : buf + 1, buf_loaded = buf == 0 ? NB - 1 : buf - 1;
     f32x4 rb[4];
     if constexpr (ROWB) {
 #pragma unroll
-      for (int u = 0; u < 4; ++u) rb[u] = *reinterpret_cast<const f32x4*>(st + C::kSb + 4 * (64 * wn + 16 * q + 4 * u));
+      for (int u = 0; u < 4; ++u) rb[u] = *reinterpret_cast<const f32x4*>(st + C::kSb + 4 * (64 * wn + C::col(u, q)));
     }
 #pragma unroll
     for (int t = 0; t < C::MT; ++t) {
-      const int row = wm * (TM / WM) + 16 * t;
-      const F fa = fragment(st + C::kA + row * 128);
-      const float s = *reinterpret_cast<const float*>(st + C::kSa + 4 * (row + i)) * scale_b;
-      f32x4 d[4];
+      __builtin_amdgcn_sched_barrier(0);      // (else all reads move to the front, and registers run out)
+      const float s = sa * scale_b;
+      F fa_next;
+      if (t + 1 < C::MT) {
+        fa_next = read_a(st, t + 1);
+        sa = read_s(st, t + 1);
+      }
+      if constexpr (loads.value) {
+        // (as many as end by half of the row tiles)
+        constexpr int EACH = (C::PER + 1 + (C::MT + 1) / 2 - 1) / ((C::MT + 1) / 2);
 #pragma unroll
-      for (int u = 0; u < 4; ++u) d[u] = mma128(fb[u], fa);
+        for (int j = EACH * t; j < EACH * (t + 1); ++j)
+          if (j <= C::PER) load(step + NB - 1, buf_loaded, j);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int before = t == 0 ? C::MT - 1 : t - 1;
+        if (!ROWB || t > 0) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[before][u][r] = __builtin_fmaf(d[u][r], ROWB ? s_before * rb[u][r] : s_before, acc[before][u][r]);
+          asm volatile("" : "+v"(acc[before][u]));      // (here and not at the block's end, where the compiler would gather them all)
+        }
+        d[u] = mma128(fb.f[u], fa);
+      }
+      s_before = s;
+      if (t + 1 < C::MT) fa = fa_next;
+    }
+    if constexpr (next.value) {
+      __builtin_amdgcn_sched_barrier(0);
+      const uint8_t* sn = lds + buf_next * C::kStage;
+      meet(std::integral_constant<int, loads.value ? NB - 2 : 0>{});
+      fb = read_b(sn);
+      fa = read_a(sn, 0);
+      sa = read_s(sn, 0);
+      scale_b = read_scale_b(sn);
+      buf = buf_next;
+    }
+    if constexpr (ROWB) {      // (the scales of b's rows are the block's own)
 #pragma unroll
       for (int u = 0; u < 4; ++u)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) acc[t][u][r] = __builtin_fmaf(d[u][r], ROWB ? s * rb[u][r] : s, acc[t][u][r]);
+        for (int r = 0; r < 4; ++r) acc[C::MT - 1][u][r] = __builtin_fmaf(d[u][r], s_before * rb[u][r], acc[C::MT - 1][u][r]);
     }
+  };
+  int step = 0;
+  for (; step + NB - 1 < steps; ++step) multiply(step, std::true_type{}, std::true_type{});
+  if constexpr (NB > 2)
+    for (; step + 1 < steps; ++step) multiply(step, std::false_type{}, std::true_type{});
+  if (WK == 1 || first + step < last) multiply(step, std::false_type{}, std::false_type{});
+  if constexpr (!ROWB) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) acc[C::MT - 1][u][r] = __builtin_fmaf(d[u][r], s_before, acc[C::MT - 1][u][r]);
   }
-  const int n = n0 + 64 * wn + 16 * q;
+  if constexpr (WK > 1) {
+    // the groups' sums, added in their order
+    f32x4* sums = reinterpret_cast<f32x4*>(lds_all) + wave * C::MT * 4 * kWave + lane;
+    __syncthreads();
+    if (group > 0)
+#pragma unroll
+      for (int t = 0; t < C::MT; ++t)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) sums[((group - 1) * C::W * C::MT * 4 + 4 * t + u) * kWave] = acc[t][u];
+    __syncthreads();
+    if (group > 0) return;
+#pragma unroll
+    for (int g = 0; g < WK - 1; ++g)
+#pragma unroll
+      for (int t = 0; t < C::MT; ++t)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) acc[t][u] += sums[(g * C::W * C::MT * 4 + 4 * t + u) * kWave];
+  }
+  const int n = n0 + 64 * wn;
   f32x4 bias[4];
 #pragma unroll
   for (int u = 0; u < 4; ++u)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) bias[u][r] = p.bias && n + 4 * u + r < p.n ? param_at(p.bias, p.bias_type, n + 4 * u + r) : 0.0f;
+    for (int r = 0; r < 4; ++r) {
+      const int c = n + C::col(u, q) + r;
+      bias[u][r] = p.bias && c < p.n ? param_at(p.bias, p.bias_type, c) : 0.0f;
+    }
 #pragma unroll
   for (int t = 0; t < C::MT; ++t) {
-    const int m = m0 + wm * (TM / WM) + 16 * t + i;
+    const int m = m0 + row0 + 16 * t + i;
     if (m >= p.m) continue;
     if (p.splits > 1) {
       float* row = (float*)p.out + ((int64_t)split * p.m + m) * p.n;
 #pragma unroll
-      for (int u = 0; u < 4; ++u) store4(row, n + 4 * u, p.n, acc[t][u]);
+      for (int u = 0; u < 4; ++u) store4(row, n + C::col(u, q), p.n, acc[t][u]);
     } else {
       O* row = (O*)p.out + (int64_t)m * p.n;
-      if (n + 16 <= p.n && sizeof(O) == 2) {
+      if (sizeof(O) == 2 && n + 64 <= p.n) {
 #pragma unroll
         for (int u = 0; u < 4; u += 2) {
           f32x8 v;
 #pragma unroll
           for (int r = 0; r < 8; ++r) v[r] = acc[t][u + r / 4][r % 4] + bias[u + r / 4][r % 4];
-          store_cols(row + n + 4 * u, v, 8);
+          store_cols(row + n + C::col(u, q), v, 8);
         }
       } else {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) store4(row, n + 4 * u, p.n, acc[t][u] + bias[u]);
+        for (int u = 0; u < 4; ++u) store4(row, n + C::col(u, q), p.n, acc[t][u] + bias[u]);
       }
     }
   }
@@ -249,55 +354,57 @@ __global__ __launch_bounds__(256) void fp8_join_kernel(const float* __restrict__
   }
 }
 
-// Few rows of a (16 MT of them): bound by reading b once.  A workgroup has 16 rows of b; its waves share the blocks of k (one each in
-// turn), read b straight into registers (16 rows of whole 128-byte lines) and a from the caches, and add their sums in LDS, in their order.
-template <int MT, typename O>
+// Up to 16 rows of a: bound by reading b once, and by the time a read takes.  A workgroup has 16 rows of b; its waves share the blocks of k,
+// read b straight into registers (16 rows of whole 128-byte lines) and a from the caches, four blocks before the first is multiplied,
+// and add their sums in LDS, in their order.  1 x 2048 x 8192 5.0 us, 1 x 4096 x 4096 4.8 (3.4 TB/s, 2.5 us of it the launch's).  With more
+// rows the caches are asked for a too often (37 x 4096 x 4096 12 us in three groups of 16, as tiles with a split of k 8).
+template <typename O>
 __global__ __launch_bounds__(512) void fp8_few_rows_product(Fp8Args p) {
   constexpr int W = 8;
-  __shared__ f32x4 sums[W][MT][kWave];
+  __shared__ f32x4 sums[W][kWave];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, q = lane >> 4;
-  const int n0 = blockIdx.x * 16;
-  const int64_t pitch = (int64_t)p.blocks * kFp8Block, sp = fp8_scale_pitch(p.m);
+  const int n0 = blockIdx.x * 16, row = min(i, p.m - 1);
+  const int64_t pitch = fp8_pitch((int64_t)p.blocks * kFp8Block), sp = fp8_scale_pitch(p.m);
   typedef Fragment<sizeof(O) == 4> F;
-  auto fragment = [&](const uint8_t* row) {
-    return F(*reinterpret_cast<const i32x4*>(row + 16 * q), *reinterpret_cast<const i32x4*>(row + 64 + 16 * q));
-  };
-  const uint8_t* rb = p.b + min(n0 + i, p.n - 1) * pitch;
-  const float* sb = p.sb + (int64_t)(n0 / kFp8Block) * p.blocks;
-  f32x4 acc[MT];
-  const uint8_t* ra[MT];
-  int row[MT];
+  const float *sb = p.sb + (int64_t)(n0 / kFp8Block) * p.blocks, *sa = p.sa + row;
+  const uint8_t *rb = p.b + min(n0 + i, p.n - 1) * pitch + 16 * q, *ra = p.a + row * pitch + 16 * q;
+  f32x4 acc = f32x4{};
+  auto multiply = [&](int first, auto count) {
+    constexpr int N = count.value;
+    i32x4 b[N][2], a[N][2];
+    float s[N];
 #pragma unroll
-  for (int t = 0; t < MT; ++t) {
-    acc[t] = f32x4{};
-    row[t] = min(16 * t + i, p.m - 1);
-    ra[t] = p.a + row[t] * pitch;
-  }
-#pragma unroll 2
-  for (int block = wave; block < p.blocks; block += W) {
-    const F fb = fragment(rb + (int64_t)block * kFp8Block);
-    const float s = sb[block];
+    for (int j = 0; j < N; ++j) {
+      const int64_t at = (int64_t)(first + W * j) * kFp8Block;
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
-      const f32x4 d = mma128(fb, fragment(ra[t] + (int64_t)block * kFp8Block));
-      const float f = s * p.sa[block * sp + row[t]];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) acc[t][r] = __builtin_fmaf(d[r], f, acc[t][r]);
+      for (int h = 0; h < 2; ++h) {
+        b[j][h] = *reinterpret_cast<const i32x4*>(rb + at + 64 * h);
+        a[j][h] = *reinterpret_cast<const i32x4*>(ra + at + 64 * h);
+      }
+      s[j] = sb[first + W * j] * sa[(first + W * j) * sp];
     }
-  }
+    __builtin_amdgcn_sched_barrier(0);      // (else the loads move to where they are used, one after the other)
 #pragma unroll
-  for (int t = 0; t < MT; ++t) sums[wave][t][lane] = acc[t];
+    for (int j = 0; j < N; ++j) {
+      const f32x4 d = mma128(F(b[j][0], b[j][1]), F(a[j][0], a[j][1]));
+#pragma unroll
+      for (int r = 0; r < 4; ++r) acc[r] = __builtin_fmaf(d[r], s[j], acc[r]);
+    }
+  };
+  int block = wave;
+  for (; block + 3 * W < p.blocks; block += 4 * W) multiply(block, std::integral_constant<int, 4>{});
+  for (; block + W < p.blocks; block += 2 * W) multiply(block, std::integral_constant<int, 2>{});
+  if (block < p.blocks) multiply(block, std::integral_constant<int, 1>{});
+  sums[wave][lane] = acc;
   __syncthreads();
-  for (int t = wave; t < MT; t += W) {
-    f32x4 v = sums[0][t][lane];
+  if (wave > 0) return;
 #pragma unroll
-    for (int w = 1; w < W; ++w) v += sums[w][t][lane];
-    const int m = 16 * t + i, n = n0 + 4 * q;
-    if (m >= p.m) continue;
+  for (int w = 1; w < W; ++w) acc += sums[w][lane];
+  const int n = n0 + 4 * q;
+  if (i >= p.m) return;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) v[r] += p.bias && n + r < p.n ? param_at(p.bias, p.bias_type, n + r) : 0.0f;
-    store4((O*)p.out + (int64_t)m * p.n, n, p.n, v);
-  }
+  for (int r = 0; r < 4; ++r) acc[r] += p.bias && n + r < p.n ? param_at(p.bias, p.bias_type, n + r) : 0.0f;
+  store4((O*)p.out + (int64_t)i * p.n, n, p.n, acc);
 }
 
 // ---- which kernel ---------------------------------------------------------------------------------------
@@ -307,15 +414,14 @@ struct Fp8Plan {
   int splits;
 };
 Fp8Plan fp8_plan(int64_t m, int64_t n, int64_t blocks, bool square) {
-  if (m <= 64 && square) return {0, 1};
+  if (m <= 16 && square) return {0, 1};
   auto tiles = [&](int t) { return ((m + t - 1) / t) * ((n + t - 1) / t); };
-  if (tiles(256) >= 192) return {256, 1};
+  // (not where more than a third of the large tiles would lie beyond the end)
+  if (tiles(256) >= 192 && 3 * m * n >= 2 * 65536 * tiles(256)) return {256, 1};
   if (tiles(128) >= 192) return {128, 1};
-  const int tile = 64;
-  const int64_t count = tiles(tile);
   int splits = 1;
-  while (splits < 16 && count * splits < 256 && blocks / (2 * splits) >= 4) splits *= 2;
-  return {tile, splits};
+  while (splits < 8 && tiles(64) * splits <= 128 && blocks / (2 * splits) >= 4) splits *= 2;
+  return {64, splits};
 }
 }  // namespace
 
@@ -324,11 +430,11 @@ int64_t fp8_matmul_workspace_elems(int64_t m, int64_t n, int64_t blocks, bool sq
   return plan.splits > 1 ? plan.splits * m * n : 0;
 }
 
-template <int TM, int TN, int WM, int WN, typename O> static void tile_product(Fp8Args p, bool square, hipStream_t stream) {
+template <int TM, int TN, int WM, int WN, int WK, int NB, typename O> static void tile_product(Fp8Args p, bool square, hipStream_t stream) {
   p.tiles_m = (p.m + TM - 1) / TM;
   p.tiles_n = (p.n + TN - 1) / TN;
-  auto* kernel = square ? fp8_tile_product<TM, TN, WM, WN, false, O> : fp8_tile_product<TM, TN, WM, WN, true, O>;
-  kernel<<<dim3((unsigned)p.tiles_m * p.tiles_n, p.splits), dim3(64 * WM * WN), 0, stream>>>(p);
+  auto* kernel = square ? fp8_tile_product<TM, TN, WM, WN, WK, NB, false, O> : fp8_tile_product<TM, TN, WM, WN, WK, NB, true, O>;
+  kernel<<<dim3((unsigned)p.tiles_m * p.tiles_n, p.splits), dim3(64 * WM * WN * WK), 0, stream>>>(p);
 }
 
 template <typename O>
@@ -337,22 +443,26 @@ int fp8_matmul(const void* a, const float* sa, const void* b, const float* sb, b
   const Fp8Plan plan = fp8_plan(m, n, blocks, square);
   Fp8Args p{(const uint8_t*)a, sa, (const uint8_t*)b, sb, bias, bias_type, out, m, n, blocks, 0, 0, plan.splits};
   if (plan.tile == 0) {
-    const dim3 grid((n + 15) / 16), block(512);
-    switch ((m + 15) / 16) {
-      case 1: fp8_few_rows_product<1, O><<<grid, block, 0, stream>>>(p); break;
-      case 2: fp8_few_rows_product<2, O><<<grid, block, 0, stream>>>(p); break;
-      case 3: fp8_few_rows_product<3, O><<<grid, block, 0, stream>>>(p); break;
-      default: fp8_few_rows_product<4, O><<<grid, block, 0, stream>>>(p);
-    }
+    fp8_few_rows_product<O><<<dim3((n + 15) / 16), dim3(512), 0, stream>>>(p);
     return 0;
   }
   if (plan.splits > 1) {
     p.out = workspace;
     p.bias = nullptr;
   }
-  if (plan.tile == 256) tile_product<256, 256, 2, 4, O>(p, square, stream);
-  else if (plan.tile == 128) tile_product<128, 128, 2, 2, O>(p, square, stream);
-  else tile_product<64, 64, 4, 1, O>(p, square, stream);
+  const int64_t tiles = (int64_t)((m + plan.tile - 1) / plan.tile) * ((n + plan.tile - 1) / plan.tile);
+  if (plan.tile == 256) {
+    // (fp32 results have widened fragments, twice the registers)
+    if constexpr (sizeof(O) == 4) tile_product<256, 128, 4, 2, 1, 2, O>(p, square, stream);
+    else tile_product<256, 256, 2, 4, 1, 2, O>(p, square, stream);
+  } else if (plan.tile == 128) {
+    if (tiles >= 512) tile_product<128, 128, 2, 2, 1, 2, O>(p, square, stream);
+    else tile_product<128, 128, 2, 2, 2, 2, O>(p, square, stream);
+  } else if (tiles * plan.splits > 256) {
+    tile_product<64, 64, 4, 1, 2, 2, O>(p, square, stream);
+  } else {
+    tile_product<64, 64, 4, 1, 2, 4, O>(p, square, stream);
+  }
   if (plan.splits > 1) {
     const int64_t count = (int64_t)m * n;
     fp8_join_kernel<O><<<dim3((unsigned)((count + 1023) / 1024)), dim3(256), 0, stream>>>(workspace, plan.splits, count, n, bias, bias_type, out);

@@ -122,7 +122,7 @@ __global__ __launch_bounds__(256) void fp8_tile_kernel(const T* __restrict__ x, 
   }
   if (SQUARE && tid == 0) scales_t[(int64_t)col_tile * row_tiles + row_tile] = all.s;
   __syncthreads();
-  const int64_t pitch_t = row_tiles * kFp8Block;
+  const int64_t pitch_t = fp8_pitch(rows);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int c = 32 * i + (tid >> 3), j = tid & 7, turn = c >> 3;      // bytes 16 j .. 16 j + 15 of the column: places 2 j and 2 j + 1, each ^ turn

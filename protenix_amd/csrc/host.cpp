@@ -1484,7 +1484,7 @@ Fp8Operand operand_of(const OperandTuple& t) { return {std::get<0>(t), std::get<
 
 Fp8Operand fp8_buffers(int64_t rows, int64_t cols, bool square, const at::TensorOptions& like) {
   const int64_t blocks = (cols + 127) / 128, lead = square ? (rows + 127) / 128 : ptx_fp8_scale_pitch(rows);
-  return {at::empty({rows, blocks * 128}, like.dtype(at::kFloat8_e4m3fn)),
+  return {at::empty({rows, ptx_fp8_pitch(cols)}, like.dtype(at::kFloat8_e4m3fn)),
           at::empty(square ? std::initializer_list<int64_t>{lead, blocks} : std::initializer_list<int64_t>{blocks, lead}, like.dtype(at::kFloat)),
           rows, cols, square};
 }

@@ -814,7 +814,7 @@ def fp8_buffers(rows: int, cols: int, square: bool, device) -> tuple:
     """An operand with its memory as it comes."""
     lib = _lib.load()
     blocks = -(-cols // 128)
-    values = torch.empty((rows, blocks * 128), dtype=torch.float8_e4m3fn, device=device)
+    values = torch.empty((rows, lib.ptx_fp8_pitch(cols)), dtype=torch.float8_e4m3fn, device=device)
     lead = -(-rows // 128) if square else lib.ptx_fp8_scale_pitch(rows)
     scales = torch.empty((lead, blocks) if square else (blocks, lead), dtype=torch.float32, device=device)
     return values, scales, rows, cols, square
