@@ -127,9 +127,6 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void fp8_tile_product(Fp8Args p)
   uint8_t* lds = lds_all + group * NB * C::kStage;
   const int wm = wave / WN, wn = wave % WN, i = lane & 15, q = lane >> 4;
   const int split = blockIdx.y;
-  int tm, tn;
-  tile_of(blockIdx.x, p.tiles_m, p.tiles_n, tm, tn);
-  const int m0 = tm * TM, n0 = tn * TN;
   // this group's blocks first .. last - 1; all groups of waves make `steps` steps, those with a block less none in the last one
   const int begin = (int)((int64_t)p.blocks * split / p.splits), count = (int)((int64_t)p.blocks * (split + 1) / p.splits) - begin;
   const int first = begin + count * group / WK, last = begin + count * (group + 1) / WK, steps = (count + WK - 1) / WK;
@@ -140,16 +137,34 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void fp8_tile_product(Fp8Args p)
   const uint32_t piece = (uint32_t)((lane & 7) ^ e) * 16;
   uint32_t first_b = (uint32_t)(64 * (wave >> 3) + C::b_row(wave & 7, e)) * pitch + piece;
   uint32_t first_a = (uint32_t)(8 * wave + e) * pitch + piece;
-  const uint32_t last_b = (uint32_t)(min(TN, p.n - n0) - 1) * pitch + piece, last_a = (uint32_t)(min(TM, p.m - m0) - 1) * pitch + piece;
-  const uint64_t base_a = uniform64((uint64_t)(p.a + (int64_t)m0 * pitch)), base_b = uniform64((uint64_t)(p.b + (int64_t)n0 * pitch));
   const int64_t sp_a = fp8_scale_pitch(p.m), sp_b = fp8_scale_pitch(p.n);
-  const uint64_t base_sa = uniform64((uint64_t)(p.sa + m0));
-  const uint32_t off_sa = 4u * (uint32_t)min((int64_t)4 * lane, sp_a - 4 - m0);
-  // b's scales: of this tile's rows, or of the waves' 64 columns each (lane l: wave l of a row of them)
-  const int block_n = ROWB ? 0 : n0 / kFp8Block;
-  const uint64_t base_sb = uniform64((uint64_t)(p.sb + (ROWB ? n0 : (int64_t)block_n * p.blocks)));
-  const uint32_t off_sb = ROWB ? 4u * (uint32_t)min((int64_t)4 * lane, sp_b - 4 - n0)
-                               : 4u * (uint32_t)(min(n0 + 64 * min(lane, WN - 1), p.n - 1) / kFp8Block - block_n) * (uint32_t)p.blocks;
+  // where a tile's operands lie
+  struct Place {
+    int m0, n0;
+    uint64_t a, b, sa, sb;
+    uint32_t last_a, last_b, off_sa, off_sb;
+  };
+  auto place = [&](uint32_t tile) {
+    Place l;
+    int tm, tn;
+    tile_of(tile, p.tiles_m, p.tiles_n, tm, tn);
+    l.m0 = tm * TM;
+    l.n0 = tn * TN;
+    l.a = uniform64((uint64_t)(p.a + (int64_t)l.m0 * pitch));
+    l.b = uniform64((uint64_t)(p.b + (int64_t)l.n0 * pitch));
+    l.last_a = (uint32_t)(min(TM, p.m - l.m0) - 1) * pitch + piece;
+    l.last_b = (uint32_t)(min(TN, p.n - l.n0) - 1) * pitch + piece;
+    l.sa = uniform64((uint64_t)(p.sa + l.m0));
+    l.off_sa = 4u * (uint32_t)min((int64_t)4 * lane, sp_a - 4 - l.m0);
+    // b's scales: of this tile's rows, or of the waves' 64 columns each (lane l: wave l of a row of them)
+    const int block_n = ROWB ? 0 : l.n0 / kFp8Block;
+    l.sb = uniform64((uint64_t)(p.sb + (ROWB ? l.n0 : (int64_t)block_n * p.blocks)));
+    l.off_sb = ROWB ? 4u * (uint32_t)min((int64_t)4 * lane, sp_b - 4 - l.n0)
+                    : 4u * (uint32_t)(min(l.n0 + 64 * min(lane, WN - 1), p.n - 1) / kFp8Block - block_n) * (uint32_t)p.blocks;
+    return l;
+  };
+  uint32_t tile = blockIdx.x;
+  Place from = place(tile);      // what is loaded next belongs to this one
   const uint32_t lds0 = lds_address(lds);
   // one of a wave's PER + 1 loads of a block: a KB of an operand each, and the scales
   auto load = [&](int step, int buf, int j) {
@@ -158,16 +173,16 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void fp8_tile_product(Fp8Args p)
     const uint64_t k = (uint64_t)block * kFp8Block;
     if (j < C::PER_B) {
       asm volatile("" : "+v"(first_b));      // (the offset is formed here: kept, they would take as many registers as there are loads)
-      load_to_lds16_s<0>(base_b + k, min(first_b + C::b_rows(j) * pitch, last_b), to + C::kB + 1024 * (wave + C::W * j));
+      load_to_lds16_s<0>(from.b + k, min(first_b + C::b_rows(j) * pitch, from.last_b), to + C::kB + 1024 * (wave + C::W * j));
     } else if (j < C::PER) {
       asm volatile("" : "+v"(first_a));
       const int r = j - C::PER_B;
-      load_to_lds16_s<0>(base_a + k, min(first_a + 8 * C::W * r * pitch, last_a), to + C::kA + 1024 * (wave + C::W * r));
+      load_to_lds16_s<0>(from.a + k, min(first_a + 8 * C::W * r * pitch, from.last_a), to + C::kA + 1024 * (wave + C::W * r));
     } else if (wave == 0) {
-      load_to_lds16_s<0>(base_sa + 4 * (uint64_t)block * sp_a, off_sa, to + C::kSa);
+      load_to_lds16_s<0>(from.sa + 4 * (uint64_t)block * sp_a, from.off_sa, to + C::kSa);
     } else if (wave == C::W - 1) {
-      if (ROWB) load_to_lds16_s<0>(base_sb + 4 * (uint64_t)block * sp_b, off_sb, to + C::kSb);
-      else load_to_lds4_s(base_sb + 4 * (uint64_t)block, off_sb, to + C::kSb);
+      if (ROWB) load_to_lds16_s<0>(from.sb + 4 * (uint64_t)block * sp_b, from.off_sb, to + C::kSb);
+      else load_to_lds4_s(from.sb + 4 * (uint64_t)block, from.off_sb, to + C::kSb);
     }
   };
   f32x4 acc[C::MT][4];
@@ -194,26 +209,30 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void fp8_tile_product(Fp8Args p)
   // A wave's stages overlap: the loads of a later block are spread over this one's first row tiles, a row tile's fragments are read while
   // the one before is multiplied, and its results scaled and added while the next one is.  The waves meet once a block, behind the last
   // multiplications, which still run while the next block's first fragments are read.
-  // Before the next block is read: this wave's loads of it have landed (all but those of the AFTER youngest blocks), and all waves' have.
-  auto meet = [&](auto after) {
-    constexpr int AFTER = after.value;
-    if (wave == 0 || wave == C::W - 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(AFTER * (C::PER + 1)) : "memory");
-    else asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(AFTER * C::PER) : "memory");
+  // Before the next block is read: this wave's loads of it have landed (all but those of the `after` youngest blocks and `stores` that were
+  // issued behind them), and all waves' have.
+  auto meet = [&](auto after, auto stores) {
+    if (wave == 0 || wave == C::W - 1)
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(after.value * (C::PER + 1) + stores.value) : "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(after.value * C::PER + stores.value) : "memory");
   };
+  constexpr std::integral_constant<int, 0> none{};
 #pragma unroll
   for (int k = 0; k < NB - 1; ++k)
     if (k == 0 || k < steps)
 #pragma unroll
       for (int j = 0; j <= C::PER; ++j) load(k, k, j);
-  if (NB - 1 <= steps) meet(std::integral_constant<int, NB - 2>{});
-  else meet(std::integral_constant<int, 0>{});
+  if (NB - 1 <= steps) meet(std::integral_constant<int, NB - 2>{}, none);
+  else meet(none, none);
   B fb = read_b(lds);
   F fa = read_a(lds, 0);
   float scale_b = read_scale_b(lds), sa = read_s(lds, 0), s_before = 0.0f;
   f32x4 d[4] = {f32x4{}, f32x4{}, f32x4{}, f32x4{}};
   int buf = 0;
-  // loads: of the block NB - 1 behind this one; next: there is one behind this one
-  auto multiply = [&](int step, auto loads, auto next) {
+  // One block; loads: of step `to_load`, into the buffer of the block before, where `loading`; next: there is a block behind this one in
+  // its tile.
+  auto multiply = [&](int to_load, bool loading, auto loads, auto next) {
     const uint8_t* st = lds + buf * C::kStage;
     const int buf_next = buf + 1 == NB ? 0 : buf + 1, buf_loaded = buf == 0 ? NB - 1 : buf - 1;
     f32x4 rb[4];
@@ -233,9 +252,10 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void fp8_tile_product(Fp8Args p)
       if constexpr (loads.value) {
         // (as many as end by half of the row tiles)
         constexpr int EACH = (C::PER + 1 + (C::MT + 1) / 2 - 1) / ((C::MT + 1) / 2);
+        if (loading)
 #pragma unroll
-        for (int j = EACH * t; j < EACH * (t + 1); ++j)
-          if (j <= C::PER) load(step + NB - 1, buf_loaded, j);
+          for (int j = EACH * t; j < EACH * (t + 1); ++j)
+            if (j <= C::PER) load(to_load, buf_loaded, j);
       }
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
@@ -253,7 +273,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void fp8_tile_product(Fp8Args p)
     if constexpr (next.value) {
       __builtin_amdgcn_sched_barrier(0);
       const uint8_t* sn = lds + buf_next * C::kStage;
-      meet(std::integral_constant<int, loads.value ? NB - 2 : 0>{});
+      meet(std::integral_constant<int, loads.value ? NB - 2 : 0>{}, none);
       fb = read_b(sn);
       fa = read_a(sn, 0);
       sa = read_s(sn, 0);
@@ -267,11 +287,19 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void fp8_tile_product(Fp8Args p)
         for (int r = 0; r < 4; ++r) acc[C::MT - 1][u][r] = __builtin_fmaf(d[u][r], s_before * rb[u][r], acc[C::MT - 1][u][r]);
     }
   };
+  // A workgroup walks over tiles (where it has one buffer to fill ahead and no sums of groups to add): the last block of one is multiplied
+  // while the next one's first is loaded, and its results are stored while that is on its way.
+  constexpr bool WALKS = WK == 1 && NB == 2;
+  for (;;) {
+  const int m0 = from.m0, n0 = from.n0;
   int step = 0;
-  for (; step + NB - 1 < steps; ++step) multiply(step, std::true_type{}, std::true_type{});
+  for (; step + NB - 1 < steps; ++step) multiply(step + NB - 1, true, std::true_type{}, std::true_type{});
   if constexpr (NB > 2)
-    for (; step + 1 < steps; ++step) multiply(step, std::false_type{}, std::true_type{});
-  if (WK == 1 || first + step < last) multiply(step, std::false_type{}, std::false_type{});
+    for (; step + 1 < steps; ++step) multiply(0, false, std::false_type{}, std::true_type{});
+  tile += gridDim.x;
+  const bool more = WALKS && tile < (uint32_t)p.tiles_m * p.tiles_n;
+  if (more) from = place(tile);
+  if (WK == 1 || first + step < last) multiply(0, more, std::integral_constant<bool, WALKS>{}, std::false_type{});
   if constexpr (!ROWB) {
 #pragma unroll
     for (int u = 0; u < 4; ++u)
@@ -328,6 +356,25 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void fp8_tile_product(Fp8Args p)
         for (int u = 0; u < 4; ++u) store4(row, n + C::col(u, q), p.n, acc[t][u] + bias[u]);
       }
     }
+  }
+  if (!more) break;
+  // the next tile's first block has landed: all but what was issued behind its loads, which is a whole tile's stores, 16 bytes a lane each,
+  // or may be fewer at an edge
+  if (m0 + TM <= p.m && n0 + TN <= p.n) meet(none, std::integral_constant<int, C::MT * 4 * 4 * (int)sizeof(O) / 16>{});
+  else meet(none, none);
+  buf ^= 1;
+  const uint8_t* st = lds + buf * C::kStage;
+  fb = read_b(st);
+  fa = read_a(st, 0);
+  sa = read_s(st, 0);
+  scale_b = read_scale_b(st);
+  s_before = 0.0f;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) d[u] = f32x4{};
+#pragma unroll
+  for (int t = 0; t < C::MT; ++t)
+#pragma unroll
+    for (int u = 0; u < 4; ++u) acc[t][u] = f32x4{};
   }
 }
 
@@ -434,7 +481,10 @@ template <int TM, int TN, int WM, int WN, int WK, int NB, typename O> static voi
   p.tiles_m = (p.m + TM - 1) / TM;
   p.tiles_n = (p.n + TN - 1) / TN;
   auto* kernel = square ? fp8_tile_product<TM, TN, WM, WN, WK, NB, false, O> : fp8_tile_product<TM, TN, WM, WN, WK, NB, true, O>;
-  kernel<<<dim3((unsigned)p.tiles_m * p.tiles_n, p.splits), dim3(64 * WM * WN * WK), 0, stream>>>(p);
+  // (walking over tiles: as many workgroups as the compute units hold)
+  const unsigned tiles = (unsigned)p.tiles_m * p.tiles_n;
+  const unsigned groups = WK == 1 && NB == 2 ? std::min(tiles, 256u * (TM * TN > 128 * 128 ? 1 : 2)) : tiles;
+  kernel<<<dim3(groups, p.splits), dim3(64 * WM * WN * WK), 0, stream>>>(p);
 }
 
 template <typename O>
