@@ -207,8 +207,8 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void fp8_tile_product(Fp8Args p)
   auto read_scale_b = [&](const uint8_t* st) { return ROWB ? 1.0f : *reinterpret_cast<const float*>(st + C::kSb + 4 * wn); };
   auto read_s = [&](const uint8_t* st, int t) { return *reinterpret_cast<const float*>(st + C::kSa + 4 * (row0 + 16 * t + i)); };
   // A wave's stages overlap: the loads of a later block are spread over this one's first row tiles, a row tile's fragments are read while
-  // the one before is multiplied, and its results scaled and added while the next one is.  The waves meet once a block, behind the last
-  // multiplications, which still run while the next block's first fragments are read.
+  // the one before is multiplied, and its results scaled and added while the next one is.  The waves meet once a block, in front of its
+  // last row tile - all reads of its buffer have returned then -, under whose multiplications the next block's first fragments are read.
   // Before the next block is read: this wave's loads of it have landed (all but those of the `after` youngest blocks and `stores` that were
   // issued behind them), and all waves' have.
   auto meet = [&](auto after, auto stores) {
@@ -244,6 +244,8 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void fp8_tile_product(Fp8Args p)
     for (int t = 0; t < C::MT; ++t) {
       __builtin_amdgcn_sched_barrier(0);      // (else all reads move to the front, and registers run out)
       const float s = sa * scale_b;
+      const bool ahead = next.value && t + 1 == C::MT;      // (known where the loop is unrolled)
+      const uint8_t* sn = lds + buf_next * C::kStage;
       F fa_next;
       if (t + 1 < C::MT) {
         fa_next = read_a(st, t + 1);
@@ -257,6 +259,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void fp8_tile_product(Fp8Args p)
           for (int j = EACH * t; j < EACH * (t + 1); ++j)
             if (j <= C::PER) load(to_load, buf_loaded, j);
       }
+      if (ahead) meet(std::integral_constant<int, loads.value ? NB - 2 : 0>{}, none);
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const int before = t == 0 ? C::MT - 1 : t - 1;
@@ -266,19 +269,17 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void fp8_tile_product(Fp8Args p)
           asm volatile("" : "+v"(acc[before][u]));      // (here and not at the block's end, where the compiler would gather them all)
         }
         d[u] = mma128(fb.f[u], fa);
+        if (ahead) fb.f[u] = fragment(sn + C::kB + (64 * wn + 16 * u) * 128);
       }
       s_before = s;
-      if (t + 1 < C::MT) fa = fa_next;
-    }
-    if constexpr (next.value) {
-      __builtin_amdgcn_sched_barrier(0);
-      const uint8_t* sn = lds + buf_next * C::kStage;
-      meet(std::integral_constant<int, loads.value ? NB - 2 : 0>{}, none);
-      fb = read_b(sn);
-      fa = read_a(sn, 0);
-      sa = read_s(sn, 0);
-      scale_b = read_scale_b(sn);
-      buf = buf_next;
+      if (ahead) {
+        fa = read_a(sn, 0);
+        sa = read_s(sn, 0);
+        scale_b = read_scale_b(sn);
+        buf = buf_next;
+      } else if (t + 1 < C::MT) {
+        fa = fa_next;
+      }
     }
     if constexpr (ROWB) {      // (the scales of b's rows are the block's own)
 #pragma unroll
