@@ -43,12 +43,20 @@ __device__ __forceinline__ uint32_t largest16(uint32_t v) {
 struct Fp8Scale {
   float s, i;
 };
+// Both quotients rounded once, in three operations each where a division takes ten: an approximation and a correction from its exact
+// remainder (Markstein: Computation of elementary functions on the IBM RISC System/6000 processor, 1990; compared with the division over
+// all mantissas).  Where top / 448 would be subnormal the result is 2^-126 either way.
 __device__ __forceinline__ Fp8Scale fp8_scale(uint32_t top) {
-  const float s = __uint_as_float(top) / 448.0f, least = 1.1754943508222875e-38f;
-  Fp8Scale r;
-  r.s = s < least ? least : s;      // (a NaN stays)
-  r.i = 1.0f / r.s;
-  return r;
+  const float a = __uint_as_float(top), least = 1.1754943508222875e-38f, r = 1.0f / 448.0f;
+  float s = a * r;
+  s = __builtin_fmaf(__builtin_fmaf(-448.0f, s, a), r, s);
+  float i = __builtin_amdgcn_rcpf(s < least ? least : s);
+  i = __builtin_fmaf(__builtin_fmaf(-(s < least ? least : s), i, 1.0f), i, i);
+  const bool infinite = top == 0x7f800000u;      // (its remainder is no number)
+  Fp8Scale q;
+  q.s = infinite ? a : s < least ? least : s;      // (a NaN stays)
+  q.i = infinite ? 0.0f : i;
+  return q;
 }
 
 typedef __attribute__((ext_vector_type(2))) uint32_t u32x2_t;

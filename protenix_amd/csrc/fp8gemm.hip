@@ -118,8 +118,9 @@ template <int TM, int TN, int WM, int WN, int NB, bool PAIRS> struct Fp8Tile {
   static_assert((W == 4 || W % 8 == 0) && TN == 64 * WN && (TN / 8) % W == 0 && (TM / 8) % W == 0 && TM <= 256 && TN <= 256, "whole loads per wave");
 };
 
+// (two workgroups of small tiles to a compute unit where their buffers leave the room: 4 waves per SIMD)
 template <int TM, int TN, int WM, int WN, int WK, int NB, bool ROWB, typename O>
-__global__ __launch_bounds__(64 * WM * WN * WK) void fp8_tile_product(Fp8Args p) {
+__global__ __launch_bounds__(64 * WM * WN * WK, TM == 64 && NB == 2 && !(ROWB && sizeof(O) == 4) ? 4 : 1) void fp8_tile_product(Fp8Args p) {
   typedef Fp8Tile<TM, TN, WM, WN, NB, sizeof(O) == 2> C;
   __shared__ __align__(16) uint8_t lds_all[WK * NB * C::kStage];
   const int lane = threadIdx.x & 63, wave_of_all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);

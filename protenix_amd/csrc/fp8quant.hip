@@ -28,14 +28,61 @@ __global__ __launch_bounds__(256) void fp8_rows_kernel(const T* __restrict__ x, 
   if (threadIdx.x % 16 == 0) scales[(int64_t)kb * fp8_scale_pitch(rows) + row] = s.s;
 }
 
+// Largest magnitudes of 8 values at a time, as whole numbers: for 16-bit types in pairs, on the bits as they come.
+template <typename T> struct Tops {
+  typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
+  static constexpr int kWords = 4;      // per 8 values, as they travel between lanes
+  u16x8 v;
+  __device__ __forceinline__ explicit Tops(const Raw8<T>& raw) : v(__builtin_bit_cast(u16x8, raw) & (unsigned short)0x7fff) {}
+  __device__ __forceinline__ void take(const Tops& o) { v = __builtin_elementwise_max(v, o.v); }
+  __device__ __forceinline__ uint32_t word(int k) const { return (uint32_t)v[2 * k] | (uint32_t)v[2 * k + 1] << 16; }
+  __device__ __forceinline__ void take_word(int k, uint32_t w) {
+    v[2 * k] = max(v[2 * k], (unsigned short)w);
+    v[2 * k + 1] = max(v[2 * k + 1], (unsigned short)(w >> 16));
+  }
+  // one of them, or the largest, as the bits of a float
+  __device__ __forceinline__ uint32_t bits(int e) const {
+    const unsigned short m = v[e];      // (by way of a variable: a cast of a vector's element takes the first one)
+    return __float_as_uint((float)__builtin_bit_cast(T, m));
+  }
+  __device__ __forceinline__ uint32_t largest_bits() const {
+    unsigned short m = v[0];
+#pragma unroll
+    for (int e = 1; e < 8; ++e) m = max(m, v[e]);
+    return __float_as_uint((float)__builtin_bit_cast(T, m));
+  }
+};
+template <> struct Tops<float> {
+  static constexpr int kWords = 8;
+  uint32_t v[8];
+  __device__ __forceinline__ explicit Tops(const Raw8<float>& raw) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = magnitude(raw[e]);
+  }
+  __device__ __forceinline__ void take(const Tops& o) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = max(v[e], o.v[e]);
+  }
+  __device__ __forceinline__ uint32_t word(int k) const { return v[k]; }
+  __device__ __forceinline__ void take_word(int k, uint32_t w) { v[k] = max(v[k], w); }
+  __device__ __forceinline__ uint32_t bits(int e) const { return v[e]; }
+  __device__ __forceinline__ uint32_t largest_bits() const {
+    uint32_t m = v[0];
+#pragma unroll
+    for (int e = 1; e < 8; ++e) m = max(m, v[e]);
+    return m;
+  }
+};
+
 // One tile of 128 x 128 per workgroup.  q, qt: either may be null.  part: null, or the tile's column sums of x, [tiles of rows][cols].
 template <typename T, bool SHORT, bool SQUARE>
 __global__ __launch_bounds__(256) void fp8_tile_kernel(const T* __restrict__ x, uint8_t* __restrict__ q, float* __restrict__ scales,
                                                        uint8_t* __restrict__ qt, float* __restrict__ scales_t, float* __restrict__ part,
                                                        int64_t rows, int cols) {
+  // (column 8 l + e of the tile at e 16 + l of the arrays by column: neighbouring lanes then use neighbouring banks)
   __shared__ __align__(16) uint8_t turned[kFp8Block * kFp8Block];
-  __shared__ uint32_t tops[4][kFp8Block];
-  __shared__ float sums[4][kFp8Block];
+  __shared__ uint32_t tops[4][Tops<T>::kWords][16];
+  __shared__ float inverse[kFp8Block], sums[4][kFp8Block];
   __shared__ uint32_t top_of_all[4];
   const int tiles = (int)fp8_blocks(cols), tid = threadIdx.x, wave = tid >> 6, l = tid & 15, g = tid >> 4;
   const int64_t row_tile = blockIdx.x / (uint32_t)tiles;
@@ -45,55 +92,72 @@ __global__ __launch_bounds__(256) void fp8_tile_kernel(const T* __restrict__ x, 
   Raw8<T> raw[8];
 #pragma unroll
   for (int p = 0; p < 8; ++p) raw[p] = load_cols<SHORT>(x + min(row0 + p, rows - 1) * cols, col, cols);
-  f32x8 v[8];
-#pragma unroll
-  for (int p = 0; p < 8; ++p) {
-    v[p] = used_cols<SHORT, T>(raw[p], n);
-    const int have = row0 + p < rows ? n : 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[p][e] = e < have ? v[p][e] : 0.0f;
-  }
-  uint32_t row_top[8];
-#pragma unroll
-  for (int p = 0; p < 8; ++p) row_top[p] = largest16(magnitude(v[p]));
-  // the largest of each column's 8 rows, then over the four groups of rows of a wave, then over the waves
-  uint32_t col_top[8];
-  float col_sum[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    uint32_t m = 0;
-    float s = 0.0f;
+  if (SHORT || (row_tile + 1) * kFp8Block > rows || (col_tile + 1) * kFp8Block > cols) {
+    // (zeros beyond the end; the values are T's own, and so their rounding to T is none)
 #pragma unroll
     for (int p = 0; p < 8; ++p) {
-      m = max(m, magnitude(v[p][e]));
-      s += v[p][e];
+      f32x8 v = used_cols<SHORT, T>(raw[p], n);
+      const int have = row0 + p < rows ? n : 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = e < have ? v[e] : 0.0f;
+      raw[p] = rounded<T>(v);
     }
-    m = max(m, (uint32_t)__shfl_xor((int)m, 16, 64));
-    col_top[e] = max(m, (uint32_t)__shfl_xor((int)m, 32, 64));
-    if (part) {
+  }
+  uint32_t row_top[8];
+  Tops<T> col_top(raw[0]);
+#pragma unroll
+  for (int p = 0; p < 8; ++p) {
+    const Tops<T> t(raw[p]);
+    if (p > 0) col_top.take(t);
+    if (!SQUARE) row_top[p] = largest16(t.largest_bits());
+  }
+  // the largest of each column's 8 rows, then over the four groups of rows of a wave, then over the waves
+#pragma unroll
+  for (int k = 0; k < Tops<T>::kWords; ++k) {
+    col_top.take_word(k, (uint32_t)__shfl_xor((int)col_top.word(k), 16, 64));
+    col_top.take_word(k, (uint32_t)__shfl_xor((int)col_top.word(k), 32, 64));
+  }
+  f32x8 v[8];
+#pragma unroll
+  for (int p = 0; p < 8; ++p) v[p] = widened<T>(raw[p]);
+  if (part) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float s = 0.0f;
+#pragma unroll
+      for (int p = 0; p < 8; ++p) s += v[p][e];
       s += __shfl_xor(s, 16, 64);
-      col_sum[e] = s + __shfl_xor(s, 32, 64);
+      s += __shfl_xor(s, 32, 64);
+      if ((tid & 63) < 16) sums[wave][16 * e + l] = s;
     }
   }
   if constexpr (SQUARE) {
-    uint32_t m = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) m = max(m, col_top[e]);
-    m = largest16(m);
+    const uint32_t m = largest16(col_top.largest_bits());
     if ((tid & 63) == 0) top_of_all[wave] = m;
-  }
-  if ((tid & 63) < 16) {
+  } else if ((tid & 63) < 16) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      if (!SQUARE) tops[wave][8 * l + e] = col_top[e];
-      if (part) sums[wave][8 * l + e] = col_sum[e];
-    }
+    for (int k = 0; k < Tops<T>::kWords; ++k) tops[wave][k][l] = col_top.word(k);
   }
   __syncthreads();
   Fp8Scale all;
   if constexpr (SQUARE) all = fp8_scale(max(max(top_of_all[0], top_of_all[1]), max(top_of_all[2], top_of_all[3])));
-  if (part && tid < kFp8Block && col_tile * kFp8Block + tid < cols)
-    part[row_tile * cols + col_tile * kFp8Block + tid] = (sums[0][tid] + sums[1][tid]) + (sums[2][tid] + sums[3][tid]);
+  if (part && tid < kFp8Block && col_tile * kFp8Block + tid < cols) {
+    const int at = 16 * (tid & 7) + (tid >> 3);
+    part[row_tile * cols + col_tile * kFp8Block + tid] = (sums[0][at] + sums[1][at]) + (sums[2][at] + sums[3][at]);
+  }
+  if (!SQUARE && qt && tid < 16) {
+    // the columns' scales, once: 8 of them per thread of 16
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+#pragma unroll
+      for (int k = 0; k < Tops<T>::kWords; ++k) col_top.take_word(k, tops[w][k][l]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const Fp8Scale s = fp8_scale(col_top.bits(e));
+      inverse[16 * e + l] = s.i;
+      if (e < n) scales_t[row_tile * fp8_scale_pitch(cols) + col + e] = s.s;
+    }
+  }
   const int64_t pitch = fp8_pitch(cols), row_tiles = fp8_blocks(rows);
   if (q) {
 #pragma unroll
@@ -106,19 +170,15 @@ __global__ __launch_bounds__(256) void fp8_tile_kernel(const T* __restrict__ x, 
     if (SQUARE && tid == 0) scales[row_tile * tiles + col_tile] = all.s;
   }
   if (!qt) return;
+  if (!SQUARE) __syncthreads();
   // Column 8 l + e of the tile as row of `turned`, its rows 8 g .. 8 g + 7 as 8 bytes in place g ^ l (of 16): the 64 lanes of a wave
   // write to, and 16 bytes later read from, all banks alike.
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const int c = 8 * l + e;
-    Fp8Scale s;
-    if constexpr (SQUARE) s = all;
-    else s = fp8_scale(max(max(tops[0][c], tops[1][c]), max(tops[2][c], tops[3][c])));
     f32x8 t;
 #pragma unroll
     for (int p = 0; p < 8; ++p) t[p] = v[p][e];
-    *reinterpret_cast<u32x2_t*>(turned + c * kFp8Block + ((g ^ l) << 3)) = fp8_pack8(t, s.i);
-    if (!SQUARE && g == 0 && e < n) scales_t[row_tile * fp8_scale_pitch(cols) + col + e] = s.s;
+    *reinterpret_cast<u32x2_t*>(turned + (8 * l + e) * kFp8Block + ((g ^ l) << 3)) = fp8_pack8(t, SQUARE ? all.i : inverse[16 * e + l]);
   }
   if (SQUARE && tid == 0) scales_t[(int64_t)col_tile * row_tiles + row_tile] = all.s;
   __syncthreads();

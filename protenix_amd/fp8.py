@@ -61,8 +61,15 @@ class Fp8Tensor:
 
     @property
     def scales(self) -> torch.Tensor:
-        _, scales, rows, _, square = self._operand
-        return scales if square else scales.t()[:rows].view(*self.shape[:-1], scales.shape[0])
+        _, scales, _, _, square = self._operand
+        if square:
+            return scales
+        # (one strided view: [blocks, rows and a few] as [*, blocks])
+        strides, step = [scales.stride(0)], 1
+        for n in reversed(self.shape[:-1]):
+            strides.append(step)
+            step *= n
+        return scales.as_strided((*self.shape[:-1], scales.shape[0]), strides[::-1])
 
     @property
     def square(self) -> bool:
