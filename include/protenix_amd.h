@@ -682,10 +682,10 @@ PTX_API int ptx_fp8_quantize(const void* x, void* q, float* scales, void* qt, fl
  * out [m][n] (out_dtype) = a b^T + bias: a [m][k] with a scale per 128 values of a row, b [n][k] with the same or, b_square, with
  * one per 128 x 128; products of a block and sums over blocks in fp32, in a fixed order, rounded once.
  *   bias       [n], bias_dtype, or NULL
- *   workspace  ptx_fp8_matmul_workspace_elems(m, n, k, b_square) fp32 elements, uninitialised (none: NULL)
- * 0 < k < 2^22, (m / 64 + 1) (n / 64 + 1) < 2^23.
+ *   workspace  ptx_fp8_matmul_workspace_elems(m, n, k, b_square, out_dtype) fp32 elements, uninitialised (none: NULL)
+ * 0 < k <= 2^24, (m / 64 + 1) (n / 64 + 1) < 2^23.
  */
-PTX_API int64_t ptx_fp8_matmul_workspace_elems(int64_t m, int64_t n, int64_t k, int b_square);
+PTX_API int64_t ptx_fp8_matmul_workspace_elems(int64_t m, int64_t n, int64_t k, int b_square, int out_dtype);
 PTX_API int ptx_fp8_matmul(const void* a, const float* a_scales, const void* b, const float* b_scales, int b_square,
                            const void* bias, void* out, float* workspace, int64_t m, int64_t n, int64_t k,
                            int out_dtype, int bias_dtype, void* stream);

@@ -108,7 +108,7 @@ SIGNATURES = {
     "ptx_fp8_scale_elems": (_l, [_l, _l, _i]),
     "ptx_fp8_col_sums_workspace_elems": (_l, [_l, _l]),
     "ptx_fp8_quantize": (_i, [_p] * 7 + [_l, _l, _i, _i, _i, _p]),
-    "ptx_fp8_matmul_workspace_elems": (_l, [_l, _l, _l, _i]),
+    "ptx_fp8_matmul_workspace_elems": (_l, [_l, _l, _l, _i, _i]),
     "ptx_fp8_matmul": (_i, [_p] * 4 + [_i] + [_p] * 3 + [_l, _l, _l, _i, _i, _p]),
     "ptx_add_rms_norm_fwd": (_i, [_p] * 7 + [_l, _i, _f, _i, _i, _i, _p]),
     "ptx_add_rms_norm_bwd_workspace_elems": (_l, [_l, _i]),

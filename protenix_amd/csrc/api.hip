@@ -1344,8 +1344,8 @@ PTX_API int ptx_fp8_quantize(const void* x, void* q, float* scales, void* qt, fl
   return after_launch("fp8_quantize");
 }
 
-PTX_API int64_t ptx_fp8_matmul_workspace_elems(int64_t m, int64_t n, int64_t k, int b_square) {
-  return ptx::fp8_matmul_workspace_elems(m, n, ptx::fp8_blocks(k), b_square != 0);
+PTX_API int64_t ptx_fp8_matmul_workspace_elems(int64_t m, int64_t n, int64_t k, int b_square, int out_dtype) {
+  return ptx::fp8_matmul_workspace_elems(m, n, ptx::fp8_blocks(k), b_square != 0, out_dtype == PTX_F32);
 }
 
 PTX_API int ptx_fp8_matmul(const void* a, const float* a_scales, const void* b, const float* b_scales, int b_square, const void* bias,
@@ -1354,13 +1354,13 @@ PTX_API int ptx_fp8_matmul(const void* a, const float* a_scales, const void* b, 
               bias_dtype);
   PTX_REQUIRE(m >= 0 && n >= 0 && k > 0, PTX_ERR_BAD_ARG, "fp8_matmul: m=%lld n=%lld k=%lld", (long long)m, (long long)n, (long long)k);
   // (a launch has fewer than 2^32 threads, 512 per tile at most, and a tile's rows are addressed in 32 bits)
-  PTX_REQUIRE(m < 0x7fffff00 && n < 0x7fffff00 && k < 1 << 22 && (double)(m / 64 + 1) * (double)(n / 64 + 1) < 8388608.0,
+  PTX_REQUIRE(m < 0x7fffff00 && n < 0x7fffff00 && k <= 1 << 24 && (double)(m / 64 + 1) * (double)(n / 64 + 1) < 8388608.0,
               PTX_ERR_UNSUPPORTED, "fp8_matmul: m=%lld n=%lld k=%lld is too large", (long long)m, (long long)n, (long long)k);
   if (m == 0 || n == 0) return PTX_OK;
   PTX_REQUIRE(a && a_scales && b && b_scales && out, PTX_ERR_BAD_ARG, "fp8_matmul: null pointer");
   PTX_REQUIRE(aligned16(a) && aligned16(b) && aligned16(a_scales) && aligned16(b_scales), PTX_ERR_BAD_ARG,
               "fp8_matmul: values and scales must be 16-byte aligned");
-  PTX_REQUIRE(workspace || ptx_fp8_matmul_workspace_elems(m, n, k, b_square) == 0, PTX_ERR_BAD_ARG, "fp8_matmul: needs the workspace");
+  PTX_REQUIRE(workspace || ptx_fp8_matmul_workspace_elems(m, n, k, b_square, out_dtype) == 0, PTX_ERR_BAD_ARG, "fp8_matmul: needs the workspace");
   PTX_DISPATCH_LN(out_dtype, ptx::fp8_matmul<T>(a, a_scales, b, b_scales, b_square != 0, bias, bias_dtype, (T*)out, workspace, (int)m, (int)n,
                                                 (int)ptx::fp8_blocks(k), (hipStream_t)stream));
   return after_launch("fp8_matmul");

@@ -458,24 +458,45 @@ __global__ __launch_bounds__(512) void fp8_few_rows_product(Fp8Args p) {
 
 // ---- which kernel ---------------------------------------------------------------------------------------
 namespace {
+// The tile kernels, as (tile; workgroups that the 256 compute units hold at once; what a round of these takes per block of k, in units of 10 ns,
+// with 16-bit and with fp32 results).  The one whose rounds take least is chosen.  us at k = 4096, in the order below (the fifth without
+// fp32): 1024 x 1024 12.0 / 16.6 / 22.9 / 41.6, 1280^2 22.0 / 19.0 / 22.9, 1536^2 32.6 / 32.3 / 23.4 / 41.8, 2048^2 - / - / 26.4 / 44.7 / 38.1 /
+// 50.4, 2560^2 - / - / 46.6 / 48.9 / 38.5 / 50.5, 3328^2 68.5 / 83.1 / 72.3 / 51.3 for the last four, 4608^2 135 / 136 / 114 / 106; fp32 1024^2 16.6 /
+// 20.6 / 31.7, 1536^2 46.8 / 44.3 / 33.3 / 44.8, 2560^2 66 / 68, 4096^2 141 / 138 for the two of 128 x 128.
+enum Fp8Kernel { kFewRows, k64Deep, k64Pair, k128Split, k128Pair, k256x128, k256 };
+struct Fp8Shape {
+  Fp8Kernel kernel;
+  int tm, tn, at_once, cost16, cost32;
+};
+constexpr Fp8Shape kFp8Shapes[] = {{k64Deep, 64, 64, 256, 36, 50},     {k64Pair, 64, 64, 512, 55, 75},      {k128Split, 128, 128, 256, 72, 100},
+                                   {k128Pair, 128, 128, 512, 138, 145}, {k256x128, 256, 128, 256, 119, 210}, {k256, 256, 256, 256, 157, 0}};
 struct Fp8Plan {
-  int tile;      // 0: few rows, else 64, 128 or 256
+  Fp8Kernel kernel;
   int splits;
 };
-Fp8Plan fp8_plan(int64_t m, int64_t n, int64_t blocks, bool square) {
-  if (m <= 16 && square) return {0, 1};
-  auto tiles = [&](int t) { return ((m + t - 1) / t) * ((n + t - 1) / t); };
-  // (not where more than a third of the large tiles would lie beyond the end)
-  if (tiles(256) >= 192 && 3 * m * n >= 2 * 65536 * tiles(256)) return {256, 1};
-  if (tiles(128) >= 192) return {128, 1};
-  int splits = 1;
-  while (splits < 8 && tiles(64) * splits <= 128 && blocks / (2 * splits) >= 4) splits *= 2;
-  return {64, splits};
+Fp8Plan fp8_plan(int64_t m, int64_t n, int64_t blocks, bool square, bool wide) {
+  // (16 x 4096 x 4096 7.2 us, as tiles 9.9; 16 x 8192 x 1024 9.5 and 9.3)
+  if (m <= 16 && square) return {kFewRows, 1};
+  auto tiles = [&](int tm, int tn) { return ((m + tm - 1) / tm) * ((n + tn - 1) / tn); };
+  Fp8Plan best{k64Deep, 1};
+  int64_t least = INT64_MAX;
+  for (const Fp8Shape& s : kFp8Shapes) {
+    const int64_t cost = (tiles(s.tm, s.tn) + s.at_once - 1) / s.at_once * (wide ? s.cost32 : s.cost16);
+    if (cost > 0 && cost < least) {
+      least = cost;
+      best.kernel = s.kernel;
+    }
+  }
+  // Few small tiles share the sum over k with one another, as many as fill the machine and leave each 8 blocks (64 x 4096 x 2048 with 1, 2, 4, 8
+  // parts 11.4, 10.0, 9.0, 10.7 us; 512 x 147456 x 128 with 1, 8, 16, 32 306, 49, 41, 48).
+  if (best.kernel == k64Deep)
+    while (best.splits < 64 && tiles(64, 64) * 2 * best.splits <= 256 && blocks / (2 * best.splits) >= 8) best.splits *= 2;
+  return best;
 }
 }  // namespace
 
-int64_t fp8_matmul_workspace_elems(int64_t m, int64_t n, int64_t blocks, bool square) {
-  const Fp8Plan plan = fp8_plan(m, n, blocks, square);
+int64_t fp8_matmul_workspace_elems(int64_t m, int64_t n, int64_t blocks, bool square, bool wide) {
+  const Fp8Plan plan = fp8_plan(m, n, blocks, square, wide);
   return plan.splits > 1 ? plan.splits * m * n : 0;
 }
 
@@ -492,28 +513,21 @@ template <int TM, int TN, int WM, int WN, int WK, int NB, typename O> static voi
 template <typename O>
 int fp8_matmul(const void* a, const float* sa, const void* b, const float* sb, bool square, const void* bias, int bias_type, O* out,
                float* workspace, int m, int n, int blocks, hipStream_t stream) {
-  const Fp8Plan plan = fp8_plan(m, n, blocks, square);
+  const Fp8Plan plan = fp8_plan(m, n, blocks, square, sizeof(O) == 4);
   Fp8Args p{(const uint8_t*)a, sa, (const uint8_t*)b, sb, bias, bias_type, out, m, n, blocks, 0, 0, plan.splits};
-  if (plan.tile == 0) {
-    fp8_few_rows_product<O><<<dim3((n + 15) / 16), dim3(512), 0, stream>>>(p);
-    return 0;
-  }
   if (plan.splits > 1) {
     p.out = workspace;
     p.bias = nullptr;
   }
-  const int64_t tiles = (int64_t)((m + plan.tile - 1) / plan.tile) * ((n + plan.tile - 1) / plan.tile);
-  if (plan.tile == 256) {
-    // (fp32 results have widened fragments, twice the registers)
-    if constexpr (sizeof(O) == 4) tile_product<256, 128, 4, 2, 1, 2, O>(p, square, stream);
-    else tile_product<256, 256, 2, 4, 1, 2, O>(p, square, stream);
-  } else if (plan.tile == 128) {
-    if (tiles >= 512) tile_product<128, 128, 2, 2, 1, 2, O>(p, square, stream);
-    else tile_product<128, 128, 2, 2, 2, 2, O>(p, square, stream);
-  } else if (tiles * plan.splits > 256) {
-    tile_product<64, 64, 4, 1, 2, 2, O>(p, square, stream);
-  } else {
-    tile_product<64, 64, 4, 1, 2, 4, O>(p, square, stream);
+  switch (plan.kernel) {
+    case kFewRows: fp8_few_rows_product<O><<<dim3((n + 15) / 16), dim3(512), 0, stream>>>(p); break;
+    case k64Deep: tile_product<64, 64, 4, 1, 2, 4, O>(p, square, stream); break;
+    case k64Pair: tile_product<64, 64, 4, 1, 2, 2, O>(p, square, stream); break;
+    case k128Split: tile_product<128, 128, 2, 2, 2, 2, O>(p, square, stream); break;
+    case k128Pair: tile_product<128, 128, 2, 2, 1, 2, O>(p, square, stream); break;
+    case k256x128: tile_product<256, 128, 4, 2, 1, 2, O>(p, square, stream); break;
+    case k256:      // (fp32 results have widened fragments, twice the registers)
+      if constexpr (sizeof(O) == 2) tile_product<256, 256, 2, 4, 1, 2, O>(p, square, stream);
   }
   if (plan.splits > 1) {
     const int64_t count = (int64_t)m * n;

@@ -1505,7 +1505,7 @@ void fp8_quantize_call(const Tensor& x, int64_t rows, bool square, Fp8Operand* q
 }
 Tensor fp8_matmul_call(const Fp8Operand& a, const Fp8Operand& b, const Tensor& bias, at::ScalarType type, at::IntArrayRef shape) {
   Tensor out = at::empty(shape, a.values.options().dtype(type)), ws;
-  const int64_t elems = ptx_fp8_matmul_workspace_elems(a.rows, b.rows, a.cols, b.square);
+  const int64_t elems = ptx_fp8_matmul_workspace_elems(a.rows, b.rows, a.cols, b.square, code_of(type));
   if (elems) ws = at::empty({elems}, out.options().dtype(at::kFloat));
   check(ptx_fp8_matmul(ptr(a.values), (const float*)ptr(a.scales), ptr(b.values), (const float*)ptr(b.scales), b.square, ptr(bias), ptr(out),
                        (float*)ptr(ws), a.rows, b.rows, a.cols, code_of(type), bias.defined() ? code_of(bias.scalar_type()) : PTX_F32,

@@ -266,7 +266,7 @@ template <typename T>
 int fp8_quantize(const T* x, void* q, float* scales, void* qt, float* scales_t, float* part, int64_t rows, int cols, bool square,
                  hipStream_t stream);
 // out [m][n] = a b^T (+ bias) of such operands of `blocks` blocks; square: b's scales.  workspace: fp8_matmul_workspace_elems() floats.
-int64_t fp8_matmul_workspace_elems(int64_t m, int64_t n, int64_t blocks, bool square);
+int64_t fp8_matmul_workspace_elems(int64_t m, int64_t n, int64_t blocks, bool square, bool wide);      // wide: fp32 results
 template <typename O>
 int fp8_matmul(const void* a, const float* sa, const void* b, const float* sb, bool square, const void* bias, int bias_type, O* out,
                float* workspace, int m, int n, int blocks, hipStream_t stream);

@@ -846,7 +846,7 @@ def fp8_matmul(a: tuple, b: tuple, bias: Optional[torch.Tensor], dtype: torch.dt
         out = torch.zeros((m, n), dtype=dtype, device=a[0].device)
         return out if bias is None else out + bias.to(dtype)
     out = torch.empty((m, n), dtype=dtype, device=a[0].device)
-    elems = lib.ptx_fp8_matmul_workspace_elems(m, n, k, int(b[4]))
+    elems = lib.ptx_fp8_matmul_workspace_elems(m, n, k, int(b[4]), _dt_ln(out))
     ws = _workspace((elems,), torch.float32, out.device) if elems else None
     with torch.cuda.device(out.device):
         _call("fp8_matmul", lib.ptx_fp8_matmul, _ptr(a[0]), _ptr(a[1]), _ptr(b[0]), _ptr(b[1]), int(b[4]), _ptr(bias), _ptr(out), _ptr(ws),

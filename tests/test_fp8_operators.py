@@ -23,7 +23,7 @@ def test_sizes():
     assert [lib.ptx_fp8_pitch(n) for n in (1, 128, 129)] == [128, 128, 256]
     assert [lib.ptx_fp8_scale_pitch(n) for n in (1, 4, 5)] == [4, 4, 8]
     assert lib.ptx_fp8_scale_elems(5, 129, 0) == 16 and lib.ptx_fp8_scale_elems(129, 129, 1) == 4
-    assert lib.ptx_fp8_matmul_workspace_elems(1, 4096, 4096, 1) == 0
+    assert lib.ptx_fp8_matmul_workspace_elems(1, 4096, 4096, 1, 1) == 0
     assert lib.ptx_add_rms_norm_bwd_workspace_elems(0, 128) == 0 and lib.ptx_add_rms_norm_bwd_workspace_elems(10, 128) >= 128
 
 
@@ -46,9 +46,9 @@ def test_c_refusals():
     assert matmul(out_dtype=2) == 1 and matmul(bias=16, bias_dtype=5) == 1 and matmul(m=-1) == 1 and matmul(n=-1) == 1 and matmul(k=0) == 1
     assert all(matmul(**{name: None}) == 1 for name in ("a", "sa", "b", "sb", "out"))
     assert all(matmul(**{name: 8}) == 1 for name in ("a", "sa", "b", "sb"))
-    assert matmul(k=1 << 22) == 2 and matmul(m=1 << 31) == 2 and matmul(m=1 << 20, n=1 << 20) == 2
+    assert matmul(k=(1 << 24) + 1) == 2 and matmul(m=1 << 31) == 2 and matmul(m=1 << 20, n=1 << 20) == 2
     assert matmul(m=0) == 0 and matmul(n=0) == 0
-    if lib.ptx_fp8_matmul_workspace_elems(70, 128, 8192, 1):
+    if lib.ptx_fp8_matmul_workspace_elems(70, 128, 8192, 1, 1):
         assert matmul(m=70, n=128, k=8192) == 1 and b"workspace" in lib.ptx_last_error_string()
 
     def norm(x=16, r=16, w=None, y=16, s=None, h=16, rows=4, cols=8, tx=1, ts=1, tw=0):

@@ -110,7 +110,8 @@ def test_blocks_that_are_not_finite_stay_that(bad):
 # rows of a on both sides of the kernels' borders (16 rows at a time up to 64, tiles of 64, 128, 256), odd columns and blocks
 PRODUCTS = [(1, 128, 16), (1, 2048, 1000), (2, 100, 17), (15, 384, 130), (16, 1000, 128), (17, 130, 64), (33, 1, 1), (48, 129, 200),
             (64, 640, 257), (65, 640, 257), (65, 64, 3), (100, 4096, 72), (128, 128, 128), (200, 8200, 136), (257, 513, 300),
-            (1035, 1000, 777), (1536, 256, 1792), (4100, 128, 520), (3000, 130, 4100)]
+            (1035, 1000, 777), (1536, 256, 1792), (4100, 128, 520), (3000, 130, 4100), (40, 150001, 70),
+            (130, 20000, 17), (1300, 300, 1290), (1600, 200, 1500), (2500, 129, 2600)]
 
 
 def _check_product(got, a, b, bias=None):
@@ -285,7 +286,7 @@ def test_rows_behind_the_last_are_left_alone():
     for m, n, k in ((5, 21, 130), (70, 130, 300), (300, 300, 300)):
         a, b = P.quantize_fp8(_matrix(m, k, BF16)), P.quantize_fp8(_matrix(n, k, BF16, 1), square=True)
         room = torch.full((m * n + 512,), 7.0, device=dev)
-        ws = torch.empty((max(lib.ptx_fp8_matmul_workspace_elems(m, n, k, 1), 1),), device=dev)
+        ws = torch.empty((max(lib.ptx_fp8_matmul_workspace_elems(m, n, k, 1, 0), 1),), device=dev)
         ops._lib.check(lib.ptx_fp8_matmul(a._operand[0].data_ptr(), a._operand[1].data_ptr(), b._operand[0].data_ptr(), b._operand[1].data_ptr(),
                                           1, None, room.data_ptr() + 4 * 256, ws.data_ptr(), m, n, k, 0, 0, ops._stream()), "matmul")
         assert (room[:256] == 7).all() and (room[256 + m * n:] == 7).all()
