@@ -99,10 +99,18 @@ __device__ __forceinline__ void tile_of(uint32_t id, int tiles_m, int tiles_n, i
   tn = (int)(in / high);
 }
 
-// Tiles of TM x TN, WM x WN waves of TM / WM x 64 each.  Both operands' 128 columns of a block go to LDS (direct loads into a ring of NB
-// buffers: NB - 1 blocks are on their way or there while one is multiplied), rows of 128 bytes whose 16-byte pieces lie at place piece ^ (row % 8).  Rows of b
-// lie in LDS so that what a wave stores at a time are runs of 64 bytes: with 16-bit results row 16 u + i of 64 holds
-// n = 32 (u / 2) + 8 (i / 4) + 4 (u % 2) + i % 4, and a lane's results of two MFMAs are 8 neighbours; with fp32 ones n = 16 u + i.
+// Tiles of TM x TN, WM x WN waves of TM / WM x 64 each, and WK such groups of waves that share the blocks of k and add their sums in LDS.
+// Both operands' 128 columns of a block go to LDS (direct loads into a ring of NB buffers: NB - 1 blocks are on their way or there
+// while one is multiplied), rows of 128 bytes whose 16-byte pieces lie at place piece ^ (row % 8): no bank conflicts.  Rows of b lie in LDS so
+// that what a wave stores at a time are runs of 64 bytes: with 16-bit results row 16 u + i of 64 holds
+// n = 32 (u / 2) + 8 (i / 4) + 4 (u % 2) + i % 4, and a lane's results of two MFMAs are 8 neighbours; with fp32 ones n = 16 u + i
+// (147456 x 128 x 512 in fp32 112 -> 84 us).
+//
+// 256 x 256, which takes what is large: 256 x 256 is the most that 256 registers a lane hold the sums of (128) with two waves per SIMD, whose
+// vector work then hides behind each other's MFMAs, and two buffers of both operands fill the LDS.  8192^3 in 455 us (2.42 PFLOP/s),
+// 8192 x 4096 x 8192 in 245 (2.24), with scales per row of both operands (twice the vector work) 527 and 278.  The MFMAs are
+// busy 60 % of the time at 1.91 GHz; a product without scales per block reaches 84 % at 1.67 GHz (375 us), so that what bounds
+// both is power.  Without its loads this kernel takes 382 us, with loads from the L1 408, from the L2 430; without the scales' vector work 421.
 template <int TM, int TN, int WM, int WN, int NB, bool PAIRS> struct Fp8Tile {
   static constexpr int W = WM * WN, MT = TM / WM / 16;
   static constexpr int kSa = 0, kSb = 1024, kB = 2048, kA = kB + TN * 128, kStage = kA + TM * 128;
@@ -253,8 +261,8 @@ __global__ __launch_bounds__(64 * WM * WN * WK, TM == 64 && NB == 2 && !(ROWB &&
         sa = read_s(st, t + 1);
       }
       if constexpr (loads.value) {
-        // (as many as end by half of the row tiles)
-        constexpr int EACH = (C::PER + 1 + (C::MT + 1) / 2 - 1) / ((C::MT + 1) / 2);
+        // (as many at a time as end by half of the row tiles; two or three of nine make no difference, all at once 2 to 5 % more)
+        constexpr int HALF = (C::MT + 1) / 2, EACH = (C::PER + HALF) / HALF;
         if (loading)
 #pragma unroll
           for (int j = EACH * t; j < EACH * (t + 1); ++j)
@@ -293,90 +301,90 @@ __global__ __launch_bounds__(64 * WM * WN * WK, TM == 64 && NB == 2 && !(ROWB &&
   // while the next one's first is loaded, and its results are stored while that is on its way.
   constexpr bool WALKS = WK == 1 && NB == 2;
   for (;;) {
-  const int m0 = from.m0, n0 = from.n0;
-  int step = 0;
-  for (; step + NB - 1 < steps; ++step) multiply(step + NB - 1, true, std::true_type{}, std::true_type{});
-  if constexpr (NB > 2)
-    for (; step + 1 < steps; ++step) multiply(0, false, std::false_type{}, std::true_type{});
-  tile += gridDim.x;
-  const bool more = WALKS && tile < (uint32_t)p.tiles_m * p.tiles_n;
-  if (more) from = place(tile);
-  if (WK == 1 || first + step < last) multiply(0, more, std::integral_constant<bool, WALKS>{}, std::false_type{});
-  if constexpr (!ROWB) {
+    const int m0 = from.m0, n0 = from.n0;
+    int step = 0;
+    for (; step + NB - 1 < steps; ++step) multiply(step + NB - 1, true, std::true_type{}, std::true_type{});
+    if constexpr (NB > 2)
+      for (; step + 1 < steps; ++step) multiply(0, false, std::false_type{}, std::true_type{});
+    tile += gridDim.x;
+    const bool more = WALKS && tile < (uint32_t)p.tiles_m * p.tiles_n;
+    if (more) from = place(tile);
+    if (WK == 1 || first + step < last) multiply(0, more, std::integral_constant<bool, WALKS>{}, std::false_type{});
+    if constexpr (!ROWB) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[C::MT - 1][u][r] = __builtin_fmaf(d[u][r], s_before, acc[C::MT - 1][u][r]);
+    }
+    if constexpr (WK > 1) {
+      // the groups' sums, added in their order
+      f32x4* sums = reinterpret_cast<f32x4*>(lds_all) + wave * C::MT * 4 * kWave + lane;
+      __syncthreads();
+      if (group > 0)
+#pragma unroll
+        for (int t = 0; t < C::MT; ++t)
+#pragma unroll
+          for (int u = 0; u < 4; ++u) sums[((group - 1) * C::W * C::MT * 4 + 4 * t + u) * kWave] = acc[t][u];
+      __syncthreads();
+      if (group > 0) return;
+#pragma unroll
+      for (int g = 0; g < WK - 1; ++g)
+#pragma unroll
+        for (int t = 0; t < C::MT; ++t)
+#pragma unroll
+          for (int u = 0; u < 4; ++u) acc[t][u] += sums[(g * C::W * C::MT * 4 + 4 * t + u) * kWave];
+    }
+    const int n = n0 + 64 * wn;
+    f32x4 bias[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) acc[C::MT - 1][u][r] = __builtin_fmaf(d[u][r], s_before, acc[C::MT - 1][u][r]);
-  }
-  if constexpr (WK > 1) {
-    // the groups' sums, added in their order
-    f32x4* sums = reinterpret_cast<f32x4*>(lds_all) + wave * C::MT * 4 * kWave + lane;
-    __syncthreads();
-    if (group > 0)
+      for (int r = 0; r < 4; ++r) {
+        const int c = n + C::col(u, q) + r;
+        bias[u][r] = p.bias && c < p.n ? param_at(p.bias, p.bias_type, c) : 0.0f;
+      }
 #pragma unroll
-      for (int t = 0; t < C::MT; ++t)
+    for (int t = 0; t < C::MT; ++t) {
+      const int m = m0 + row0 + 16 * t + i;
+      if (m >= p.m) continue;
+      if (p.splits > 1) {
+        float* row = (float*)p.out + ((int64_t)split * p.m + m) * p.n;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) sums[((group - 1) * C::W * C::MT * 4 + 4 * t + u) * kWave] = acc[t][u];
-    __syncthreads();
-    if (group > 0) return;
-#pragma unroll
-    for (int g = 0; g < WK - 1; ++g)
-#pragma unroll
-      for (int t = 0; t < C::MT; ++t)
-#pragma unroll
-        for (int u = 0; u < 4; ++u) acc[t][u] += sums[(g * C::W * C::MT * 4 + 4 * t + u) * kWave];
-  }
-  const int n = n0 + 64 * wn;
-  f32x4 bias[4];
-#pragma unroll
-  for (int u = 0; u < 4; ++u)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int c = n + C::col(u, q) + r;
-      bias[u][r] = p.bias && c < p.n ? param_at(p.bias, p.bias_type, c) : 0.0f;
-    }
-#pragma unroll
-  for (int t = 0; t < C::MT; ++t) {
-    const int m = m0 + row0 + 16 * t + i;
-    if (m >= p.m) continue;
-    if (p.splits > 1) {
-      float* row = (float*)p.out + ((int64_t)split * p.m + m) * p.n;
-#pragma unroll
-      for (int u = 0; u < 4; ++u) store4(row, n + C::col(u, q), p.n, acc[t][u]);
-    } else {
-      O* row = (O*)p.out + (int64_t)m * p.n;
-      if (sizeof(O) == 2 && n + 64 <= p.n) {
-#pragma unroll
-        for (int u = 0; u < 4; u += 2) {
-          f32x8 v;
-#pragma unroll
-          for (int r = 0; r < 8; ++r) v[r] = acc[t][u + r / 4][r % 4] + bias[u + r / 4][r % 4];
-          store_cols(row + n + C::col(u, q), v, 8);
-        }
+        for (int u = 0; u < 4; ++u) store4(row, n + C::col(u, q), p.n, acc[t][u]);
       } else {
+        O* row = (O*)p.out + (int64_t)m * p.n;
+        if (sizeof(O) == 2 && n + 64 <= p.n) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) store4(row, n + C::col(u, q), p.n, acc[t][u] + bias[u]);
+          for (int u = 0; u < 4; u += 2) {
+            f32x8 v;
+#pragma unroll
+            for (int r = 0; r < 8; ++r) v[r] = acc[t][u + r / 4][r % 4] + bias[u + r / 4][r % 4];
+            store_cols(row + n + C::col(u, q), v, 8);
+          }
+        } else {
+#pragma unroll
+          for (int u = 0; u < 4; ++u) store4(row, n + C::col(u, q), p.n, acc[t][u] + bias[u]);
+        }
       }
     }
-  }
-  if (!more) break;
-  // the next tile's first block has landed: all but what was issued behind its loads, which is a whole tile's stores, 16 bytes a lane each,
-  // or may be fewer at an edge
-  if (m0 + TM <= p.m && n0 + TN <= p.n) meet(none, std::integral_constant<int, C::MT * 4 * 4 * (int)sizeof(O) / 16>{});
-  else meet(none, none);
-  buf ^= 1;
-  const uint8_t* st = lds + buf * C::kStage;
-  fb = read_b(st);
-  fa = read_a(st, 0);
-  sa = read_s(st, 0);
-  scale_b = read_scale_b(st);
-  s_before = 0.0f;
+    if (!more) break;
+    // the next tile's first block has landed: all but what was issued behind its loads, which is a whole tile's stores, 16 bytes a lane each,
+    // or may be fewer at an edge
+    if (m0 + TM <= p.m && n0 + TN <= p.n) meet(none, std::integral_constant<int, C::MT * 4 * 4 * (int)sizeof(O) / 16>{});
+    else meet(none, none);
+    buf ^= 1;
+    const uint8_t* st = lds + buf * C::kStage;
+    fb = read_b(st);
+    fa = read_a(st, 0);
+    sa = read_s(st, 0);
+    scale_b = read_scale_b(st);
+    s_before = 0.0f;
 #pragma unroll
-  for (int u = 0; u < 4; ++u) d[u] = f32x4{};
+    for (int u = 0; u < 4; ++u) d[u] = f32x4{};
 #pragma unroll
-  for (int t = 0; t < C::MT; ++t)
+    for (int t = 0; t < C::MT; ++t)
 #pragma unroll
-    for (int u = 0; u < 4; ++u) acc[t][u] = f32x4{};
+      for (int u = 0; u < 4; ++u) acc[t][u] = f32x4{};
   }
 }
 

@@ -4,6 +4,9 @@
 // Bound by memory: an element is read once and written once per direction.  Rows alone: 16 lanes hold a block in registers.  Else
 // a workgroup holds a tile of 128 x 128 in its registers, 8 x 8 per thread, takes the largest magnitudes of its rows among 16 lanes
 // and of its columns through LDS, and turns the bytes round in LDS, from where the transposed rows go out in whole lines of 128 bytes.
+// 16384 x 4096 bf16 both ways 49 us on the same tensors again (5.5 TB/s, a plain copy's rate; 59 where they come from HBM among other
+// passes), its rows alone 39 (5.3); 8192 x 4096 square both ways 26.  Tiles in one run per XCD instead of round them take 51 - 56 us, loads past
+// the caches 49 - 55.
 #include "fp8.h"
 #include "dropout.h"
 #include "kernels.h"
