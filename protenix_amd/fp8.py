@@ -191,11 +191,13 @@ def linear_fp8(x: Operand, weight: Operand, bias: Optional[torch.Tensor] = None,
     forward-mode is refused).
 
     x, weight: float32, bfloat16 or float16 tensors, each of its own type, or `Fp8Tensor`s (in use without gradients: a weight laid out
-    once by `quantize_fp8(weight, square=True)`, what `add_rms_norm(quantize=True)` left of x).  dtype: of the result (x's by
-    default, bfloat16 for x in 8 bits).
+    once by `quantize_fp8(weight, square=True)`, what `add_rms_norm(quantize=True)` left of x).  dtype: of the result (by
+    default x's, or for float32 x under torch.autocast that one's; bfloat16 for x in 8 bits).
     Training: x and dy in blocks of 128 along the axis each product sums over, the weight in blocks of 128 x 128; dx = dy W and
     dW = dy^T x are products of such operands too, with the rounding to 8 bits taken as the identity, and db is summed in fp32,
     in a fixed order.  Gradients have their inputs' types.  Neither x nor the weight is kept, only their 8-bit forms."""
+    if dtype is None and isinstance(x, torch.Tensor):
+        dtype = ops.autocast_compute_dtype(x)      # (as `Linear`: for fp32 x under torch.autocast its type)
     if ops.use_native_operators() and isinstance(x, torch.Tensor):
         out = None
         if isinstance(weight, torch.Tensor):

@@ -206,6 +206,17 @@ def test_linear_of_batches_and_strides():
     assert torch.equal(g, torch.autograd.grad(P.linear_fp8(x, w), x, torch.ones_like(dy))[0])
 
 
+def test_linear_under_autocast():
+    x, w, b, dy = _train(30, 200, 60, F32, F32, F32)
+    for dtype in (BF16, F16):
+        with torch.autocast("cuda", dtype=dtype):
+            y = P.linear_fp8(x, w, b)
+            assert y.dtype == dtype and P.linear_fp8(x.to(BF16), w).dtype == BF16
+            assert P.linear_fp8(x, w, b, dtype=F32).dtype == F32
+        assert torch.equal(y, P.linear_fp8(x, w, b, dtype=dtype))
+        assert [g.dtype for g in torch.autograd.grad(y, (x, w, b), dy.to(dtype))] == [F32] * 3
+
+
 def test_linear_frozen_inputs():
     x, w, b, dy = _train(150, 200, 130, tb=F32)
     full = torch.autograd.grad(P.linear_fp8(x, w, b), (x, w, b), dy)
