@@ -484,7 +484,8 @@ struct Fp8Plan {
 };
 Fp8Plan fp8_plan(int64_t m, int64_t n, int64_t blocks, bool square, bool wide) {
   // (16 x 4096 x 4096 7.2 us, as tiles 9.9; 16 x 8192 x 1024 9.5 and 9.3)
-  if (m <= 16 && square) return {kFewRows, 1};
+  // (and a launch has fewer than 2^32 threads: 512 per 16 columns)
+  if (m <= 16 && square && n <= 1 << 26) return {kFewRows, 1};
   auto tiles = [&](int tm, int tn) { return ((m + tm - 1) / tm) * ((n + tn - 1) / tn); };
   Fp8Plan best{k64Deep, 1};
   int64_t least = INT64_MAX;

@@ -1485,8 +1485,7 @@ Fp8Operand operand_of(const OperandTuple& t) { return {std::get<0>(t), std::get<
 Fp8Operand fp8_buffers(int64_t rows, int64_t cols, bool square, const at::TensorOptions& like) {
   const int64_t blocks = (cols + 127) / 128, lead = square ? (rows + 127) / 128 : ptx_fp8_scale_pitch(rows);
   return {at::empty({rows, ptx_fp8_pitch(cols)}, like.dtype(at::kFloat8_e4m3fn)),
-          at::empty(square ? std::initializer_list<int64_t>{lead, blocks} : std::initializer_list<int64_t>{blocks, lead}, like.dtype(at::kFloat)),
-          rows, cols, square};
+          at::empty({square ? lead : blocks, square ? blocks : lead}, like.dtype(at::kFloat)), rows, cols, square};
 }
 // x [.., cols], dense, as a matrix of `rows` rows
 void fp8_quantize_call(const Tensor& x, int64_t rows, bool square, Fp8Operand* q, Fp8Operand* qt, Tensor* sums, at::ScalarType sums_type) {
@@ -1547,6 +1546,8 @@ optional<Tensor> matmul_fp8(const OperandTuple& a_, const OperandTuple& b_, cons
     return c10::nullopt;
   py::gil_scoped_release nogil;
   at::DeviceGuard dev(a.values.device());
+  const Tensor bi = given(bias);
+  refuse_tangents({&bi});
   return fp8_matmul_call(a, b, dense(bias), type, with_last(a_shape, b.rows));
 }
 
@@ -1689,7 +1690,7 @@ struct AddRmsNormFn : torch::autograd::Function<AddRmsNormFn> {
 
 // (y, h), or (an operand, h) with quantize
 py::object add_rms_norm(const Tensor& x, const optional<Tensor>& residual, const optional<Tensor>& weight, double eps, bool quantize) {
-  if (!x.is_cuda() || !float_type(x) || x.dim() < 1 || x.numel() == 0) return py::none();
+  if (!x.is_cuda() || !float_type(x) || x.dim() < 1 || x.numel() == 0 || x.size(-1) > INT32_MAX) return py::none();
   if (residual && (residual->device() != x.device() || residual->sizes() != x.sizes() ||
                    (residual->scalar_type() != x.scalar_type() && residual->scalar_type() != at::kFloat)))
     return py::none();

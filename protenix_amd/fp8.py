@@ -45,7 +45,7 @@ class Fp8Tensor:
             if square:
                 operand[1].copy_(scales)
             else:
-                operand[1][:, :rows] = scales.reshape(rows, -1).t()
+                operand[1][:, :rows] = scales.reshape(rows, scales.shape[-1]).t()
         self._operand, self.shape = operand, torch.Size(values.shape)
 
     @classmethod
@@ -150,6 +150,7 @@ def matmul_fp8(a: Fp8Tensor, b: Fp8Tensor, bias: Optional[torch.Tensor] = None, 
     if a.square:
         raise RuntimeError("a has a scale per 128 values of a row (square scales are b's)")
     _check_bias(bias, b.shape[0], b.device)
+    _refuse_tangents(bias)
     _refuse_wanted(bias)
     bias = None if bias is None else bias.contiguous()
     out = ops.fp8_matmul(a._operand, b._operand, bias, _out_type(dtype))

@@ -54,6 +54,8 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor] = None, weigh
     ops._dt_ln(x)
     if x.dim() < 1 or x.shape[-1] == 0:
         raise RuntimeError(f"a norm over the last dimension of {tuple(x.shape)}")
+    if x.shape[-1] > 16384:      # (here, since a column count travels in 32 bits)
+        raise RuntimeError(f"a norm over at most 16384 columns, got {x.shape[-1]}")
     if residual is not None:
         if residual.device != x.device or residual.shape != x.shape:
             raise RuntimeError(f"x {tuple(x.shape)} on {x.device} and residual {tuple(residual.shape)} on {residual.device} differ")

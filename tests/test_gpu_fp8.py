@@ -1,6 +1,9 @@
 """8-bit blocks and their products against 64-bit forms: layouts, roundings, gradients, sizes on all sides of the tiles."""
+import threading
+
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import protenix_amd as P
 from protenix_amd import ops
@@ -259,6 +262,8 @@ def test_empty_sizes():
     t = P.quantize_fp8(x.detach())
     assert t.values.shape == (0, 200) and t.scales.shape == (0, 2)
     assert P.matmul_fp8(t, P.quantize_fp8(w.detach(), square=True)).shape == (0, 30)
+    again = P.Fp8Tensor(t.values, t.scales)
+    assert again.values.shape == (0, 200) and P.matmul_fp8(again, P.quantize_fp8(w.detach(), square=True)).shape == (0, 30)
 
 
 def test_workspaces_hold_nothing(monkeypatch):
@@ -365,6 +370,97 @@ def test_large_offsets():
     u = P.quantize_fp8(x[:m], along=-2)
     last = P.quantize_fp8(x[m - 128:m].contiguous(), along=-2)
     assert torch.equal(u.values[:, -128:].view(torch.uint8), last.values.view(torch.uint8)) and torch.equal(u.scales[:, -1:], last.scales)
+
+
+def test_more_columns_than_a_launch_has_threads_for():
+    """One row by 2^27 of a weight: 512 threads for 16 columns each would be more than 2^32."""
+    n = (1 << 27) + 70
+    last = P.quantize_fp8(_matrix(256, 128, BF16), square=True)      # (n ends 70 rows behind a block of rows: the last block and the one before)
+    values = torch.zeros((n, 128), dtype=torch.uint8, device="cuda")
+    values[-70 - 128:] = last.values.view(torch.uint8)[:70 + 128]
+    scales = torch.zeros((n // 128 + 1, 1), device="cuda")
+    scales[-2:] = last.scales
+    w = P.Fp8Tensor(values.view(torch.float8_e4m3fn), scales, square=True)
+    del values
+    x = P.quantize_fp8(_matrix(1, 128, BF16, 1))
+    y = P.matmul_fp8(x, w, dtype=F32)
+    short = P.Fp8Tensor(last.values[:70 + 128], last.scales, square=True)
+    _check_product(y[:, -70 - 128:], Q.held_by(x), Q.held_by(short))
+    assert (y[:, :-70 - 128] == 0).all()
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_forward_mode_derivatives_are_refused(native, monkeypatch):
+    monkeypatch.setattr(ops, "native_enabled", native)
+    x, w, b = (torch.randn(s, device="cuda") for s in ((8, 16), (16, 16), (16,)))
+    xq, wq = P.quantize_fp8(x), P.quantize_fp8(w, square=True)
+    calls = [lambda t: P.linear_fp8(t(x), w), lambda t: P.linear_fp8(x, t(w)), lambda t: P.linear_fp8(x, w, t(b)), lambda t: P.linear_fp8(t(x), wq),
+             lambda t: P.linear_fp8(xq, wq, t(b)), lambda t: P.matmul_fp8(xq, wq, t(b)), lambda t: P.add_rms_norm(t(x)),
+             lambda t: P.add_rms_norm(x, t(x)), lambda t: P.add_rms_norm(x, None, t(b)), lambda t: P.add_rms_norm(x, x, t(b), quantize=True)]
+    with forward_ad.dual_level():
+        for f in calls:
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="forward-mode"):
+                    f(lambda t: forward_ad.make_dual(t, torch.ones_like(t)))
+            f(lambda t: t)
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_recorded_gradients_of_a_leaf_that_an_eager_graph_holds_are_refused(native, monkeypatch):
+    monkeypatch.setattr(ops, "native_enabled", native)
+    x, w, g = (torch.randn(s, device="cuda", requires_grad=True) for s in ((8, 16), (16, 16), (16,)))
+    calls = [lambda: P.linear_fp8(x, w.detach()), lambda: P.linear_fp8(x.detach(), w), lambda: P.linear_fp8(x.detach(), w.detach(), g),
+             lambda: P.add_rms_norm(x)[0], lambda: P.add_rms_norm(x.detach(), x)[0], lambda: P.add_rms_norm(x.detach(), None, g)[0]]
+    alive = [f() for f in calls]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for f in calls:
+            with pytest.raises(RuntimeError, match="eager graph that is still alive"):
+                f()
+        with torch.no_grad():      # (nothing to accumulate: taken)
+            out = [f() for f in calls]
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, alive))
+
+
+def test_threads():
+    x, w, b, dy = _train(130, 384, 520, tb=F32)
+    gain = torch.ones(384, device="cuda", requires_grad=True)
+
+    def call():
+        y, h = P.add_rms_norm(x, None, gain)
+        out = P.linear_fp8(y, w, b)
+        with torch.no_grad():
+            used = P.linear_fp8(P.add_rms_norm(x, None, gain, quantize=True)[0], P.quantize_fp8(w, square=True), b)
+        return (out, used, *torch.autograd.grad(out, (x, gain, w, b), dy))
+
+    want = call()
+    torch.cuda.synchronize()
+    got = {}
+
+    def work(i):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(5):
+                mine = call()
+        s.synchronize()
+        got[i] = mine
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(3)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert len(got) == 3 and all(torch.equal(a, c) for g in got.values() for a, c in zip(g, want))
+
+
+def test_one_tensor_in_both_places():
+    w = _matrix(200, 200, F32).requires_grad_()
+    copies = [w.detach().clone().requires_grad_() for _ in range(2)]
+    dy = _matrix(200, 200, F32, 1)
+    got, = torch.autograd.grad(P.linear_fp8(w, w), w, dy)
+    a, c = torch.autograd.grad(P.linear_fp8(*copies), copies, dy)
+    assert torch.equal(got, a + c)
 
 
 def test_a_layer_in_training_and_in_use():

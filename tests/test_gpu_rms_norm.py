@@ -267,6 +267,42 @@ def test_python_and_native_paths_give_the_same_bits(monkeypatch):
         assert len(first) == len(second) and all(a.shape == c.shape and a.dtype == c.dtype and torch.equal(a, c) for a, c in zip(first, second))
 
 
+def test_one_tensor_as_update_and_residual():
+    x, _, w, dy, dh = _inputs((7, 200), F32)
+    copies = [x.detach().clone().requires_grad_() for _ in range(2)]
+    got, = torch.autograd.grad(P.add_rms_norm(x, x, w), x, (dy, dh))
+    a, c = torch.autograd.grad(P.add_rms_norm(*copies, w), copies, (dy, dh))
+    assert torch.equal(got, a + c)
+
+
+def test_columns_beyond_32_bits_are_refused():
+    x = torch.ones((), device="cuda").expand(1, (1 << 32) + 128)
+    for call in (lambda: P.add_rms_norm(x), lambda: P.add_rms_norm(x, quantize=True)):
+        with pytest.raises(RuntimeError, match="16384"):
+            call()
+
+
+def test_large_offsets():
+    """More than 2^32 elements: the last rows are those of a short call, with their gradients."""
+    rows, cols = (1 << 32) // 4096 + 77, 4096
+    x = torch.empty((rows, cols), dtype=BF16, device="cuda")
+    x[:-50] = 1.0
+    tail = _inputs((50, cols), BF16)[0].detach()
+    x[-50:] = tail
+    t = tail.clone().requires_grad_()
+    y, h = P.add_rms_norm(t)
+    dt, = torch.autograd.grad((y, h), t, (tail, tail))
+    x.requires_grad_()
+    far, same = P.add_rms_norm(x)
+    assert torch.equal(far[-50:], y) and torch.equal(far[3], far[rows // 2])
+    dx, = torch.autograd.grad((far, same), x, (x.detach(), x.detach()))
+    assert torch.equal(dx[-50:], dt) and torch.equal(dx[3], dx[rows // 2])
+    del far, same, dx
+    with torch.no_grad():
+        q, short = P.add_rms_norm(x, quantize=True)[0], P.add_rms_norm(t, quantize=True)[0]
+    assert torch.equal(q.values[-50:].view(torch.uint8), short.values.view(torch.uint8)) and torch.equal(q.scales[-50:], short.scales)
+
+
 def test_refusals():
     x, r, w, _, _ = _inputs((4, 200), BF16, F32)
     with pytest.raises(RuntimeError, match="no gradients"):
