@@ -275,6 +275,20 @@ def test_one_tensor_as_update_and_residual():
     assert torch.equal(got, a + c)
 
 
+@pytest.mark.parametrize("cols", [7, 64, 67, 600, 1025, 4100, 9001])
+def test_written_in_place(cols):
+    """The C entry point's y over x and h over the residual."""
+    lib = ops._lib.load()
+    for tx, tr in TYPES:
+        x, r, w, _, _ = _inputs((333, cols), tx, tr, seed=cols)
+        with torch.no_grad():
+            y, h = P.add_rms_norm(x, r, w)
+            a, b = x.detach().clone(), r.detach().clone()
+            ops._lib.check(lib.ptx_add_rms_norm_fwd(a.data_ptr(), b.data_ptr(), w.data_ptr(), a.data_ptr(), None, b.data_ptr(), None, 333, cols, EPS,
+                                                    ops._LN_DTYPES[tx], ops._LN_DTYPES[tr], ops._LN_DTYPES[w.dtype], ops._stream()), "add_rms_norm")
+        assert torch.equal(a, y) and torch.equal(b, h)
+
+
 def test_columns_beyond_32_bits_are_refused():
     x = torch.ones((), device="cuda").expand(1, (1 << 32) + 128)
     for call in (lambda: P.add_rms_norm(x), lambda: P.add_rms_norm(x, quantize=True)):
