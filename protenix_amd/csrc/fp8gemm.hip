@@ -77,6 +77,36 @@ __device__ __forceinline__ float param_at(const void* p, int type, int64_t i) {
   return type == 0 ? ((const float*)p)[i] : type == 1 ? (float)((const bf16_t*)p)[i] : (float)((const f16_t*)p)[i];
 }
 
+// The bias at columns col(u, r) (beyond the last one: that one once more), 0 without one.  The type is asked for once: a branch at each value has
+// a wait behind each load (1035 x 1000 x 777 with a bias in bf16 7.6 -> 6.0 us).
+template <int N, typename T, typename Col> __device__ __forceinline__ void load_bias_as(f32x4 (&out)[N], const T* bias, int cols, Col col) {
+  T v[N][4];
+#pragma unroll
+  for (int u = 0; u < N; ++u)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[u][r] = bias[min(col(u, r), cols - 1)];
+#pragma unroll
+  for (int u = 0; u < N; ++u) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) out[u][r] = (float)v[u][r];
+    // (the wait for the loads belongs here: behind the branch it would be one for all loads of what comes next, without a bias too, and what no
+    // store uses would be waited for in every block of the next tile)
+    asm volatile("" : "+v"(out[u]));
+  }
+}
+template <int N, typename Col> __device__ __forceinline__ void load_bias(f32x4 (&out)[N], const void* bias, int type, int cols, Col col) {
+  if (!bias) {
+#pragma unroll
+    for (int u = 0; u < N; ++u) out[u] = f32x4{};
+  } else if (type == 0) {
+    load_bias_as(out, (const float*)bias, cols, col);
+  } else if (type == 1) {
+    load_bias_as(out, (const bf16_t*)bias, cols, col);
+  } else {
+    load_bias_as(out, (const f16_t*)bias, cols, col);
+  }
+}
+
 // Four values of one row from column n on (bias and rounding), as many as there are.
 template <typename O> __device__ __forceinline__ void store4(O* row, int n, int cols, const f32x4& v) {
   typedef O O4 __attribute__((ext_vector_type(4), aligned(sizeof(O))));
@@ -218,13 +248,12 @@ __global__ __launch_bounds__(64 * WM * WN * WK, TM == 64 && NB == 2 && !(ROWB &&
   // A wave's stages overlap: the loads of a later block are spread over this one's first row tiles, a row tile's fragments are read while
   // the one before is multiplied, and its results scaled and added while the next one is.  The waves meet once a block, in front of its
   // last row tile - all reads of its buffer have returned then -, under whose multiplications the next block's first fragments are read.
-  // Before the next block is read: this wave's loads of it have landed (all but those of the `after` youngest blocks and `stores` that were
-  // issued behind them), and all waves' have.
-  auto meet = [&](auto after, auto stores) {
+  // Before the next block is read: this wave's loads of it have landed (all but those of the `after` youngest blocks), and all waves' have.
+  auto meet = [&](auto after) {
     if (wave == 0 || wave == C::W - 1)
-      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(after.value * (C::PER + 1) + stores.value) : "memory");
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(after.value * (C::PER + 1)) : "memory");
     else
-      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(after.value * C::PER + stores.value) : "memory");
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(after.value * C::PER) : "memory");
   };
   constexpr std::integral_constant<int, 0> none{};
 #pragma unroll
@@ -232,8 +261,8 @@ __global__ __launch_bounds__(64 * WM * WN * WK, TM == 64 && NB == 2 && !(ROWB &&
     if (k == 0 || k < steps)
 #pragma unroll
       for (int j = 0; j <= C::PER; ++j) load(k, k, j);
-  if (NB - 1 <= steps) meet(std::integral_constant<int, NB - 2>{}, none);
-  else meet(none, none);
+  if (NB - 1 <= steps) meet(std::integral_constant<int, NB - 2>{});
+  else meet(none);
   B fb = read_b(lds);
   F fa = read_a(lds, 0);
   float scale_b = read_scale_b(lds), sa = read_s(lds, 0), s_before = 0.0f;
@@ -268,7 +297,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK, TM == 64 && NB == 2 && !(ROWB &&
           for (int j = EACH * t; j < EACH * (t + 1); ++j)
             if (j <= C::PER) load(to_load, buf_loaded, j);
       }
-      if (ahead) meet(std::integral_constant<int, loads.value ? NB - 2 : 0>{}, none);
+      if (ahead) meet(std::integral_constant<int, loads.value ? NB - 2 : 0>{});
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const int before = t == 0 ? C::MT - 1 : t - 1;
@@ -336,13 +365,12 @@ __global__ __launch_bounds__(64 * WM * WN * WK, TM == 64 && NB == 2 && !(ROWB &&
     }
     const int n = n0 + 64 * wn;
     f32x4 bias[4];
+    // (here and not where a row is stored: what it reads would be waited for in every block of the next tile, since a row may not be)
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int c = n + C::col(u, q) + r;
-        bias[u][r] = p.bias && c < p.n ? param_at(p.bias, p.bias_type, c) : 0.0f;
-      }
+    for (int u = 0; u < 4; ++u) asm volatile("" : "+v"(acc[C::MT - 1][u]));
+    // (the next tile's first block has landed before the first store: stores in front of these loads cost 1 to 3 % where k is short)
+    if (more) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    load_bias(bias, p.bias, p.bias_type, p.n, [&](int u, int r) { return n + C::col(u, q) + r; });
 #pragma unroll
     for (int t = 0; t < C::MT; ++t) {
       const int m = m0 + row0 + 16 * t + i;
@@ -368,10 +396,8 @@ __global__ __launch_bounds__(64 * WM * WN * WK, TM == 64 && NB == 2 && !(ROWB &&
       }
     }
     if (!more) break;
-    // the next tile's first block has landed: all but what was issued behind its loads, which is a whole tile's stores, 16 bytes a lane each,
-    // or may be fewer at an edge
-    if (m0 + TM <= p.m && n0 + TN <= p.n) meet(none, std::integral_constant<int, C::MT * 4 * 4 * (int)sizeof(O) / 16>{});
-    else meet(none, none);
+    // (what this wave loaded of the next tile has landed)
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     buf ^= 1;
     const uint8_t* st = lds + buf * C::kStage;
     fb = read_b(st);
@@ -398,10 +424,10 @@ __global__ __launch_bounds__(256) void fp8_join_kernel(const float* __restrict__
   if (at + 4 <= count) {
     F4 s = *reinterpret_cast<const F4*>(part + at);
     for (int k = 1; k < splits; ++k) s += *reinterpret_cast<const F4*>(part + k * count + at);
-    if (bias)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[e] += param_at(bias, bias_type, (at + e) % n);
-    store4(out + at, 0, 4, f32x4{s[0], s[1], s[2], s[3]});
+    const int first = (int)(at % n);
+    f32x4 add[1];
+    load_bias(add, bias, bias_type, n, [&](int, int e) { return n < 4 ? (first + e) % n : first + e < n ? first + e : first + e - n; });
+    store4(out + at, 0, 4, f32x4{s[0], s[1], s[2], s[3]} + add[0]);
   } else {
     for (int64_t c = at; c < count; ++c) {
       float s = part[c];
@@ -426,6 +452,9 @@ __global__ __launch_bounds__(512) void fp8_few_rows_product(Fp8Args p) {
   const float *sb = p.sb + (int64_t)(n0 / kFp8Block) * p.blocks, *sa = p.sa + row;
   const uint8_t *rb = p.b + min(n0 + i, p.n - 1) * pitch + 16 * q, *ra = p.a + row * pitch + 16 * q;
   f32x4 acc = f32x4{};
+  // (in front of everything, by the wave that stores)
+  f32x4 bias[1] = {f32x4{}};
+  if (wave == 0) load_bias(bias, p.bias, p.bias_type, p.n, [&](int, int r) { return n0 + 4 * q + r; });
   auto multiply = [&](int first, auto count) {
     constexpr int N = count.value;
     i32x4 b[N][2], a[N][2];
@@ -459,9 +488,7 @@ __global__ __launch_bounds__(512) void fp8_few_rows_product(Fp8Args p) {
   for (int w = 1; w < W; ++w) acc += sums[w][lane];
   const int n = n0 + 4 * q;
   if (i >= p.m) return;
-#pragma unroll
-  for (int r = 0; r < 4; ++r) acc[r] += p.bias && n + r < p.n ? param_at(p.bias, p.bias_type, n + r) : 0.0f;
-  store4((O*)p.out + (int64_t)i * p.n, n, p.n, acc);
+  store4((O*)p.out + (int64_t)i * p.n, n, p.n, acc + bias[0]);
 }
 
 // ---- which kernel ---------------------------------------------------------------------------------------
@@ -469,15 +496,17 @@ namespace {
 // The tile kernels, as (tile; workgroups that the 256 compute units hold at once; what a round of these takes per block of k, in units of 10 ns,
 // with 16-bit and with fp32 results).  The one whose rounds take least is chosen.  us at k = 4096, in the order below (the fifth without
 // fp32): 1024 x 1024 12.0 / 16.6 / 22.9 / 41.6, 1280^2 22.0 / 19.0 / 22.9, 1536^2 32.6 / 32.3 / 23.4 / 41.8, 2048^2 - / - / 26.4 / 44.7 / 38.1 /
-// 50.4, 2560^2 - / - / 46.6 / 48.9 / 38.5 / 50.5, 3328^2 68.5 / 83.1 / 72.3 / 51.3 for the last four, 4608^2 135 / 136 / 114 / 106; fp32 1024^2 16.6 /
+// 50.4, 2560^2 - / - / 46.6 / 48.9 / 38.5 / 50.5, 3328^2 68.5 / 83.1 / 72.3 / 51.3 for the last four, 4608^2 135 / 136 / 114 / 106;
+// 192 x 256 and 256 x 256 3328^2 52 / 56, 4608^2 92 / 106, 6144 x 4096 105 / 106, 8192 x 8192 270 / 230 (whole rounds are bound by power); fp32 1024^2 16.6 /
 // 20.6 / 31.7, 1536^2 46.8 / 44.3 / 33.3 / 44.8, 2560^2 66 / 68, 4096^2 141 / 138 for the two of 128 x 128.
-enum Fp8Kernel { kFewRows, k64Deep, k64Pair, k128Split, k128Pair, k256x128, k256 };
+enum Fp8Kernel { kFewRows, k64Deep, k64Pair, k128Split, k128Pair, k256x128, k192, k256 };
 struct Fp8Shape {
   Fp8Kernel kernel;
   int tm, tn, at_once, cost16, cost32;
 };
 constexpr Fp8Shape kFp8Shapes[] = {{k64Deep, 64, 64, 256, 36, 50},     {k64Pair, 64, 64, 512, 55, 75},      {k128Split, 128, 128, 256, 72, 100},
-                                   {k128Pair, 128, 128, 512, 138, 145}, {k256x128, 256, 128, 256, 119, 210}, {k256, 256, 256, 256, 157, 0}};
+                                   {k128Pair, 128, 128, 512, 138, 145}, {k256x128, 256, 128, 256, 119, 210}, {k192, 192, 256, 256, 146, 0},
+                                   {k256, 256, 256, 256, 175, 0}};
 struct Fp8Plan {
   Fp8Kernel kernel;
   int splits;
@@ -535,6 +564,9 @@ int fp8_matmul(const void* a, const float* sa, const void* b, const float* sb, b
     case k128Split: tile_product<128, 128, 2, 2, 2, 2, O>(p, square, stream); break;
     case k128Pair: tile_product<128, 128, 2, 2, 1, 2, O>(p, square, stream); break;
     case k256x128: tile_product<256, 128, 4, 2, 1, 2, O>(p, square, stream); break;
+    case k192:
+      if constexpr (sizeof(O) == 2) tile_product<192, 256, 2, 4, 1, 2, O>(p, square, stream);
+      break;
     case k256:      // (fp32 results have widened fragments, twice the registers)
       if constexpr (sizeof(O) == 2) tile_product<256, 256, 2, 4, 1, 2, O>(p, square, stream);
   }

@@ -114,7 +114,8 @@ def test_blocks_that_are_not_finite_stay_that(bad):
 PRODUCTS = [(1, 128, 16), (1, 2048, 1000), (2, 100, 17), (15, 384, 130), (16, 1000, 128), (17, 130, 64), (33, 1, 1), (48, 129, 200),
             (64, 640, 257), (65, 640, 257), (65, 64, 3), (100, 4096, 72), (128, 128, 128), (200, 8200, 136), (257, 513, 300),
             (1035, 1000, 777), (1536, 256, 1792), (4100, 128, 520), (3000, 130, 4100), (40, 150001, 70),
-            (130, 20000, 17), (1300, 300, 1290), (1600, 200, 1500), (2500, 129, 2600)]
+            (130, 20000, 17), (1300, 300, 1290), (1600, 200, 1500), (2500, 129, 2600),
+            (2900, 130, 2950), (4500, 64, 4600)]
 
 
 def _check_product(got, a, b, bias=None):
