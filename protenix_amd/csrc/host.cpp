@@ -1502,6 +1502,20 @@ void fp8_quantize_call(const Tensor& x, int64_t rows, bool square, Fp8Operand* q
                          qt ? (float*)ptr(qt->scales) : nullptr, sums ? ptr(*sums) : nullptr, (float*)ptr(ws), rows, cols, square,
                          code_of(x.scalar_type()), sums ? code_of(sums_type) : PTX_F32, current_stream(x)), "fp8_quantize");
 }
+// An operand's values [*, k] and scales per row [*, blocks] as views: x's own dimensions, rows a pitch apart.
+Tensor fp8_values(const Tensor& data, const std::vector<int64_t>& shape) {
+  std::vector<int64_t> strides(shape.size(), 1);
+  int64_t step = data.size(1);
+  for (size_t d = shape.size() - 1; d-- > 0; step *= shape[d]) strides[d] = step;
+  return data.as_strided(shape, strides);
+}
+Tensor fp8_scales(const Tensor& scales, std::vector<int64_t> shape) {
+  shape.back() = scales.size(0);
+  std::vector<int64_t> strides(shape.size(), scales.size(1));
+  int64_t step = 1;
+  for (size_t d = shape.size() - 1; d-- > 0; step *= shape[d]) strides[d] = step;
+  return scales.as_strided(shape, strides);
+}
 Tensor fp8_matmul_call(const Fp8Operand& a, const Fp8Operand& b, const Tensor& bias, at::ScalarType type, at::IntArrayRef shape) {
   Tensor out = at::empty(shape, a.values.options().dtype(type)), ws;
   const int64_t elems = ptx_fp8_matmul_workspace_elems(a.rows, b.rows, a.cols, b.square, code_of(type));
@@ -1753,6 +1767,8 @@ PYBIND11_MODULE(_host, m) {
   m.def("dropout_add", &dropout_add);
   m.def("dropout_add_layer_norm", &dropout_add_layer_norm);
   m.def("relative_bias", &relative_bias);
+  m.def("fp8_values", &fp8_values);
+  m.def("fp8_scales", &fp8_scales);
   m.def("quantize_fp8", &quantize_fp8);
   m.def("matmul_fp8", &matmul_fp8);
   m.def("linear_fp8", &linear_fp8);

@@ -56,20 +56,11 @@ class Fp8Tensor:
 
     @property
     def values(self) -> torch.Tensor:
-        data, k = self._operand[0], self.shape[-1]
-        return (data if data.shape[1] == k else data[:, :k]).view(self.shape)
+        return native.host().fp8_values(self._operand[0], self.shape)
 
     @property
     def scales(self) -> torch.Tensor:
-        _, scales, _, _, square = self._operand
-        if square:
-            return scales
-        # (one strided view: [blocks, rows and a few] as [*, blocks])
-        strides, step = [scales.stride(0)], 1
-        for n in reversed(self.shape[:-1]):
-            strides.append(step)
-            step *= n
-        return scales.as_strided((*self.shape[:-1], scales.shape[0]), strides[::-1])
+        return self._operand[1] if self._operand[4] else native.host().fp8_scales(self._operand[1], self.shape)
 
     @property
     def square(self) -> bool:
