@@ -115,7 +115,7 @@ PRODUCTS = [(1, 128, 16), (1, 2048, 1000), (2, 100, 17), (15, 384, 130), (16, 10
             (64, 640, 257), (65, 640, 257), (65, 64, 3), (100, 4096, 72), (128, 128, 128), (200, 8200, 136), (257, 513, 300),
             (1035, 1000, 777), (1536, 256, 1792), (4100, 128, 520), (3000, 130, 4100), (40, 150001, 70),
             (130, 20000, 17), (1300, 300, 1290), (1600, 200, 1500), (2500, 129, 2600),
-            (2900, 130, 2950), (4500, 64, 4600)]
+            (2900, 130, 2950), (4500, 64, 4600), (70, 20000, 3), (20, 20000, 1)]
 
 
 def _check_product(got, a, b, bias=None):
