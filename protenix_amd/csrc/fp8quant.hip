@@ -4,9 +4,8 @@
 // Bound by memory: an element is read once and written once per direction.  Rows alone: 16 lanes hold a block in registers.  Else
 // a workgroup holds a tile of 128 x 128 in its registers, 8 x 8 per thread, takes the largest magnitudes of its rows among 16 lanes
 // and of its columns through LDS, and turns the bytes round in LDS, from where the transposed rows go out in whole lines of 128 bytes.
-// 16384 x 4096 bf16 both ways 49 us on the same tensors again (5.5 TB/s, a plain copy's rate; 59 where they come from HBM among other
-// passes), its rows alone 39 (5.3); 8192 x 4096 square both ways 26.  Tiles in one run per XCD instead of round them take 51 - 56 us, loads past
-// the caches 49 - 55.
+// 16384 x 4096 bf16 both ways 55.7 us among other passes (4.9 TB/s; a plain copy 5.8), its rows alone 39 (5.3); 8192 x 4096 square both
+// ways 28.7.  On the same tensors again 49, with tiles in one run per XCD 51 - 56, with loads past the caches 49 - 55.
 #include "fp8.h"
 #include "dropout.h"
 #include "kernels.h"
@@ -88,8 +87,13 @@ __global__ __launch_bounds__(256) void fp8_tile_kernel(const T* __restrict__ x, 
   __shared__ float inverse[kFp8Block], sums[4][kFp8Block];
   __shared__ uint32_t top_of_all[4];
   const int tiles = (int)fp8_blocks(cols), tid = threadIdx.x, wave = tid >> 6, l = tid & 15, g = tid >> 4;
-  const int64_t row_tile = blockIdx.x / (uint32_t)tiles;
-  const int col_tile = blockIdx.x - (uint32_t)row_tile * tiles;
+  // (tiles go down BAND rows of them before the next column's, so that the lines of 128 bytes that neighbouring tiles write of a transposed row
+  // go out together: 16384 x 4096 bf16 59 -> 55.7 us, with 2, 4 or 32 58, 57, 57, with 8 columns' tiles side by side in a band 58.5; of fp32, which reads more than it writes, 44.7 -> 45.7)
+  constexpr uint32_t BAND = sizeof(T) == 2 ? 8 : 1;
+  const uint32_t of_band = BAND * (uint32_t)tiles, band = blockIdx.x / of_band, in = blockIdx.x - band * of_band;
+  const uint32_t high = min(BAND, (uint32_t)fp8_blocks(rows) - band * BAND);
+  const int64_t row_tile = band * BAND + in % high;
+  const int col_tile = (int)(in / high);
   const int64_t row0 = row_tile * kFp8Block + 8 * g;      // this thread's rows row0 .. row0 + 7
   const int col = col_tile * kFp8Block + 8 * l, n = max(min(cols - col, 8), 0);
   Raw8<T> raw[8];
