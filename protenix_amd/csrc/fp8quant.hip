@@ -88,8 +88,9 @@ __global__ __launch_bounds__(256) void fp8_tile_kernel(const T* __restrict__ x, 
   __shared__ uint32_t top_of_all[4];
   const int tiles = (int)fp8_blocks(cols), tid = threadIdx.x, wave = tid >> 6, l = tid & 15, g = tid >> 4;
   // (tiles go down BAND rows of them before the next column's, so that the lines of 128 bytes that neighbouring tiles write of a transposed row
-  // go out together: 16384 x 4096 bf16 59 -> 55.7 us, with 2, 4 or 32 58, 57, 57, with 8 columns' tiles side by side in a band 58.5; of fp32, which reads more than it writes, 44.7 -> 45.7)
-  constexpr uint32_t BAND = sizeof(T) == 2 ? 8 : 1;
+  // go out together: 16384 x 4096 bf16 59 -> 55.7 us, with 2, 4 or 32 58, 57, 57, with 8 columns' tiles side by side in a band 58.5; of fp32, which reads more than it writes, 44.7 -> 45.7,
+  // and 8192 x 2048 square 11.3 -> 11.8)
+  constexpr uint32_t BAND = sizeof(T) == 2 && !SQUARE ? 8 : 1;
   const uint32_t of_band = BAND * (uint32_t)tiles, band = blockIdx.x / of_band, in = blockIdx.x - band * of_band;
   const uint32_t high = min(BAND, (uint32_t)fp8_blocks(rows) - band * BAND);
   const int64_t row_tile = band * BAND + in % high;
