@@ -683,6 +683,8 @@ PTX_API int ptx_fp8_quantize(const void* x, void* q, float* scales, void* qt, fl
  * one per 128 x 128; products of a block and sums over blocks in fp32, in a fixed order, rounded once.
  *   bias       [n], bias_dtype, or NULL
  *   workspace  ptx_fp8_matmul_workspace_elems(m, n, k, b_square, out_dtype) fp32 elements, uninitialised (none: NULL)
+ * Scales may be any numbers: also where the product of two leaves fp32's range a block's result is right if it lies within it (a block
+ * with a scale of 2^-126 or less: to 2^-125).
  * 0 < k <= 2^24, (m / 64 + 1) (n / 64 + 1) < 2^23.
  */
 PTX_API int64_t ptx_fp8_matmul_workspace_elems(int64_t m, int64_t n, int64_t k, int b_square, int out_dtype);

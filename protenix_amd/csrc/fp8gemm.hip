@@ -73,6 +73,20 @@ struct Fp8Args {
   int splits;                // of the blocks; more than one: out is fp32 [splits][m][n] without bias
 };
 
+// A block's result v (0, or 2^-18 to 2^25 in magnitude) times its two scales x and y, whose product may lie beyond fp32 where the result does not:
+// v x y = (v 2^half) rest, with half of the exponent of x y on either side.  rest is x y of 24 bits; where x y is a normal number both factors are
+// too, and so v x y has the bits that it has with x y formed first; elsewhere they are wherever the result is neither 0 nor infinite.  The tile
+// kernels form x y first, one for many v, and take this only for tiles with a scale outside 2^-63 .. 2^63.  Scales of 2^-126 and
+// below, those of blocks of zeros, do not count there (zeros in rows or tokens cost nothing more): x y may then be off by 2^-150, and the
+// block's result, of values below 448 2^-126, by 2^-125.
+struct Fp8Factors {
+  int half;
+  float rest;
+};
+__device__ __forceinline__ Fp8Factors factors(float x, float y) {
+  const int e = __builtin_amdgcn_frexp_expf(x) + __builtin_amdgcn_frexp_expf(y), half = e >> 1;
+  return {half, __builtin_amdgcn_ldexpf(__builtin_amdgcn_frexp_mantf(x) * __builtin_amdgcn_frexp_mantf(y), e - half)};
+}
 __device__ __forceinline__ float param_at(const void* p, int type, int64_t i) {
   return type == 0 ? ((const float*)p)[i] : type == 1 ? (float)((const bf16_t*)p)[i] : (float)((const f16_t*)p)[i];
 }
@@ -243,9 +257,27 @@ __global__ __launch_bounds__(64 * WM * WN * WK, TM == 64 && NB == 2 && !(ROWB &&
     return B{{fragment(tb), fragment(tb + 16 * 128), fragment(tb + 32 * 128), fragment(tb + 48 * 128)}};
   };
   auto read_a = [&](const uint8_t* st, int t) { return fragment(st + C::kA + (row0 + 16 * t) * 128); };
+  // The smallest (but for 2^-126 and below) and the largest of the scales of this wave's rows and columns in a tile: where they lie within
+  // 2^-63 .. 2^63 every product of two is a normal number, else the tile is formed again by far_products().  As whole numbers: 2^-126 and
+  // below are the largest of those less 2^-126 and a bit, negative ones the largest of all.  Each block looks at all of them once, a lane at
+  // those at at_sa and at_sb of a stage (rows and columns that are not there have any scales: the last one's once more).  8192^3 471 -> 485 us,
+  // with scales per row 548 -> 555, tiles of 64 x 64 0 - 3 %; a compare and a branch at each row tile in place of this: 3 and 5 %.
+  constexpr int SA = (16 * C::MT + kWave - 1) / kWave;
+  constexpr uint32_t LEAST = 0x00800001u;
+  int at_sa[SA], at_sb = 0;
+  uint32_t low = ~0u, high = 0;
+  auto begin_scales = [&]() {
+#pragma unroll
+    for (int h = 0; h < SA; ++h)
+      at_sa[h] = C::kSa + 4 * min(row0 + (C::MT == 1 ? i : min(64 * h + lane, 16 * C::MT - 1)), p.m - from.m0 - 1);
+    if (ROWB) at_sb = C::kSb + 4 * min(64 * wn + lane, p.n - from.n0 - 1);
+    low = ~0u;
+    high = 0;
+  };
+  begin_scales();
   // (the scale of b by way of LDS too: a load that the compiler knows of would wait for all of these)
   auto read_scale_b = [&](const uint8_t* st) { return ROWB ? 1.0f : *reinterpret_cast<const float*>(st + C::kSb + 4 * wn); };
-  auto read_s = [&](const uint8_t* st, int t) { return *reinterpret_cast<const float*>(st + C::kSa + 4 * (row0 + 16 * t + i)); };
+  auto read_s = [&](const uint8_t* st, int t) { return *reinterpret_cast<const float*>(st + (C::MT == 1 ? at_sa[0] : C::kSa + 4 * (row0 + 16 * t + i))); };
   // A wave's stages overlap: the loads of a later block are spread over this one's first row tiles, a row tile's fragments are read while
   // the one before is multiplied, and its results scaled and added while the next one is.  The waves meet once a block, in front of its
   // last row tile - all reads of its buffer have returned then -, under whose multiplications the next block's first fragments are read.
@@ -269,6 +301,50 @@ __global__ __launch_bounds__(64 * WM * WN * WK, TM == 64 && NB == 2 && !(ROWB &&
   float scale_b = read_scale_b(lds), sa = read_s(lds, 0), s_before = 0.0f;
   f32x4 d[4] = {f32x4{}, f32x4{}, f32x4{}, f32x4{}};
   int buf = 0;
+  // The wave's part of the tile once more, straight from memory, with each product as Fp8Factors has it: the same bits where the scales' is a
+  // normal number.
+  auto far_products = [&](int m0, int n0) {
+#pragma unroll
+    for (int t = 0; t < C::MT; ++t)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) acc[t][u] = f32x4{};
+    for (int block = first; block < last; ++block) {
+      int l = lane;
+      asm volatile("" : "+v"(l));      // (addresses are formed where they are used: kept over the blocks they take more registers than there are)
+      const int li = l & 15, lq = l >> 4;
+      auto from_memory = [&](const uint8_t* x, int row) {
+        const uint8_t* at = x + (int64_t)row * pitch + block * kFp8Block + 16 * lq;
+        return F(*reinterpret_cast<const i32x4*>(at), *reinterpret_cast<const i32x4*>(at + 64));
+      };
+      B b;
+      f32x4 of_b[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        b.f[u] = from_memory(p.b, min(n0 + 64 * wn + C::b_row(2 * u + (li >> 3), li & 7), p.n - 1));
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int col = min(n0 + 64 * wn + (ROWB ? C::col(u, lq) + r : 0), p.n - 1);
+          of_b[u][r] = p.sb[ROWB ? block * sp_b + col : (int64_t)(col / kFp8Block) * p.blocks + block];
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < C::MT; ++t) {
+        __builtin_amdgcn_sched_barrier(0);
+        const int row = min(m0 + row0 + 16 * t + li, p.m - 1);
+        const F a = from_memory(p.a, row);
+        const float of_a = p.sa[block * sp_a + row];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const f32x4 v = mma128(b.f[u], a);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const Fp8Factors f = factors(of_a, of_b[u][r]);
+            acc[t][u][r] = __builtin_fmaf(__builtin_amdgcn_ldexpf(v[r], f.half), f.rest, acc[t][u][r]);
+          }
+        }
+      }
+    }
+  };
   // One block; loads: of step `to_load`, into the buffer of the block before, where `loading`; next: there is a block behind this one in
   // its tile.
   auto multiply = [&](int to_load, bool loading, auto loads, auto next) {
@@ -279,12 +355,18 @@ __global__ __launch_bounds__(64 * WM * WN * WK, TM == 64 && NB == 2 && !(ROWB &&
 #pragma unroll
       for (int u = 0; u < 4; ++u) rb[u] = *reinterpret_cast<const f32x4*>(st + C::kSb + 4 * (64 * wn + C::col(u, q)));
     }
+    uint32_t scales[SA + 1];
 #pragma unroll
     for (int t = 0; t < C::MT; ++t) {
       __builtin_amdgcn_sched_barrier(0);      // (else all reads move to the front, and registers run out)
       const float s = sa * scale_b;
       const bool ahead = next.value && t + 1 == C::MT;      // (known where the loop is unrolled)
       const uint8_t* sn = lds + buf_next * C::kStage;
+      if (t == 0) {
+#pragma unroll
+        for (int h = 0; h < SA; ++h) scales[h] = C::MT == 1 ? __float_as_uint(sa) : *reinterpret_cast<const uint32_t*>(st + at_sa[h]);
+        scales[SA] = ROWB ? *reinterpret_cast<const uint32_t*>(st + at_sb) : __float_as_uint(scale_b);
+      }
       F fa_next;
       if (t + 1 < C::MT) {
         fa_next = read_a(st, t + 1);
@@ -309,6 +391,13 @@ __global__ __launch_bounds__(64 * WM * WN * WK, TM == 64 && NB == 2 && !(ROWB &&
         }
         d[u] = mma128(fb.f[u], fa);
         if (ahead) fb.f[u] = fragment(sn + C::kB + (64 * wn + 16 * u) * 128);
+      }
+      if (t == 0) {
+#pragma unroll
+        for (int h = 0; h <= SA; ++h) {
+          low = min(low, scales[h] - LEAST);
+          high = max(high, scales[h]);
+        }
       }
       s_before = s;
       if (ahead) {
@@ -346,6 +435,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK, TM == 64 && NB == 2 && !(ROWB &&
 #pragma unroll
         for (int r = 0; r < 4; ++r) acc[C::MT - 1][u][r] = __builtin_fmaf(d[u][r], s_before, acc[C::MT - 1][u][r]);
     }
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(low < 0x20000000u - LEAST || high > 0x5f000000u) != 0, 0)) far_products(m0, n0);
     if constexpr (WK > 1) {
       // the groups' sums, added in their order
       f32x4* sums = reinterpret_cast<f32x4*>(lds_all) + wave * C::MT * 4 * kWave + lane;
@@ -405,6 +495,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK, TM == 64 && NB == 2 && !(ROWB &&
     fa = read_a(st, 0);
     sa = read_s(st, 0);
     scale_b = read_scale_b(st);
+    begin_scales();
     s_before = 0.0f;
 #pragma unroll
     for (int u = 0; u < 4; ++u) d[u] = f32x4{};
@@ -459,7 +550,7 @@ __global__ __launch_bounds__(512) void fp8_few_rows_product(Fp8Args p) {
   auto multiply = [&](int first, auto count) {
     constexpr int N = count.value;
     i32x4 b[N][2], a[N][2];
-    float s[N];
+    float s[N], t[N];
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const int64_t at = (int64_t)(first + W * j) * kFp8Block;
@@ -468,14 +559,16 @@ __global__ __launch_bounds__(512) void fp8_few_rows_product(Fp8Args p) {
         b[j][h] = *reinterpret_cast<const i32x4*>(rb + at + 64 * h);
         a[j][h] = *reinterpret_cast<const i32x4*>(ra + at + 64 * h);
       }
-      s[j] = sb[first + W * j] * sa[(first + W * j) * sp];
+      s[j] = sb[first + W * j];
+      t[j] = sa[(first + W * j) * sp];
     }
     __builtin_amdgcn_sched_barrier(0);      // (else the loads move to where they are used, one after the other)
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const f32x4 d = mma128(F(b[j][0], b[j][1]), F(a[j][0], a[j][1]));
+      const Fp8Factors f = factors(s[j], t[j]);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) acc[r] = __builtin_fmaf(d[r], s[j], acc[r]);
+      for (int r = 0; r < 4; ++r) acc[r] = __builtin_fmaf(__builtin_amdgcn_ldexpf(d[r], f.half), f.rest, acc[r]);
     }
   };
   int block = wave;
