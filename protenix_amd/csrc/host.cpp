@@ -1536,7 +1536,10 @@ std::vector<int64_t> with_last(at::IntArrayRef shape, int64_t last) {
 }
 
 optional<std::tuple<optional<OperandTuple>, optional<OperandTuple>>> quantize_fp8(const Tensor& x_, bool square, bool rows_too, bool columns_too) {
-  if (!x_.is_cuda() || !float_type(x_) || x_.dim() < 1 || x_.numel() == 0 || (square && x_.dim() != 2)) return c10::nullopt;
+  if (!x_.is_cuda() || !float_type(x_) || x_.dim() < 1 || x_.numel() == 0 || (square && x_.dim() != 2) ||
+      (at::GradMode::is_enabled() && wants(x_) && !x_.is_leaf()))
+    return c10::nullopt;
+  refuse_tangents({&x_});
   optional<OperandTuple> first, second;
   {
     py::gil_scoped_release nogil;

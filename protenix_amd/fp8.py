@@ -36,7 +36,8 @@ class Fp8Tensor:
         want = (-(-lead[0] // BLOCK), -(-k // BLOCK)) if square else (*lead, -(-k // BLOCK))
         if tuple(scales.shape) != want:
             raise RuntimeError(f"values {tuple(values.shape)} have scales {want}{' (square)' if square else ''}, got {tuple(scales.shape)}")
-        rows = math.prod(lead)
+        _refuse_lost_gradients(values, scales)
+        values, scales, rows = values.detach(), scales.detach(), math.prod(lead)
         with torch.cuda.device(values.device):
             operand = ops.fp8_buffers(rows, k, bool(square), values.device)
             data = operand[0].view(torch.uint8)
@@ -86,7 +87,8 @@ def _matrix(x: torch.Tensor, name: str) -> torch.Tensor:
 
 
 def quantize_fp8(x: torch.Tensor, *, square: bool = False, along: Union[int, Tuple[int, int]] = -1):
-    """x [*, k], float32, bfloat16 or float16, in 8-bit blocks (no gradient: a rounding has none; `linear_fp8` has its own).
+    """x [*, k], float32, bfloat16 or float16, in 8-bit blocks (no gradient: a rounding has none; `linear_fp8` has its own.  So an x
+    on the way of one, forward-mode or of a graph, is refused; a leaf is taken, a weight to serve, and gets nothing from here).
 
     along=-1: blocks of the last dimension; the result has x's shape.  along=-2: the rows (all other dimensions as one) are the axis
     that will be summed over: the transposed matrix [k, rows], blocks along its rows.  along=(-1, -2): both, from one pass over x.
@@ -107,6 +109,7 @@ def quantize_fp8(x: torch.Tensor, *, square: bool = False, along: Union[int, Tup
         raise RuntimeError(f"square blocks are of a matrix [n, k], got {tuple(x.shape)}")
     if along != -1 and matrix.shape[0] == 0:
         raise RuntimeError("along=-2: no rows to sum over")
+    _refuse_lost_gradients(x)
     q, qt, _ = ops.fp8_quantize(matrix.detach(), bool(square), along != -2, along != -1)
     got = [Fp8Tensor._of(q, x.shape) if q else None, Fp8Tensor._of(qt, (matrix.shape[1], matrix.shape[0])) if qt else None]
     return tuple(got) if along == (-1, -2) else got[along == -2]
@@ -151,6 +154,12 @@ def matmul_fp8(a: Fp8Tensor, b: Fp8Tensor, bias: Optional[torch.Tensor] = None, 
 def _refuse_wanted(*tensors: Optional[torch.Tensor]) -> None:
     if _wants_grad(*tensors):
         raise RuntimeError("operands in 8 bits have no gradients: give linear_fp8 the tensors themselves, or call under torch.no_grad()")
+
+
+def _refuse_lost_gradients(*tensors: torch.Tensor) -> None:
+    """What passes a gradient on to others; a leaf is taken as it stands."""
+    _refuse_tangents(*tensors)
+    _refuse_wanted(*(t for t in tensors if not t.is_leaf))
 
 
 class _LinearFp8(torch.autograd.Function):
