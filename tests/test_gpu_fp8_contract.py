@@ -5,6 +5,7 @@ from torch.autograd import forward_ad
 
 import protenix_amd as P
 from protenix_amd import ops
+from tests import fp8_oracle as Q
 
 pytestmark = pytest.mark.gpu
 
@@ -47,3 +48,27 @@ def test_operands_of_parameters(native, monkeypatch):
         P.Fp8Tensor(q.values, scales * 1.0, square=True)
     with forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
         P.Fp8Tensor(q.values, forward_ad.make_dual(q.scales, q.scales.clone()), square=True)
+
+
+def test_scales_and_their_inverses_at_every_mantissa():
+    """s = a / 448 and i = 1 / s are each rounded once: for all 2^23 mantissas of a, s itself, and i by values that lie where one unit of i
+    decides between two numbers of 8 bits."""
+    ties = torch.arange(17, 32, 2, dtype=torch.float64, device="cuda")      # in the middle of two e4m3 numbers
+    steps = torch.arange(-7, 8, dtype=torch.int32, device="cuda")
+    told = 0
+    for first in range(0, 1 << 23, 1 << 18):
+        a = (torch.arange(first, first + (1 << 18), dtype=torch.int32, device="cuda") + (140 << 23)).view(torch.float32)
+        s = (a.double() / 448).float()
+        i = (1 / s.double()).float()
+        near = (ties[None, :] / i.double()[:, None]).float()
+        x = torch.zeros((1 << 18, 128), device="cuda")
+        x[:, 0] = a
+        x[:, 1:121] = (near.view(torch.int32)[:, :, None] + steps).view(torch.float32).reshape(1 << 18, 120)
+        t = P.quantize_fp8(x)
+        assert torch.equal(t.scales[:, 0], s), first
+        rounded = lambda inverse: Q.round_e4m3((x.double() * inverse.double()[:, None]).float().double()).float()
+        want = rounded(i)
+        assert torch.equal(t.values.float(), want), first
+        for unit in (-1, 1):
+            told += (rounded((i.view(torch.int32) + unit).view(torch.float32)) != want).any(1).sum().item()
+    assert told > 1.9 * 2**23, told / 2**23      # (an inverse off by a unit either way shows)
