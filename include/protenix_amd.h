@@ -680,7 +680,10 @@ PTX_API int ptx_fp8_quantize(const void* x, void* q, float* scales, void* qt, fl
                              void* stream);
 /*
  * out [m][n] (out_dtype) = a b^T + bias: a [m][k] with a scale per 128 values of a row, b [n][k] with the same or, b_square, with
- * one per 128 x 128; products of a block and sums over blocks in fp32, in a fixed order, rounded once.
+ * one per 128 x 128; sums in fp32, in a fixed order, rounded once.  Within a block: for fp32 results in fp32 too; for 16-bit ones
+ * as the 8-bit matrix instruction forms them, which cuts each product below 2^-13 of the power of two of the largest among 8
+ * neighbouring k, so that a result is off by up to 7 2^-13 times the sum of those largest products (normal data: 1.4e-5 of the
+ * result; where large products cancel one another ask for fp32).
  *   bias       [n], bias_dtype, or NULL
  *   workspace  ptx_fp8_matmul_workspace_elems(m, n, k, b_square, out_dtype) fp32 elements, uninitialised (none: NULL)
  * Scales may be any numbers: also where the product of two leaves fp32's range a block's result is right if it lies within it (a block

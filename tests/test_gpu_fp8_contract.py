@@ -6,6 +6,7 @@ from torch.autograd import forward_ad
 import protenix_amd as P
 from protenix_amd import ops
 from tests import fp8_oracle as Q
+from tests.residual_oracle import half_step, smallest
 
 pytestmark = pytest.mark.gpu
 
@@ -72,3 +73,32 @@ def test_scales_and_their_inverses_at_every_mantissa():
         for unit in (-1, 1):
             told += (rounded((i.view(torch.int32) + unit).view(torch.float32)) != want).any(1).sum().item()
     assert told > 1.9 * 2**23, told / 2**23      # (an inverse off by a unit either way shows)
+
+
+@pytest.mark.parametrize("shape", [(5, 1024, 96), (70, 1000, 130), (300, 1024, 290), (1300, 500, 1290), (2500, 256, 2600), (3000, 256, 4100)])
+@pytest.mark.parametrize("square", [True, False])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_large_products_that_cancel(shape, square, dtype):
+    """Channels that stand out, two of each 8, whose products cancel: results in 16 bits are off by no more than is said of them (each of
+    the other products of a group by 2^-13 of its largest), those in fp32 by no more than fp32 sums are."""
+    m, k, n = shape
+    g = torch.Generator().manual_seed(sum(shape))
+    x, w = torch.randn((m, k), generator=g), torch.randn((n, k), generator=g)
+    x[:, ::8] *= 100
+    x[:, 3::8] = -x[:, ::8][:, :x[:, 3::8].shape[1]]
+    w[:, 3::8] = w[:, ::8][:, :w[:, 3::8].shape[1]]
+    a, b = P.quantize_fp8(x.cuda()), P.quantize_fp8(w.cuda(), square=square)
+    ad, bd = Q.held_by(a), Q.held_by(b)
+    got = P.matmul_fp8(a, b, dtype=dtype).cpu().double()
+    want = torch.mm(ad, bd.t().contiguous())
+    off, said = (got - want).abs(), half_step(dtype) * want.abs() + smallest(dtype)
+    size = torch.mm(ad.abs(), bd.abs().t().contiguous())
+    blocks = -(-k // 128)
+    said = said + (2.0**-16 + (blocks + 3) * 2.0**-24) * size
+    if dtype != torch.float32:
+        # the largest of a group of 8 is one of the two that stand out, or no more than the sum of the others
+        rest = torch.ones(k, dtype=torch.bool)
+        rest[::8] = rest[3::8] = False
+        one = torch.mm(ad[:, ::8].abs(), bd[:, ::8].abs().t().contiguous())
+        said = said + 7 * 2.0**-13 * (one + torch.mm(ad[:, rest].abs(), bd[:, rest].abs().t().contiguous()))
+    assert (off <= said).all(), ((off / said).max().item(), (off > said).sum().item())
