@@ -102,3 +102,34 @@ def test_large_products_that_cancel(shape, square, dtype):
         one = torch.mm(ad[:, ::8].abs(), bd[:, ::8].abs().t().contiguous())
         said = said + 7 * 2.0**-13 * (one + torch.mm(ad[:, rest].abs(), bd[:, rest].abs().t().contiguous()))
     assert (off <= said).all(), ((off / said).max().item(), (off > said).sum().item())
+
+
+@pytest.mark.parametrize("leaf", ["x", "w", "b"])
+def test_each_gradient_against_differences(leaf):
+    """Along a leaf's own direction (it times 1 + t, which moves its scales alone): dy close to y makes the slopes as large as their
+    share of the sum of magnitudes, that of b is exact but for fp32, and neither allows a gradient that is 0 or has the wrong sign."""
+    g = torch.Generator().manual_seed(7)
+    x, w, b = (torch.randn(s, generator=g).mul(v).cuda().requires_grad_() for s, v in (((130, 256), 1.0), ((140, 256), 0.1), ((140,), 1.0)))
+    y = P.linear_fp8(x, w, b)
+    dy = y.detach() + 0.1 * torch.randn(y.shape, generator=g).cuda()
+    grads = dict(zip("xwb", torch.autograd.grad(y, (x, w, b), dy)))
+    leaves, t = dict(x=x.detach(), w=w.detach(), b=b.detach()), 2.0**-3
+    value = lambda s: (P.linear_fp8(*(v * s if n == leaf else v for n, v in leaves.items())).double() * dy.double()).sum().item()
+    slope = (value(1 + t) - value(1 - t)) / (2 * t)
+    got = (grads[leaf].double() * leaves[leaf].double()).sum().item()
+    xd, wd, dd = leaves["x"].double(), leaves["w"].double(), dy.double()
+    size = (y.double() * dd).abs().sum().item()
+    # two values of y in fp32 on either side, off by half a step and the 2^-16 of their sums' magnitudes (product_bound()); db's own additions
+    magnitudes = torch.mm(xd.abs(), wd.abs().t().contiguous())
+    if leaf == "b":
+        # (what the products are off by is the same on both sides)
+        tol = 2.0**-23 * ((magnitudes + y.double().abs()) * dd.abs()).sum().item() / t + 140 * 2.0**-24 * (dd.abs().sum(0) * leaves["b"].double().abs()).sum().item()
+    else:
+        # dx and dW take dy in 8 bits, x and W as blocks along other axes or in full: a rounding is off by at most half a step, evenly on both
+        # sides of 0, so by a third of its square in the mean; 8 times the deviation of all of them, and 2^-10 for slopes of their density
+        step = lambda v: 2.0**-4 * v.abs() + 2.0**-18 * v.abs().max()
+        spread = [(step(dd) * torch.mm(xd, wd.t().contiguous())), (step(xd) * torch.mm(dd, wd)), (step(wd) * torch.mm(dd.t().contiguous(), xd))]
+        tol = 8 * sum(v.square().sum().item() / 3 for v in spread)**0.5 * 2**0.5 + 2.0**-10 * size
+    assert abs(slope - got) <= tol, (slope, got, tol)
+    # (of y's variance 256 0.1^2 = 2.56 is the products', 1 the bias': 0.72 and 0.28 of it)
+    assert abs(slope) > 8 * tol and abs(slope) > (0.2 if leaf == "b" else 0.6) * size, (slope, tol, size)

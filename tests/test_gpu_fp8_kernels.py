@@ -44,6 +44,7 @@ def _check(a, b, dtype):
     tol = lost * size + half_step(dtype) * want.abs() + smallest(dtype)
     assert (off <= tol).all(), (ad.shape, bd.shape, (off / tol).max().item(), (off > tol).sum().item())
 
+
 def _launched(profile):
     """(what, template arguments) of the products' kernels."""
     found = set()
