@@ -590,7 +590,7 @@ __global__ __launch_bounds__(512) void fp8_few_rows_product(Fp8Args p) {
 // ---- which kernel ---------------------------------------------------------------------------------------
 namespace {
 // The tile kernels, as (tile; workgroups that the 256 compute units hold at once; what a round of these takes per block of k, in units of 10 ns,
-// with 16-bit and with fp32 results).  The one whose rounds take least is chosen.  us at k = 4096, in the order below (the fifth without
+// with 16-bit and with fp32 results; 0: not built).  The one whose rounds take least is chosen.  us at k = 4096, in the order below (the fifth without
 // fp32): 1024 x 1024 12.0 / 16.6 / 22.9 / 41.6, 1280^2 22.0 / 19.0 / 22.9, 1536^2 32.6 / 32.3 / 23.4 / 41.8, 2048^2 - / - / 26.4 / 44.7 / 38.1 /
 // 50.4, 2560^2 - / - / 46.6 / 48.9 / 38.5 / 50.5, 3328^2 68.5 / 83.1 / 72.3 / 51.3 for the last four, 4608^2 135 / 136 / 114 / 106;
 // 192 x 256 and 256 x 256 3328^2 52 / 56, 4608^2 92 / 106, 6144 x 4096 105 / 106, 8192 x 8192 270 / 230 (whole rounds are bound by power); fp32 1024^2 16.6 /
@@ -601,7 +601,7 @@ struct Fp8Shape {
   int tm, tn, at_once, cost16, cost32;
 };
 constexpr Fp8Shape kFp8Shapes[] = {{k64Deep, 64, 64, 256, 36, 50},     {k64Pair, 64, 64, 512, 55, 75},      {k128Split, 128, 128, 256, 72, 100},
-                                   {k128Pair, 128, 128, 512, 138, 145}, {k256x128, 256, 128, 256, 119, 210}, {k192, 192, 256, 256, 146, 0},
+                                   {k128Pair, 128, 128, 512, 138, 145}, {k256x128, 256, 128, 256, 119, 0}, {k192, 192, 256, 256, 146, 0},
                                    {k256, 256, 256, 256, 175, 0}};
 struct Fp8Plan {
   Fp8Kernel kernel;
@@ -659,7 +659,9 @@ int fp8_matmul(const void* a, const float* sa, const void* b, const float* sb, b
     case k64Pair: tile_product<64, 64, 4, 1, 2, 2, O>(p, square, stream); break;
     case k128Split: tile_product<128, 128, 2, 2, 2, 2, O>(p, square, stream); break;
     case k128Pair: tile_product<128, 128, 2, 2, 1, 2, O>(p, square, stream); break;
-    case k256x128: tile_product<256, 128, 4, 2, 1, 2, O>(p, square, stream); break;
+    case k256x128:      // (with fp32 results two workgroups of 128 x 128 to a compute unit take fewer or as many rounds, of 145 against 210)
+      if constexpr (sizeof(O) == 2) tile_product<256, 128, 4, 2, 1, 2, O>(p, square, stream);
+      break;
     case k192:
       if constexpr (sizeof(O) == 2) tile_product<192, 256, 2, 4, 1, 2, O>(p, square, stream);
       break;
