@@ -175,7 +175,7 @@ template <int TM, int TN, int WM, int WN, int NB, bool PAIRS> struct Fp8Tile {
 
 // (two workgroups of small tiles to a compute unit where their buffers leave the room: 4 waves per SIMD)
 template <int TM, int TN, int WM, int WN, int WK, int NB, bool ROWB, typename O>
-__global__ __launch_bounds__(64 * WM * WN * WK, TM == 64 && NB == 2 && !(ROWB && sizeof(O) == 4) ? 4 : 1) void fp8_tile_product(Fp8Args p) {
+__global__ __launch_bounds__(64 * WM * WN * WK, TM == 64 && NB == 2 ? 4 : 1) void fp8_tile_product(Fp8Args p) {
   typedef Fp8Tile<TM, TN, WM, WN, NB, sizeof(O) == 2> C;
   __shared__ __align__(16) uint8_t lds_all[WK * NB * C::kStage];
   const int lane = threadIdx.x & 63, wave_of_all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -615,6 +615,9 @@ Fp8Plan fp8_plan(int64_t m, int64_t n, int64_t blocks, bool square, bool wide) {
   Fp8Plan best{k64Deep, 1};
   int64_t least = INT64_MAX;
   for (const Fp8Shape& s : kFp8Shapes) {
+    // (its fp32 results with scales per row take 150 registers, and so one workgroup to a compute unit: 1300 x 1024 x 1300 14.5 us, two rounds of k64Deep
+    // 13.6, 1024 x 4096 x 1100 40.0 and 32.5)
+    if (s.kernel == k64Pair && wide && !square) continue;
     const int64_t cost = (tiles(s.tm, s.tn) + s.at_once - 1) / s.at_once * (wide ? s.cost32 : s.cost16);
     if (cost > 0 && cost < least) {
       least = cost;
@@ -637,7 +640,9 @@ int64_t fp8_matmul_workspace_elems(int64_t m, int64_t n, int64_t blocks, bool sq
 template <int TM, int TN, int WM, int WN, int WK, int NB, typename O> static void tile_product(Fp8Args p, bool square, hipStream_t stream) {
   p.tiles_m = (p.m + TM - 1) / TM;
   p.tiles_n = (p.n + TN - 1) / TN;
-  auto* kernel = square ? fp8_tile_product<TM, TN, WM, WN, WK, NB, false, O> : fp8_tile_product<TM, TN, WM, WN, WK, NB, true, O>;
+  auto* kernel = fp8_tile_product<TM, TN, WM, WN, WK, NB, false, O>;
+  if constexpr (TM > 64 || NB > 2 || sizeof(O) == 2)      // (the one that fp8_plan leaves out)
+    if (!square) kernel = fp8_tile_product<TM, TN, WM, WN, WK, NB, true, O>;
   // (walking over tiles: as many workgroups as the compute units hold)
   const unsigned tiles = (unsigned)p.tiles_m * p.tiles_n;
   const unsigned groups = WK == 1 && NB == 2 ? std::min(tiles, 256u * (TM * TN > 128 * 128 ? 1 : 2)) : tiles;

@@ -66,7 +66,8 @@ def test_every_kernel_is_right(dtype, square):
         for a, b in operands:
             P.matmul_fp8(a, b, dtype=dtype)
         torch.cuda.synchronize()
-    want = {("tile_product", tile, not square, dtype) for tile in (TILES if dtype == F32 else TILES16)} | {("join_kernel", (), False, dtype)}
+    tiles = TILES16 if dtype != F32 else TILES if square else TILES - {(64, 64, 4, 1, 2, 2)}
+    want = {("tile_product", tile, not square, dtype) for tile in tiles} | {("join_kernel", (), False, dtype)}
     if square:
         want.add(("few_rows_product", (), False, dtype))
     got = _launched(profile)
