@@ -260,7 +260,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK, TM == 64 && NB == 2 ? 4 : 1) voi
   };
   auto read_a = [&](const uint8_t* st, int t) { return fragment(st + C::kA + (row0 + 16 * t) * 128); };
   // The smallest (but for 2^-126 and below) and the largest of the scales of this wave's rows and columns in a tile: where they lie within
-  // 2^-63 .. 2^63 every product of two is a normal number, else the tile is formed again by far_products().  As whole numbers: 2^-126 and
+  // 2^-63 .. 2^63 every product of two is a normal number, else far_apart() looks closer and far_products() forms the tile again.  As whole numbers: 2^-126 and
   // below are the largest of those less 2^-126 and a bit, negative ones the largest of all.  Each block looks at all of them once, a lane at
   // those at at_sa and at_sb of a stage (rows and columns that are not there have any scales: the last one's once more).  8192^3 471 -> 485 us,
   // with scales per row 548 -> 555, tiles of 64 x 64 0 - 3 %; a compare and a branch at each row tile in place of this: 3 and 5 %.
@@ -303,6 +303,34 @@ __global__ __launch_bounds__(64 * WM * WN * WK, TM == 64 && NB == 2 ? 4 : 1) voi
   float scale_b = read_scale_b(lds), sa = read_s(lds, 0), s_before = 0.0f;
   f32x4 d[4] = {f32x4{}, f32x4{}, f32x4{}, f32x4{}};
   int buf = 0;
+  // Whether the smallest or the largest scales of these rows and columns have such a product (of magnitudes, without infinities and NaN): gradients
+  // of 1e-22 in a few rows beside ordinary weights do not, and the tile stands (8192 x 4096 x 8192 with one such row in 128: 256 -> 301 us, formed
+  // again 943).
+  auto far_apart = [&](int m0, int n0) {
+    uint32_t low_a = ~0u, high_a = 0, low_b = ~0u, high_b = 0;
+    auto look = [&](float v, uint32_t& lo, uint32_t& hi) {
+      const uint32_t x = __float_as_uint(v) & 0x7fffffffu;
+      if (x >= 0x7f800000u) return;
+      lo = min(lo, x - LEAST);
+      hi = max(hi, x);
+    };
+#pragma unroll 4
+    for (int block = first; block < last; ++block) {
+#pragma unroll
+      for (int h = 0; h < SA; ++h) look(p.sa[block * sp_a + min(m0 + row0 + min(64 * h + lane, 16 * C::MT - 1), p.m - 1)], low_a, high_a);
+      const int col = min(n0 + 64 * wn + (ROWB ? lane : 0), p.n - 1);
+      look(p.sb[ROWB ? block * sp_b + col : (int64_t)(col / kFp8Block) * p.blocks + block], low_b, high_b);
+    }
+#pragma unroll
+    for (int m = 1; m < kWave; m <<= 1) {
+      low_a = min(low_a, (uint32_t)__shfl_xor((int)low_a, m, 64));
+      high_a = max(high_a, (uint32_t)__shfl_xor((int)high_a, m, 64));
+      low_b = min(low_b, (uint32_t)__shfl_xor((int)low_b, m, 64));
+      high_b = max(high_b, (uint32_t)__shfl_xor((int)high_b, m, 64));
+    }
+    const float least = __uint_as_float(low_a + LEAST) * __uint_as_float(low_b + LEAST), most = __uint_as_float(high_a) * __uint_as_float(high_b);
+    return __builtin_amdgcn_ballot_w64((low_a != ~0u && low_b != ~0u && least < 0x1p-126f) || most > 0x1.fffffep127f) != 0;
+  };
   // The wave's part of the tile once more, straight from memory, with each product as Fp8Factors has it: the same bits where the scales' is a
   // normal number.
   auto far_products = [&](int m0, int n0) {
@@ -437,7 +465,8 @@ __global__ __launch_bounds__(64 * WM * WN * WK, TM == 64 && NB == 2 ? 4 : 1) voi
 #pragma unroll
         for (int r = 0; r < 4; ++r) acc[C::MT - 1][u][r] = __builtin_fmaf(d[u][r], s_before, acc[C::MT - 1][u][r]);
     }
-    if (__builtin_expect(__builtin_amdgcn_ballot_w64(low < 0x20000000u - LEAST || high > 0x5f000000u) != 0, 0)) far_products(m0, n0);
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(low < 0x20000000u - LEAST || high > 0x5f000000u) != 0, 0))
+      if (far_apart(m0, n0)) far_products(m0, n0);
     if constexpr (WK > 1) {
       // the groups' sums, added in their order
       f32x4* sums = reinterpret_cast<f32x4*>(lds_all) + wave * C::MT * 4 * kWave + lane;

@@ -96,9 +96,9 @@ def test_a_row_has_the_same_bits_beside_any_scales(square, dtype):
         a = P.quantize_fp8(torch.randn((m, k), generator=g).cuda())
         b = P.quantize_fp8(torch.randn((n, k), generator=g).cuda(), square=square)
         want = P.matmul_fp8(a, b, dtype=dtype)
-        for extreme in (2.0**-126, 2.0**100, 0.0, float("nan")):
+        for extreme in (2.0**-70, 2.0**-120, 2.0**-126, 2.0**100, 2.0**125, 0.0, float("nan"), float("inf")):
             other = P.Fp8Tensor(a.values, torch.where((torch.arange(m, device="cuda") % 3 == 1)[:, None], extreme, a.scales))
-            if extreme == extreme:
+            if extreme < 1:
                 other._operand[1][:, m:] = 2.0**-126      # (read along with the others)
             rest = torch.arange(m, device="cuda") % 3 != 1
             assert torch.equal(P.matmul_fp8(other, b, dtype=dtype)[rest], want[rest])
