@@ -1607,7 +1607,10 @@ optional<Tensor> linear_fp8(const Tensor& x_, const Tensor& weight, const option
       weight.device() != x_.device() || x_.size(-1) != weight.size(1) || !fits_bias(bias, weight.size(0), x_.device()))
     return c10::nullopt;
   const auto type = type_ ? *type_ : x_.scalar_type();
-  if (!product_type(type)) return c10::nullopt;
+  constexpr int64_t most = 1 << 24;      // (values that a product sums over)
+  if (!product_type(type) ||
+      (at::GradMode::is_enabled() && ((wants(weight) && x_.numel() / x_.size(-1) > most) || (wants(x_) && weight.size(0) > most))))
+    return c10::nullopt;
   py::gil_scoped_release nogil;
   at::DeviceGuard dev(x_.device());
   const Tensor b = given(bias);

@@ -16,6 +16,7 @@ from . import native, ops
 from .dropout import _refuse_foreign_accumulators, _refuse_tangents, _wants_grad
 
 BLOCK = 128
+_MOST_SUMMED = 1 << 24      # values that a product sums over (ptx_fp8_matmul's k)
 
 
 class Fp8Tensor:
@@ -198,7 +199,8 @@ def linear_fp8(x: Operand, weight: Operand, bias: Optional[torch.Tensor] = None,
     default x's, or for float32 x under torch.autocast that one's; bfloat16 for x in 8 bits); see `matmul_fp8` for the sums of 16-bit ones.
     Training: x and dy in blocks of 128 along the axis each product sums over, the weight in blocks of 128 x 128; dx = dy W and
     dW = dy^T x are products of such operands too, with the rounding to 8 bits taken as the identity, and db is summed in fp32,
-    in a fixed order.  Gradients have their inputs' types.  Neither x nor the weight is kept, only their 8-bit forms."""
+    in a fixed order.  Gradients have their inputs' types.  Neither x nor the weight is kept, only their 8-bit forms.  A product sums
+    over at most 2^24 values, and so do gradients: rows of x for the weight's, of the weight for x's."""
     if dtype is None and isinstance(x, torch.Tensor):
         dtype = ops.autocast_compute_dtype(x)      # (as `Linear`: for fp32 x under torch.autocast its type)
     if ops.use_native_operators() and isinstance(x, torch.Tensor):
@@ -224,6 +226,10 @@ def linear_fp8(x: Operand, weight: Operand, bias: Optional[torch.Tensor] = None,
     _refuse_tangents(*plain)
     if isinstance(x, torch.Tensor) and isinstance(weight, torch.Tensor) and _wants_grad(*plain):
         _refuse_foreign_accumulators(*plain)
+        # (here, and not in the backward pass: the gradients are products over the rows of x and over those of the weight)
+        rows = math.prod(x.shape[:-1])
+        if (weight.requires_grad and rows > _MOST_SUMMED) or (x.requires_grad and n > _MOST_SUMMED):
+            raise RuntimeError(f"gradients of linear_fp8 sum over at most {_MOST_SUMMED} rows, got {rows} of x and {n} of the weight")
         return _LinearFp8.apply(x, weight, bias, dtype)
     if isinstance(x, Fp8Tensor) or isinstance(weight, Fp8Tensor):
         _refuse_wanted(*plain)

@@ -133,3 +133,16 @@ def test_each_gradient_against_differences(leaf):
     assert abs(slope - got) <= tol, (slope, got, tol)
     # (of y's variance 256 0.1^2 = 2.56 is the products', 1 the bias': 0.72 and 0.28 of it)
     assert abs(slope) > 8 * tol and abs(slope) > (0.2 if leaf == "b" else 0.6) * size, (slope, tol, size)
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_gradients_over_more_rows_than_a_product_sums_are_refused_in_front(native, monkeypatch):
+    """Before anything is launched, not in the backward pass."""
+    monkeypatch.setattr(ops, "native_enabled", native)
+    long = torch.zeros((1, 8), dtype=torch.bfloat16, device="cuda").expand((1 << 24) + 1, 8)
+    short = torch.zeros((3, 8), dtype=torch.bfloat16, device="cuda")
+    for x, w in ((long, short.clone().requires_grad_()), (short.clone().requires_grad_(), long)):
+        before = torch.cuda.memory_allocated()
+        with pytest.raises(RuntimeError, match="at most 16777216"):
+            P.linear_fp8(x, w)
+        assert torch.cuda.memory_allocated() == before
