@@ -672,7 +672,7 @@ PTX_API int64_t ptx_fp8_scale_elems(int64_t rows, int64_t cols, int square);
  * blocks along x's rows, as a product over the rows takes it.  Either pair may be NULL.
  *   col_sums   sums of x over its rows [cols], col_sums_dtype, or NULL (summed in fp32, in a fixed order); needs the workspace of
  *              ptx_fp8_col_sums_workspace_elems(rows, cols) fp32 elements, uninitialised
- * Fewer than 2^28 blocks of 128 values of a row.
+ * (rows + 127) times the blocks of 128 values of a row is below 2^28.
  */
 PTX_API int64_t ptx_fp8_col_sums_workspace_elems(int64_t rows, int64_t cols);
 PTX_API int ptx_fp8_quantize(const void* x, void* q, float* scales, void* qt, float* scales_t, void* col_sums,

@@ -153,11 +153,12 @@ __device__ __forceinline__ void tile_of(uint32_t id, int tiles_m, int tiles_n, i
 // (147456 x 128 x 512 in fp32 112 -> 84 us).
 //
 // 256 x 256, which takes what is large: 256 x 256 is the most that 256 registers a lane hold the sums of (128) with two waves per SIMD, whose
-// vector work then hides behind each other's MFMAs, and two buffers of both operands fill the LDS.  8192^3 in 455 us (2.42 PFLOP/s),
-// 8192 x 4096 x 8192 in 245 (2.24), with scales per row of both operands (twice the vector work) 527 and 278.  The MFMAs are
-// busy 60 % of the time at 1.91 GHz; a product without scales per block reaches 84 % at 1.67 GHz (375 us), so that what bounds
-// both is power.  Without its loads this kernel takes 382 us, with loads from the L1 408, from the L2 430; without the scales' vector work 421.
-// Of short k: 147456 x 128 x 512 41 us, in fp32 78 (4.1 TB/s; a fill in the same tiles 5.5): loads 7, products 4 and 4.5 rounds of tiles that take 5.
+// vector work then hides behind each other's MFMAs, and two buffers of both operands fill the LDS.  8192^3 in 477 us (2.30 PFLOP/s),
+// 8192 x 4096 x 8192 in 250 (2.20), with scales per row of both operands (twice the vector work) 546 and 282.  The MFMAs were
+// busy 60 % of the time at 1.91 GHz, when it did not look at the range of the scales yet (457 us); a product without scales per block reaches 84 % at 1.67 GHz (375 us), so that what bounds
+// both is power.  Without its loads that kernel took 382 us, with loads from the L1 408, from the L2 430; without the scales' vector work 421.
+// Of short k: 147456 x 128 x 512 42 us among other passes (39 by itself), in fp32 77 (4.1 TB/s; a fill in the same tiles 5.5): loads 7, products 4 and 4.5 rounds
+// of tiles that take 5.
 template <int TM, int TN, int WM, int WN, int NB, bool PAIRS> struct Fp8Tile {
   static constexpr int W = WM * WN, MT = TM / WM / 16;
   static constexpr int kSa = 0, kSb = 1024, kB = 2048, kA = kB + TN * 128, kStage = kA + TM * 128;
@@ -562,7 +563,7 @@ __global__ __launch_bounds__(256) void fp8_join_kernel(const float* __restrict__
 
 // Up to 16 rows of a: bound by reading b once, and by the time a read takes.  A workgroup has 16 rows of b; its waves share the blocks of k,
 // read b straight into registers (16 rows of whole 128-byte lines) and a from the caches, four blocks before the first is multiplied,
-// and add their sums in LDS, in their order.  1 x 2048 x 8192 5.0 us, 1 x 4096 x 4096 4.8 (3.4 TB/s, 2.5 us of it the launch's).  With more
+// and add their sums in LDS, in their order.  1 x 2048 x 8192 5.3 us, 1 x 4096 x 4096 5.5 (3.0 TB/s, 2.5 us of it the launch's).  With more
 // rows the caches are asked for a too often (37 x 4096 x 4096 12 us in three groups of 16, as tiles with a split of k 8).
 template <typename O>
 __global__ __launch_bounds__(512) void fp8_few_rows_product(Fp8Args p) {
@@ -619,7 +620,7 @@ __global__ __launch_bounds__(512) void fp8_few_rows_product(Fp8Args p) {
 // ---- which kernel ---------------------------------------------------------------------------------------
 namespace {
 // The tile kernels, as (tile; workgroups that the 256 compute units hold at once; what a round of these takes per block of k, in units of 10 ns,
-// with 16-bit and with fp32 results; 0: not built).  The one whose rounds take least is chosen.  us at k = 4096, in the order below (the fifth without
+// with 16-bit and with fp32 results; 0: not built).  The one whose rounds take least is chosen.  us at k = 4096 when the costs were set, in the order below (the fifth without
 // fp32): 1024 x 1024 12.0 / 16.6 / 22.9 / 41.6, 1280^2 22.0 / 19.0 / 22.9, 1536^2 32.6 / 32.3 / 23.4 / 41.8, 2048^2 - / - / 26.4 / 44.7 / 38.1 /
 // 50.4, 2560^2 - / - / 46.6 / 48.9 / 38.5 / 50.5, 3328^2 68.5 / 83.1 / 72.3 / 51.3 for the last four, 4608^2 135 / 136 / 114 / 106;
 // 192 x 256 and 256 x 256 3328^2 52 / 56, 4608^2 92 / 106, 6144 x 4096 105 / 106, 8192 x 8192 270 / 230 (whole rounds are bound by power); fp32 1024^2 16.6 /
@@ -637,7 +638,7 @@ struct Fp8Plan {
   int splits;
 };
 Fp8Plan fp8_plan(int64_t m, int64_t n, int64_t blocks, bool square, bool wide) {
-  // (16 x 4096 x 4096 7.2 us, as tiles 9.9; 16 x 8192 x 1024 9.5 and 9.3)
+  // (16 x 4096 x 4096 6.6 us, as tiles 9.9; 16 x 8192 x 1024 9.5 and 9.3)
   // (and a launch has fewer than 2^32 threads: 512 per 16 columns)
   if (m <= 16 && square && n <= 1 << 26) return {kFewRows, 1};
   auto tiles = [&](int tm, int tn) { return ((m + tm - 1) / tm) * ((n + tn - 1) / tn); };

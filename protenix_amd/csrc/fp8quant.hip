@@ -5,7 +5,7 @@
 // a workgroup holds a tile of 128 x 128 in its registers, 8 x 8 per thread, takes the largest magnitudes of its rows among 16 lanes
 // and of its columns through LDS, and turns the bytes round in LDS, from where the transposed rows go out in whole lines of 128 bytes.
 // 16384 x 4096 bf16 both ways 55.7 us among other passes (4.9 TB/s; a plain copy 5.8), its rows alone 39 (5.3); 8192 x 4096 square both
-// ways 28.7.  On the same tensors again 49, with tiles in one run per XCD 51 - 56, with loads past the caches 49 - 55.
+// ways 29.1, in a training pass 35.  On the same tensors again 49, with tiles in one run per XCD 51 - 56, with loads past the caches 49 - 55.
 #include "fp8.h"
 #include "dropout.h"
 #include "kernels.h"

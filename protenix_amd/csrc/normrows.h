@@ -66,8 +66,8 @@ template <int G, int WAVES> struct Lay {
   X(1, 1, 1, true) X(1, 1, 1, false) X(2, 1, 1, false) X(4, 1, 1, false) X(8, 1, 1, false) X(16, 1, 1, false) X(32, 1, 1, false) \
   X(64, 1, 1, false) X(64, 8, 1, false) X(64, 16, 1, false) X(64, 16, 2, false)
 // A launch's shape: workgroups of one row in the fewest waves that hold it, or of four waves of rows, which walk the rows: the same number
-// of them for each of the 256 compute units, the first that holds `waves` waves, or as have `turns` turns to make (but one per compute
-// unit).  (With 256 waves / w of them, whatever that leaves over, some units walk two shares one after the other: 64 M bf16
+// of them for each of the 256 compute units, the first that holds `waves` waves, or as many fewer as leave each `turns` turns (rounded
+// down, so that some make one more; but one per compute unit).  (With 256 waves / w of them, whatever that leaves over, some units walk two shares one after the other: 64 M bf16
 // elements in rows of 2800 backward 4.0 TB/s, with 2 for each 4.9.)
 struct Walk {
   int groups, threads;
