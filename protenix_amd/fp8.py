@@ -24,7 +24,7 @@ class Fp8Tensor:
 
     values: float8_e4m3fn [*, k]; scales: float32 [*, ceil(k / 128)], or with square=True [ceil(n / 128), ceil(k / 128)] for values
     [n, k].  `values` and `scales` are views of the operand's own memory, whose layout is the kernels'; what is given here is copied
-    into that layout (weights of a checkpoint, say)."""
+    into that layout (weights of a checkpoint, say), without a graph: tensors inside one are refused, leaves taken."""
 
     def __init__(self, values: torch.Tensor, scales: torch.Tensor, *, square: bool = False) -> None:
         ops._dev(values, "values")
@@ -88,8 +88,8 @@ def _matrix(x: torch.Tensor, name: str) -> torch.Tensor:
 
 
 def quantize_fp8(x: torch.Tensor, *, square: bool = False, along: Union[int, Tuple[int, int]] = -1):
-    """x [*, k], float32, bfloat16 or float16, in 8-bit blocks (no gradient: a rounding has none; `linear_fp8` has its own.  So an x
-    on the way of one, forward-mode or of a graph, is refused; a leaf is taken, a weight to serve, and gets nothing from here).
+    """x [*, k], float32, bfloat16 or float16, in 8-bit blocks.  No gradient: a rounding has none, and `linear_fp8` has its own.  So an x
+    inside a graph, or a dual tensor, is refused; a leaf (a weight to serve) is taken, and gets none from here.
 
     along=-1: blocks of the last dimension; the result has x's shape.  along=-2: the rows (all other dimensions as one) are the axis
     that will be summed over: the transposed matrix [k, rows], blocks along its rows.  along=(-1, -2): both, from one pass over x.

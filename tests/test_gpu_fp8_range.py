@@ -11,7 +11,7 @@ F32, BF16 = torch.float32, torch.bfloat16
 # one of every kernel, with 16-bit and with fp32 results: few rows, 64 x 64 with and without parts of k and with two workgroups to a compute unit,
 # 128 x 128 with k shared by waves and without, 256 x 128, 192 x 256, 256 x 256; odd sizes, more tiles than workgroups, a last block of a few columns
 SHAPES = [(1, 300, 70), (13, 4300, 33), (70, 300, 130), (130, 9001, 100), (1300, 300, 1290), (1600, 200, 1500), (2500, 260, 2600), (2900, 130, 2950),
-          (3000, 300, 4100), (4500, 300, 4600)]
+          (3000, 300, 4100), (4500, 300, 4600), (100, 130, 40000), (100000, 130, 100), (4100, 260, 4100), (8300, 130, 8300)]
 
 
 def _operand(rows, cols, square, seed, odd):
